@@ -32,6 +32,18 @@ class StatusC(Structure):
     _fields_ = [("code", c_uint32), ("block", c_uint32), ("site", c_uint32), ("aux", c_uint32)]
 
 
+class PagedCacheC(Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p),
+                ("k_strides", c_int64 * 3), ("v_strides", c_int64 * 3), ("k_scale_strides", c_int64 * 3),
+                ("v_scale_strides", c_int64 * 3), ("k_global", c_float), ("v_global", c_float), ("format", c_int),
+                ("num_pages", c_int), ("kv_heads", c_int), ("page_size", c_int), ("head_dim", c_int)]
+
+
+class PagedBatchC(Structure):
+    _fields_ = [("block_table", c_void_p), ("block_table_pitch", c_int64), ("cu_q", c_void_p), ("kv_lens", c_void_p),
+                ("batch", c_int), ("max_pages", c_int), ("max_q_len", c_int)]
+
+
 # name -> (restype, argtypes); the single source of truth for the Python side of the ABI.
 SIGNATURES = {
     "b200tile_abi_version": (c_int, []),
@@ -87,6 +99,15 @@ SIGNATURES = {
                                                POINTER(c_int64), c_int64, POINTER(c_int64), c_void_p]),
     "b200tile_splitk_reduce_merge": (c_int, [c_char_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                              POINTER(c_int64), c_int64, POINTER(c_int64), c_void_p]),
+    "b200tile_paged_kv_append": (c_int, [c_char_p, POINTER(PagedCacheC), POINTER(PagedBatchC), c_void_p, c_void_p,
+                                         c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, POINTER(c_int64),
+                                         POINTER(c_int64), POINTER(c_int64), POINTER(c_int64), c_void_p]),
+    "b200tile_paged_kv_gather": (c_int, [c_char_p, POINTER(PagedCacheC), POINTER(PagedBatchC), c_void_p, c_void_p,
+                                         c_int, POINTER(c_int64), POINTER(c_int64), c_void_p]),
+    "b200tile_paged_attention_workspace_bytes": (c_uint64, [POINTER(PagedCacheC), POINTER(PagedBatchC), c_int]),
+    "b200tile_paged_attention": (c_int, [c_char_p, POINTER(PagedCacheC), POINTER(PagedBatchC), c_void_p, c_void_p,
+                                         c_int, c_int, POINTER(c_int64), POINTER(c_int64), c_float, c_int, c_int,
+                                         c_float, c_void_p, c_uint64, c_void_p]),
     "b200tile_linear_fp8_blk128": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_char_p,
                                            c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64,
                                            c_int64, c_float, c_void_p]),

@@ -1,0 +1,908 @@
+// Attention of few query rows over a paged key/value cache, 16-bit or NVFP4 (every length, mask and row count is
+// handled here; sequences with many rows go to fmha_paged_tile.cu).
+//
+//   o_i = sum_j softmax_j(score(q_i . k_j)) v_j      over the keys j < len that the masks of row i leave
+//
+// Query rows are packed per K/V head (row = token * group + head of the group) in blocks of 8 or 16, so that a K/V row
+// is read once for all heads that share it.  What bounds it is HBM: each cached byte is used for `group` rows only.
+//
+// Work split.  One worker is ONE WARP.  Sequence b has steps(b) steps of 16 keys, an item is (sequence, row block, K/V
+// head), and the steps of all items form one line that is cut into equal runs, one per worker.  Lengths may be as
+// uneven as they like: every warp of the machine reads the same number of bytes, whatever the batch looks like, and
+// nothing about the lengths has to be known on the host (a captured graph may be replayed with other lengths).  A run
+// that holds whole items writes their output; a run that holds part of an item writes (m, l, O) in 32 bits, at most
+// two such parts per worker, and the merge kernel adds the parts of an item in the order of the workers.  No atomics
+// and no state between launches: the same call gives the same bits.
+//
+// Inside a worker the products are transposed, S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16): the 16 rows of the
+// instruction are keys (or head dimensions) and its 8 columns the query rows, so 8 rows fill it; the usual orientation
+// would multiply a block half full of zeros and hold twice the accumulators.  P^T comes from S^T by movmatrix.
+#include <math_constants.h>
+
+#include <algorithm>
+
+#include "paged_common.cuh"
+
+namespace b200 {
+namespace {
+
+__device__ __forceinline__ void ldm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint32_t mat_trans(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+template <bool F16>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* desc, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(desc), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(ok ? BYTES : 0)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
+  uint32_t r;
+  asm("{.reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t;}" : "=r"(r) : "r"(two_bytes));
+  return r;
+}
+// Nibble I of each 16-bit half -> f16 with the value e2m1 * 2^-14: the sign goes to bit 15, exponent and mantissa to
+// bits 9..11, where f16 reads them with a bias that is 14 too small and its subnormals are e2m1's.
+template <int I>
+__device__ __forceinline__ uint32_t e2m1_to_f16x2(uint32_t w) {
+  const uint32_t sgn = I == 3 ? w : w << (12 - 4 * I);
+  const uint32_t mag = I == 3 ? w >> 3 : w << (9 - 4 * I);
+  return (sgn & 0x80008000u) | (mag & 0x0E000E00u);
+}
+
+constexpr int STEP = 16;             // keys per step
+constexpr float F4_UNIT = 128.0f;    // the FP4 operands are held as value * 2^-7 (scale * 2^7 stays finite in f16)
+
+struct SplitParams {
+  PagedBatch batch;
+  const uint16_t* q;
+  uint16_t* out;
+  long long q_ts, q_hs, o_ts, o_hs;
+  ScoreParams score;
+  int kv_heads, group, causal, window, row_limit;
+  float out_scale;                   // FP4: v_global * 2^7 (the score carries k_global * 2^7)
+  float* part;
+  int4* desc;
+  long long part_floats;
+  int workers, by_item, rb_max;
+  int min_steps;
+  // FP4 operands: byte strides
+  const uint8_t *k, *v, *ks, *vs;
+  long long k_st[3], v_st[3], ks_st[3], vs_st[3];
+};
+
+// Steps of one item of the sequence, from key step `base`; 0 for a sequence without rows here, and at least 1 for one
+// with rows (a row that sees no key still has to be written).
+struct SeqWork {
+  SeqView s;
+  int base, steps, rbs;
+};
+template <int RB>
+__device__ __forceinline__ SeqWork seq_work(const SplitParams& p, int b) {
+  SeqWork w;
+  w.s = seq_view(p.batch, b);
+  const int rows = w.s.n * p.group;
+  w.rbs = rows > p.row_limit ? 0 : (rows + RB - 1) / RB;
+  int lo = 0, hi = w.s.len;
+  if (p.causal) {
+    hi = min(hi, w.s.pos0 + w.s.n);
+    if (p.window > 0) lo = max(0, w.s.pos0 - p.window + 1);
+  }
+  w.base = hi > lo ? lo / STEP : 0;
+  w.steps = hi > lo ? (hi + STEP - 1) / STEP - w.base : 1;
+  return w;
+}
+
+// Per-warp state of one part of an item: the block's rows as this lane sees them.
+template <int NT>
+struct RowMask {
+  int lo[NT][2], hi[NT][2];          // visible keys of query rows 8 nt + 2t and + 1
+  int lo_min, hi_max;                // over the block
+  int lo_max, hi_min;                // a step inside [lo_max, hi_min) needs no mask
+};
+template <int NT>
+__device__ __forceinline__ RowMask<NT> row_mask(const SplitParams& p, const SeqView& s, int rb, int lane) {
+  RowMask<NT> m;
+  const int rows = s.n * p.group, first = rb * 8 * NT;
+  auto range = [&](int row, int& lo, int& hi) {
+    lo = 0;
+    hi = s.len;
+    if (p.causal) {
+      const int pos = s.pos0 + row / p.group;
+      hi = min(hi, pos + 1);
+      if (p.window > 0) lo = max(0, pos - p.window + 1);
+    }
+  };
+  int l0, h0, l1, h1;
+  range(first, l0, h0);
+  range(min(rows, first + 8 * NT) - 1, l1, h1);
+  m.lo_min = l0;
+  m.lo_max = l1;
+  m.hi_min = h0;
+  m.hi_max = h1;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int row = first + nt * 8 + (lane & 3) * 2 + j;
+      if (row < rows) range(row, m.lo[nt][j], m.hi[nt][j]);
+      else { m.lo[nt][j] = 0; m.hi[nt][j] = 0; }
+    }
+  return m;
+}
+
+// The online softmax of one step: s[nt] holds S^T (keys g and g + 8, rows 2t and 2t + 1 of block nt) and becomes the
+// B operand of O^T += V^T P^T.  Maximum and sum in 32 bits.  P is handed over as a 16-bit value plus the 16-bit rest
+// of it (HILO): the rounding of P alone would put an error as large as the output's own rounding beside it, and the
+// second product costs nothing next to the loads.
+template <bool F16, int NT, int DT, bool CAP, bool HILO>
+__device__ __forceinline__ void softmax_step(const SplitParams& p, const RowMask<NT>& rm, int key0, int lane, bool ragged,
+                                             float (&s)[NT][4], float (&m_run)[NT][2], float (&l_run)[NT][2],
+                                             float (&o)[DT][NT][4], uint32_t (&pb)[NT][2], uint32_t (&pl)[NT][2]) {
+  const int g = lane >> 2;
+  float alpha[NT][2];
+  bool grew = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x = paged_score<CAP>(p.score, s[nt][e]);
+      if (ragged) {
+        const int key = key0 + g + (e >> 1) * 8;
+        if (key < rm.lo[nt][e & 1] || key >= rm.hi[nt][e & 1]) x = -CUDART_INF_F;
+      }
+      s[nt][e] = x;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float mx = fmaxf(s[nt][j], s[nt][2 + j]);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      const float m_new = fmaxf(m_run[nt][j], mx);
+      const float m_use = m_new == -CUDART_INF_F ? 0.0f : m_new;   // nothing seen yet: keep the arguments finite
+      alpha[nt][j] = paged_ex2(m_run[nt][j] - m_use);
+      grew |= m_new != m_run[nt][j];
+      m_run[nt][j] = m_new;
+      const float a = paged_ex2(s[nt][j] - m_use), b = paged_ex2(s[nt][2 + j] - m_use);
+      s[nt][j] = a;
+      s[nt][2 + j] = b;
+      l_run[nt][j] = l_run[nt][j] * alpha[nt][j] + (a + b);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t hi = paged_pack16<F16>(s[nt][2 * h], s[nt][2 * h + 1]);
+      pb[nt][h] = mat_trans(hi);
+      if (HILO) {
+        const float2 f = paged_unpack16<F16>(hi);
+        pl[nt][h] = mat_trans(paged_pack16<F16>(s[nt][2 * h] - f.x, s[nt][2 * h + 1] - f.y));
+      }
+    }
+  }
+  if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        o[i][nt][0] *= alpha[nt][0];
+        o[i][nt][1] *= alpha[nt][1];
+        o[i][nt][2] *= alpha[nt][0];
+        o[i][nt][3] *= alpha[nt][1];
+      }
+  }
+}
+
+// One 16-bit K/V step: TMA boxes of 16 keys x 64 elements with the 128-byte swizzle, in a ring of the warp's own.
+template <int D>
+struct Core16 {
+  static constexpr int WARPS = 8, STAGES = 3;
+  static constexpr int HALVES = D / 64, BOX = STEP * 128, TILE = HALVES * BOX, STAGE = 2 * TILE;
+  static constexpr int RING = WARPS * STAGES * STAGE;
+  static constexpr int SMEM = 1024 + RING + WARPS * STAGES * 8 + 16;
+};
+// One FP4 step: 16 keys of packed values and scales copied with cp.async into a ring of the warp's own.
+template <int D>
+struct Core4 {
+  static constexpr int WARPS = 12, STAGES = 4;
+  static constexpr int ROW = D / 2, SROW = D / 16;
+  static constexpr int STAGE = 2 * STEP * (ROW + SROW);
+  static constexpr int RING = WARPS * STAGES * STAGE;
+  static constexpr int SMEM = RING;
+};
+
+// Finds the first piece of work of every worker of the CTA.  s_sum[i] = steps of the sequences before chunk i.
+template <int RB, int THREADS>
+__device__ __forceinline__ long long block_line(const SplitParams& p, long long* s_sum) {
+  const int per = (p.batch.batch + THREADS - 1) / THREADS;
+  long long mine = 0;
+  for (int b = threadIdx.x * per; b < min(p.batch.batch, (int)(threadIdx.x + 1) * per); ++b) {
+    const SeqWork w = seq_work<RB>(p, b);
+    mine += (long long)w.rbs * p.kv_heads * w.steps;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += up;
+  }
+  __shared__ long long s_warp[32];
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  long long before = 0, total = 0;
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += s_warp[w];
+    total += s_warp[w];
+  }
+  s_sum[threadIdx.x] = before + inc - mine;
+  __syncthreads();
+  return total;
+}
+
+template <int D, bool F16, int NT, bool CAP, bool FP4>
+__global__ void __launch_bounds__(FP4 ? 384 : 256, 1)
+fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                        const __grid_constant__ SplitParams p, uint32_t* status) {
+  using C16 = Core16<D>;
+  using C4 = Core4<D>;
+  constexpr int WARPS = FP4 ? C4::WARPS : C16::WARPS, THREADS = WARPS * 32;
+  constexpr int STAGES = FP4 ? C4::STAGES : C16::STAGES;
+  constexpr int DT = D / 16, RB = 8 * NT;
+  constexpr bool HILO = !FP4 || F16;         // bf16 output over f16 probabilities needs no second product
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ long long s_sum[THREADS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  // the merge kernel may be scheduled now; it waits for this grid before it reads
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const uint32_t base = FP4 ? smem_u32(smem_raw) : (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint32_t ring, bars = 0;
+  WaitCtx wctx{nullptr, status};
+  if constexpr (!FP4) {
+    ring = base + warp * (STAGES * C16::STAGE);
+    bars = base + C16::RING + warp * STAGES * 8;
+    volatile uint32_t* abort_flag =
+        reinterpret_cast<volatile uint32_t*>(smem_raw + (base - smem_u32(smem_raw)) + C16::RING + WARPS * STAGES * 8);
+    wctx.abort_flag = abort_flag;
+    if (threadIdx.x == 0) *abort_flag = 0;
+    if (lane == 0) {
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+      for (int s = 0; s < STAGES; ++s) mbar_init(bars + s * 8, 1);
+      fence_mbar_init();
+    }
+  } else {
+    ring = base + warp * (STAGES * C4::STAGE);
+  }
+  const long long total = block_line<RB, THREADS>(p, s_sum);
+
+  const int wid = warp * gridDim.x + blockIdx.x;     // neighbouring runs on different SMs
+  long long per = (total + p.workers - 1) / p.workers;
+  if (per < p.min_steps) per = p.min_steps;
+  long long u = (long long)wid * per;
+  const long long u_end = min(total, u + per);
+  if (!p.by_item && lane == 0) p.desc[wid] = make_int4(0, 0, 0, 0);
+  if (u >= u_end) return;
+
+  // the sequence that holds step u: binary search over the chunks, then along the chunk
+  int c_lo = 0, c_hi = THREADS - 1;
+  while (c_lo < c_hi) {
+    const int mid = (c_lo + c_hi + 1) >> 1;
+    if (s_sum[mid] <= u) c_lo = mid;
+    else c_hi = mid - 1;
+  }
+  const int chunk = (p.batch.batch + THREADS - 1) / THREADS;
+  int b = c_lo * chunk;
+  long long line = s_sum[c_lo];                       // first step of sequence b
+  SeqWork sw = seq_work<RB>(p, b);
+  while (line + (long long)sw.rbs * p.kv_heads * sw.steps <= u) {
+    line += (long long)sw.rbs * p.kv_heads * sw.steps;
+    if (++b >= p.batch.batch) return;
+    sw = seq_work<RB>(p, b);
+  }
+
+  uint32_t ring_at = 0;        // steps taken through the ring since the kernel began (stage and phase of the next)
+  const int rowk = ((lane >> 3) & 1) * 8 + (lane & 7), rowv = (lane >> 4) * 8 + (lane & 7);
+  const int ck = lane >> 4, cv = (lane >> 3) & 1;
+
+  while (u < u_end) {
+    const long long rel = u - line;
+    const int item = (int)(rel / sw.steps);
+    const int st0 = (int)(rel - (long long)item * sw.steps);
+    const int st1 = (int)min((long long)sw.steps, st0 + (u_end - u));
+    const int rb = item / p.kv_heads, h = item - rb * p.kv_heads;
+    const SeqView& sv = sw.s;
+    const int rows = min(RB, sv.n * p.group - rb * RB);
+    const RowMask<NT> rm = row_mask<NT>(p, sv, rb, lane);
+    // the part's key steps, cut to what the block's rows can see
+    const int k0 = max(sw.base + st0, rm.lo_min / STEP);
+    const int k1 = rm.hi_max > rm.lo_min ? min(sw.base + st1, (rm.hi_max + STEP - 1) / STEP) : 0;
+    const int nk = k1 - k0;
+
+    // page numbers of 32 steps at a time, one per lane
+    int pages = 0, pages_at = 0;
+    auto fetch_pages = [&](int i) {
+      pages_at = i;
+      const int key = (k0 + i + lane) * STEP;
+      pages = i + lane < nk ? page_of(p.batch, b, key, status) : 0;
+    };
+    const int slot_mask = (1 << p.batch.page_shift) - 1;
+    auto issue = [&](int i) {
+      if (i >= nk) return;                            // warp-uniform
+      if (i - pages_at >= 32) fetch_pages(i);
+      const int pg = __shfl_sync(0xffffffffu, pages, i - pages_at);
+      const int slot = ((k0 + i) * STEP) & slot_mask;
+      const uint32_t dst = ring + ((ring_at + i) % STAGES) * (FP4 ? C4::STAGE : C16::STAGE);
+      if constexpr (!FP4) {
+        const uint32_t bar = bars + ((ring_at + i) % STAGES) * 8;
+        if (lane == 0) {
+          mbar_expect_tx(bar, C16::STAGE);
+#pragma unroll
+          for (int x = 0; x < C16::HALVES; ++x) {
+            tma_load_4d(dst + x * C16::BOX, &tmK, bar, x * 64, slot, h, pg);
+            tma_load_4d(dst + C16::TILE + x * C16::BOX, &tmV, bar, x * 64, slot, h, pg);
+          }
+        }
+      } else {
+        const bool ok = pg < p.batch.num_pages;
+        const int pgc = ok ? pg : 0;                  // a valid address for the copies that read nothing
+        const uint8_t* kp = p.k + (long long)pgc * p.k_st[0] + (long long)h * p.k_st[1] + (long long)slot * p.k_st[2];
+        const uint8_t* vp = p.v + (long long)pgc * p.v_st[0] + (long long)h * p.v_st[1] + (long long)slot * p.v_st[2];
+        constexpr int CH = C4::ROW / 16;              // 16-byte chunks per row
+#pragma unroll
+        for (int c = 0; c < STEP * CH / 32; ++c) {
+          const int x = c * 32 + lane, r = x / CH, o = (x % CH) * 16;
+          cp_async_16(dst + r * C4::ROW + o, kp + r * p.k_st[2] + o, ok);
+          cp_async_16(dst + STEP * C4::ROW + r * C4::ROW + o, vp + r * p.v_st[2] + o, ok);
+        }
+        const int r = lane & 15;
+        const bool is_v = lane >= 16;
+        const uint8_t* sp = is_v ? p.vs + (long long)pgc * p.vs_st[0] + (long long)h * p.vs_st[1] + (slot + r) * p.vs_st[2]
+                                 : p.ks + (long long)pgc * p.ks_st[0] + (long long)h * p.ks_st[1] + (slot + r) * p.ks_st[2];
+        cp_async_small<C4::SROW>(dst + 2 * STEP * C4::ROW + (is_v ? STEP * C4::SROW : 0) + r * C4::SROW, sp, ok);
+      }
+    };
+    if (nk > 0) {
+      fetch_pages(0);
+#pragma unroll
+      for (int s = 0; s < STAGES - (FP4 ? 1 : 0); ++s) {
+        issue(s);
+        if (FP4) asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+    }
+
+    // Q^T as the B operand: query row 8 nt + g, two adjacent dimensions per register (FP4: the pairs that the K words
+    // unpack to, see below; the row is brought to a power of two near 1 first, so that f16 holds it whatever its size)
+    uint32_t qb[NT][DT][2];
+    float q_unit[NT][2];                              // what the rows 2t, 2t + 1 were divided by
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = rb * RB + nt * 8 + g;
+      const int tok = row / p.group;
+      const bool ok = tok < sv.n;
+      const uint16_t* qr = p.q + (long long)(sv.q0 + (ok ? tok : 0)) * p.q_ts +
+                           (long long)(h * p.group + (ok ? row - tok * p.group : 0)) * p.q_hs;
+      if constexpr (!FP4) {
+#pragma unroll
+        for (int ks = 0; ks < DT; ++ks)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            qb[nt][ks][x] = ok ? *reinterpret_cast<const uint32_t*>(qr + ks * 16 + x * 8 + 2 * t) : 0u;
+      } else {
+        // lane t holds dimensions [D/4 t, D/4 (t + 1)); word w of 8 of them gives k-steps 2w and 2w + 1
+        float f[D / 4];
+        float mx = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t w = ok ? *reinterpret_cast<const uint32_t*>(qr + t * (D / 4) + 2 * i) : 0u;
+          const float2 v = paged_unpack16<F16>(w);
+          f[2 * i] = v.x;
+          f[2 * i + 1] = v.y;
+          mx = fmaxf(mx, fmaxf(fabsf(v.x), fabsf(v.y)));
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        // power of two with mx * inv in [1, 2); rows that are zero, infinite or NaN keep factor 1
+        const uint32_t e = __float_as_uint(mx) & 0x7f800000u;
+        const bool scaled = e > (27u << 23) && e < (227u << 23);
+        const float inv = scaled ? __uint_as_float((254u << 23) - e) : 1.0f;
+        const float unit = scaled ? __uint_as_float(e) : 1.0f;
+#pragma unroll
+        for (int w = 0; w < D / 32; ++w)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)                 // nibbles x and x + 4 of the word
+            qb[nt][2 * w + (x >> 1)][x & 1] = pack_f16x2(f[w * 8 + x] * inv, f[w * 8 + x + 4] * inv);
+        // rows 2t and 2t + 1 sit in the lanes with g = 2t, 2t + 1
+        q_unit[nt][0] = __shfl_sync(0xffffffffu, unit, 8 * t);
+        q_unit[nt][1] = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
+      }
+    }
+
+    float m_run[NT][2], l_run[NT][2], o[DT][NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m_run[nt][0] = m_run[nt][1] = -CUDART_INF_F;
+      l_run[nt][0] = l_run[nt][1] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < DT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
+    }
+
+    for (int i = 0; i < nk; ++i) {
+      const int key0 = (k0 + i) * STEP;
+      const bool ragged = key0 < rm.lo_max || key0 + STEP > rm.hi_min;
+      const uint32_t slot_at = (ring_at + i) % STAGES;
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+      // keys of this lane's V operand that no row of the block sees hold anything at all: cleared bit by bit
+      uint32_t vm0 = 0xffffffffu, vm1 = 0xffffffffu;
+      const bool clear = key0 < rm.lo_min || key0 + STEP > rm.hi_max;
+      if (clear) {
+        auto seen = [&](int key) { return key >= rm.lo_min && key < rm.hi_max; };
+        const int ka = key0 + 2 * t;
+        vm0 = (seen(ka) ? 0xffffu : 0u) | (seen(ka + 1) ? 0xffff0000u : 0u);
+        vm1 = (seen(ka + 8) ? 0xffffu : 0u) | (seen(ka + 9) ? 0xffff0000u : 0u);
+      }
+      uint32_t pb[NT][2], pl[NT][2];
+      if constexpr (!FP4) {
+        if (!__all_sync(0xffffffffu, mbar_wait(wctx, bars + slot_at * 8, ((ring_at + i) / STAGES) & 1u, 90u + slot_at))) {
+          // gave up: the copies still in flight get their (bounded) time before the shared memory goes
+          for (int x = 1; x < STAGES && i + x < nk; ++x)
+            mbar_wait(wctx, bars + ((ring_at + i + x) % STAGES) * 8, ((ring_at + i + x) / STAGES) & 1u, 99u);
+          return;
+        }
+        const uint32_t sK = ring + slot_at * C16::STAGE, sV = sK + C16::TILE;
+#pragma unroll
+        for (int ks = 0; ks < DT; ++ks) {
+          uint32_t a[4];
+          ldm_x4(sK + (ks >> 2) * C16::BOX + rowk * 128 + ((((ks & 3) * 2 + ck) ^ (lane & 7)) << 4), a);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(s[nt], a, qb[nt][ks][0], qb[nt][ks][1]);
+        }
+        softmax_step<F16, NT, DT, CAP, HILO>(p, rm, key0, lane, ragged, s, m_run, l_run, o, pb, pl);
+#pragma unroll
+        for (int c = 0; c < DT; ++c) {
+          uint32_t a[4];
+          ldm_x4_trans(sV + (c >> 2) * C16::BOX + rowv * 128 + ((((c & 3) * 2 + cv) ^ (lane & 7)) << 4), a);
+          if (clear) {
+            a[0] &= vm0;
+            a[1] &= vm0;
+            a[2] &= vm1;
+            a[3] &= vm1;
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_16816<F16>(o[c][nt], a, pb[nt][0], pb[nt][1]);
+            mma_16816<F16>(o[c][nt], a, pl[nt][0], pl[nt][1]);
+          }
+        }
+        __syncwarp();                                 // every lane is done with the slot before it is filled again
+        issue(i + STAGES);
+      } else {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        __syncwarp();
+        issue(i + STAGES - 1);                        // into the slot that the last step was done with
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const uint32_t sK = ring + slot_at * C4::STAGE, sV = sK + STEP * C4::ROW;
+        const uint32_t sKs = sV + STEP * C4::ROW, sVs = sKs + STEP * C4::SROW;
+        // K: keys g and g + 8, D/4 dimensions of each (D/8 bytes), one scale per two words
+        constexpr int WORDS = D / 32;
+        uint32_t wk[2][WORDS];
+        uint32_t sc[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t at = sK + (g + 8 * x) * C4::ROW + t * (D / 8);
+          if constexpr (WORDS == 4)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(wk[x][0]), "=r"(wk[x][1]), "=r"(wk[x][2]), "=r"(wk[x][3]) : "r"(at));
+          else
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(wk[x][0]), "=r"(wk[x][1]) : "r"(at));
+          uint32_t two;                               // scales of this lane's dimensions
+          if constexpr (WORDS == 4) {
+            asm volatile("{.reg .b16 h; ld.shared.b16 h, [%1]; cvt.u32.u16 %0, h;}"
+                         : "=r"(two) : "r"(sKs + (g + 8 * x) * C4::SROW + t * 2));
+          } else {
+            asm volatile("{.reg .b16 h; ld.shared.u8 h, [%1]; cvt.u32.u16 %0, h;}"
+                         : "=r"(two) : "r"(sKs + (g + 8 * x) * C4::SROW + t));
+          }
+          sc[x] = hmul2(e4m3x2_to_f16x2(two), 0x58005800u);   // * 2^7
+        }
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {
+          uint32_t f0[4], f1[4];
+          const uint32_t s0 = __byte_perm(sc[0], sc[0], w >= 2 ? 0x3232 : 0x1010);
+          const uint32_t s1 = __byte_perm(sc[1], sc[1], w >= 2 ? 0x3232 : 0x1010);
+          f0[0] = hmul2(e2m1_to_f16x2<0>(wk[0][w]), s0);
+          f0[1] = hmul2(e2m1_to_f16x2<1>(wk[0][w]), s0);
+          f0[2] = hmul2(e2m1_to_f16x2<2>(wk[0][w]), s0);
+          f0[3] = hmul2(e2m1_to_f16x2<3>(wk[0][w]), s0);
+          f1[0] = hmul2(e2m1_to_f16x2<0>(wk[1][w]), s1);
+          f1[1] = hmul2(e2m1_to_f16x2<1>(wk[1][w]), s1);
+          f1[2] = hmul2(e2m1_to_f16x2<2>(wk[1][w]), s1);
+          f1[3] = hmul2(e2m1_to_f16x2<3>(wk[1][w]), s1);
+          const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_16816<true>(s[nt], a0, qb[nt][2 * w][0], qb[nt][2 * w][1]);
+            mma_16816<true>(s[nt], a1, qb[nt][2 * w + 1][0], qb[nt][2 * w + 1][1]);
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] *= q_unit[nt][e & 1];
+        softmax_step<true, NT, DT, CAP, HILO>(p, rm, key0, lane, ragged, s, m_run, l_run, o, pb, pl);
+        // V: dimensions [D/8 g, D/8 (g + 1)) of keys 2t, 2t + 1, 2t + 8, 2t + 9; the halves of two keys' words side by
+        // side give (key, key + 1) pairs of one dimension per nibble.  Row m of tile c <-> dimension D/8 g + 2c (+ 1).
+        constexpr int VW = D / 64;                    // words per key
+        uint32_t wv[4][VW], sb[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int key = 2 * t + (x & 1) + (x >> 1) * 8;
+          const uint32_t at = sV + key * C4::ROW + g * (D / 16);
+          if constexpr (VW == 2)
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(wv[x][0]), "=r"(wv[x][1]) : "r"(at));
+          else
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wv[x][0]) : "r"(at));
+          const uint32_t sat = sVs + key * C4::SROW + g * (D / 8) / 16;
+          asm volatile("{.reg .b16 h; ld.shared.u8 h, [%1]; cvt.u32.u16 %0, h;}" : "=r"(sb[x]) : "r"(sat));
+        }
+        // a masked key's scale may be a NaN pattern: the mask clears the product, not the factor
+        const uint32_t sv0 = hmul2(e4m3x2_to_f16x2(sb[0] | (sb[1] << 8)), 0x58005800u);
+        const uint32_t sv1 = hmul2(e4m3x2_to_f16x2(sb[2] | (sb[3] << 8)), 0x58005800u);
+#pragma unroll
+        for (int w = 0; w < VW; ++w)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t sel = half ? 0x7632u : 0x5410u;
+            const uint32_t x0 = __byte_perm(wv[0][w], wv[1][w], sel), x1 = __byte_perm(wv[2][w], wv[3][w], sel);
+            uint32_t f0[4], f1[4];
+            f0[0] = hmul2(e2m1_to_f16x2<0>(x0), sv0) & vm0;
+            f0[1] = hmul2(e2m1_to_f16x2<1>(x0), sv0) & vm0;
+            f0[2] = hmul2(e2m1_to_f16x2<2>(x0), sv0) & vm0;
+            f0[3] = hmul2(e2m1_to_f16x2<3>(x0), sv0) & vm0;
+            f1[0] = hmul2(e2m1_to_f16x2<0>(x1), sv1) & vm1;
+            f1[1] = hmul2(e2m1_to_f16x2<1>(x1), sv1) & vm1;
+            f1[2] = hmul2(e2m1_to_f16x2<2>(x1), sv1) & vm1;
+            f1[3] = hmul2(e2m1_to_f16x2<3>(x1), sv1) & vm1;
+#pragma unroll
+            for (int c2 = 0; c2 < 2; ++c2) {
+              const uint32_t a[4] = {f0[2 * c2], f0[2 * c2 + 1], f1[2 * c2], f1[2 * c2 + 1]};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_16816<true>(o[(w * 2 + half) * 2 + c2][nt], a, pb[nt][0], pb[nt][1]);
+                if (HILO) mma_16816<true>(o[(w * 2 + half) * 2 + c2][nt], a, pl[nt][0], pl[nt][1]);
+              }
+            }
+          }
+      }
+    }
+    if (FP4 && nk > 0) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+    }
+    if (nk > 0) ring_at += nk;
+
+    // ---- the part's result ----
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], 4);
+        l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], 8);
+        l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], 16);
+      }
+    const bool whole = st0 == 0 && st1 == sw.steps;
+    if (whole) {
+      float inv[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)   // a row that saw nothing is 0; NaN stays NaN
+          inv[nt][j] = l_run[nt][j] == 0.0f ? 0.0f : (FP4 ? p.out_scale : 1.0f) / l_run[nt][j];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int row = rb * RB + nt * 8 + g;
+        const int tok = row / p.group;
+        uint16_t* orow = p.out + (long long)(sv.q0 + tok) * p.o_ts + (long long)(h * p.group + row - tok * p.group) * p.o_hs;
+#pragma unroll
+        for (int c = 0; c < DT; ++c) {
+          // (dimension, rows 2t, 2t + 1) -> (row g, lanes' dimensions 2t, 2t + 1 of the tile's eight)
+          const uint32_t a = mat_trans(paged_pack16<F16>(o[c][nt][0] * inv[nt][0], o[c][nt][1] * inv[nt][1]));
+          const uint32_t d2 = mat_trans(paged_pack16<F16>(o[c][nt][2] * inv[nt][0], o[c][nt][3] * inv[nt][1]));
+          if (nt * 8 + g < rows) {
+            if constexpr (!FP4) {
+              *reinterpret_cast<uint32_t*>(orow + c * 16 + 2 * t) = a;
+              *reinterpret_cast<uint32_t*>(orow + c * 16 + 8 + 2 * t) = d2;
+            } else {
+              // tile row m stands for dimension D/8 m + 2c, row m + 8 for the next one
+              *reinterpret_cast<uint32_t*>(orow + (D / 8) * (2 * t) + 2 * c) = __byte_perm(a, d2, 0x5410);
+              *reinterpret_cast<uint32_t*>(orow + (D / 8) * (2 * t + 1) + 2 * c) = __byte_perm(a, d2, 0x7632);
+            }
+          }
+        }
+      }
+    } else {
+      const int slot = st0 == 0 ? 1 : 0;              // an item's first part, or the continuation of an earlier worker's
+      float* dst = p.part + ((long long)wid * 2 + slot) * p.part_floats;
+#pragma unroll
+      for (int c = 0; c < DT; ++c)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          reinterpret_cast<float4*>(dst)[(c * NT + nt) * 32 + lane] =
+              make_float4(o[c][nt][0], o[c][nt][1], o[c][nt][2], o[c][nt][3]);
+      float* ml = dst + DT * NT * 128;
+      if (g == 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            ml[nt * 8 + 2 * t + j] = m_run[nt][j];
+            ml[RB + nt * 8 + 2 * t + j] = l_run[nt][j];
+          }
+      }
+    }
+    if (st0 == 0 && lane == 0) {
+      const long long rest = line + (long long)(item + 1) * sw.steps - u_end;    // steps left to the next workers
+      const int parts = whole ? 0 : 1 + (int)((rest + per - 1) / per);
+      const long long at = p.by_item ? ((long long)b * p.rb_max + rb) * p.kv_heads + h : wid;
+      if (p.by_item || parts) p.desc[at] = make_int4(parts, wid, b, rb * p.kv_heads + h);
+    }
+    u += st1 - st0;
+    if (u >= line + (long long)sw.rbs * p.kv_heads * sw.steps) {
+      line += (long long)sw.rbs * p.kv_heads * sw.steps;
+      do {
+        if (++b >= p.batch.batch) return;
+        sw = seq_work<RB>(p, b);
+      } while (sw.rbs == 0);
+    }
+  }
+}
+
+// Adds the parts of the items that were cut: O = sum w_i O_i / sum w_i l_i with w_i = exp2(m_i - max m).  The parts
+// are stored the way the worker held them (one float4 per lane and 16 x 8 tile), so a warp adds one tile with
+// full-width loads; PW warps share the parts of a tile and are added through shared memory in a fixed order.
+template <int D, bool F16, int NT, bool FP4, int PW>
+__global__ void __launch_bounds__(256) fmha_paged_merge_kernel(const __grid_constant__ SplitParams p) {
+  constexpr int DT = D / 16, RB = 8 * NT, CT = 8 / PW;
+  __shared__ float4 s_o[8][NT][32];
+  __shared__ float s_ml[8][NT][2][4][2];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (p.by_item) {
+    // items that do not exist in this launch have no descriptor
+    const int b = blockIdx.x / (p.rb_max * p.kv_heads), rb = (blockIdx.x / p.kv_heads) % p.rb_max;
+    if (rb >= seq_work<RB>(p, b).rbs) return;
+  }
+  const int4 d = p.desc[blockIdx.x];
+  if (d.x == 0) return;
+  const int pw = warp % PW, c = blockIdx.y * CT + warp / PW;
+  const int b = d.z, rb = d.w / p.kv_heads, h = d.w % p.kv_heads;
+  float m[NT][2], l[NT][2], o[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt][0] = m[nt][1] = -CUDART_INF_F;
+    l[nt][0] = l[nt][1] = 0.0f;
+    o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.0f;
+  }
+  auto add = [&](int nt, const float (&pm)[2], const float (&plx)[2], const float4& v) {
+    const float vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float mn = fmaxf(m[nt][j], pm[j]);
+      const float mu = mn == -CUDART_INF_F ? 0.0f : mn;
+      const float wa = paged_ex2(m[nt][j] - mu), wb = paged_ex2(pm[j] - mu);
+      m[nt][j] = mn;
+      l[nt][j] = l[nt][j] * wa + plx[j] * wb;
+      o[nt][j] = o[nt][j] * wa + vv[j] * wb;
+      o[nt][2 + j] = o[nt][2 + j] * wa + vv[2 + j] * wb;
+    }
+  };
+  if (c < DT) {
+#pragma unroll 4
+    for (int i = pw; i < d.x; i += PW) {
+      const float* src = p.part + ((long long)(d.y + i) * 2 + (i == 0 ? 1 : 0)) * p.part_floats;
+      const float* ml = src + DT * NT * 128;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float4 v = reinterpret_cast<const float4*>(src)[(c * NT + nt) * 32 + lane];
+        const float2 pm = *reinterpret_cast<const float2*>(ml + nt * 8 + 2 * t);
+        const float2 pl = *reinterpret_cast<const float2*>(ml + RB + nt * 8 + 2 * t);
+        const float a[2] = {pm.x, pm.y}, q[2] = {pl.x, pl.y};
+        add(nt, a, q, v);
+      }
+    }
+  }
+  if (PW > 1) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      s_o[warp][nt][lane] = make_float4(o[nt][0], o[nt][1], o[nt][2], o[nt][3]);
+      if (g == 0) {
+        s_ml[warp][nt][0][t][0] = m[nt][0];
+        s_ml[warp][nt][0][t][1] = m[nt][1];
+        s_ml[warp][nt][1][t][0] = l[nt][0];
+        s_ml[warp][nt][1][t][1] = l[nt][1];
+      }
+    }
+    __syncthreads();
+    if (pw != 0) return;
+    for (int w = 1; w < PW; ++w)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float a[2] = {s_ml[warp + w][nt][0][t][0], s_ml[warp + w][nt][0][t][1]};
+        const float q[2] = {s_ml[warp + w][nt][1][t][0], s_ml[warp + w][nt][1][t][1]};
+        add(nt, a, q, s_o[warp + w][nt][lane]);
+      }
+  }
+  if (c >= DT) return;
+  const SeqView sv = seq_view(p.batch, b);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const float i0 = l[nt][0] == 0.0f ? 0.0f : (FP4 ? p.out_scale : 1.0f) / l[nt][0];
+    const float i1 = l[nt][1] == 0.0f ? 0.0f : (FP4 ? p.out_scale : 1.0f) / l[nt][1];
+    const uint32_t a = mat_trans(paged_pack16<F16>(o[nt][0] * i0, o[nt][1] * i1));
+    const uint32_t d2 = mat_trans(paged_pack16<F16>(o[nt][2] * i0, o[nt][3] * i1));
+    const int row = rb * RB + nt * 8 + g;
+    const int tok = row / p.group;
+    if (tok >= sv.n) continue;
+    uint16_t* orow = p.out + (long long)(sv.q0 + tok) * p.o_ts + (long long)(h * p.group + row - tok * p.group) * p.o_hs;
+    if constexpr (!FP4) {
+      *reinterpret_cast<uint32_t*>(orow + c * 16 + 2 * t) = a;
+      *reinterpret_cast<uint32_t*>(orow + c * 16 + 8 + 2 * t) = d2;
+    } else {
+      *reinterpret_cast<uint32_t*>(orow + (D / 8) * (2 * t) + 2 * c) = __byte_perm(a, d2, 0x5410);
+      *reinterpret_cast<uint32_t*>(orow + (D / 8) * (2 * t + 1) + 2 * c) = __byte_perm(a, d2, 0x7632);
+    }
+  }
+}
+
+template <int D, bool F16, int NT, bool CAP, bool FP4>
+int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
+  using C16 = Core16<D>;
+  using C4 = Core4<D>;
+  constexpr int SMEM = FP4 ? C4::SMEM : C16::SMEM;
+  constexpr int THREADS = (FP4 ? C4::WARPS : C16::WARPS) * 32;
+  const b200h::DeviceInfo* di = b200h::device_info();
+  if (!di) return B200_ERR_CUDA;
+  const b200tile_paged_cache& c = *a.cache;
+  SplitParams p = {};
+  p.batch = a.batch;
+  p.q = static_cast<const uint16_t*>(a.q);
+  p.out = static_cast<uint16_t*>(a.out);
+  p.q_ts = a.q_ts; p.q_hs = a.q_hs; p.o_ts = a.o_ts; p.o_hs = a.o_hs;
+  p.score = a.score;
+  p.kv_heads = c.kv_heads;
+  p.group = a.q_heads / c.kv_heads;
+  p.causal = a.causal;
+  p.window = a.window;
+  p.row_limit = a.row_limit;
+  p.part = static_cast<float*>(a.workspace);
+  p.part_floats = (long long)plan.part_floats;
+  p.desc = reinterpret_cast<int4*>(static_cast<char*>(a.workspace) + plan.desc_off);
+  p.workers = plan.workers;
+  p.by_item = plan.by_item;
+  p.rb_max = (int)((std::min<long long>((long long)a.batch.max_q * p.group, a.row_limit) + 8 * NT - 1) / (8 * NT));
+  p.min_steps = 2;
+  CUtensorMap tmK = {}, tmV = {};
+  if constexpr (FP4) {
+    p.score.scale_log2 *= c.k_global * F4_UNIT;
+    p.score.cap_arg *= c.k_global * F4_UNIT;
+    p.out_scale = c.v_global * F4_UNIT;
+    p.k = static_cast<const uint8_t*>(c.k);
+    p.v = static_cast<const uint8_t*>(c.v);
+    p.ks = static_cast<const uint8_t*>(c.k_scales);
+    p.vs = static_cast<const uint8_t*>(c.v_scales);
+    for (int i = 0; i < 3; ++i) {
+      p.k_st[i] = c.k_strides[i]; p.v_st[i] = c.v_strides[i];
+      p.ks_st[i] = c.k_scale_strides[i]; p.vs_st[i] = c.v_scale_strides[i];
+    }
+  } else {
+    const CUtensorMapDataType dt = F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    if (int rc = b200h::encode_tmap_pages(&tmK, dt, c.k, D, c.page_size, c.kv_heads, c.num_pages, c.k_strides, 64, STEP))
+      return rc;
+    if (int rc = b200h::encode_tmap_pages(&tmV, dt, c.v, D, c.page_size, c.kv_heads, c.num_pages, c.v_strides, 64, STEP))
+      return rc;
+  }
+  auto kern = fmha_paged_split_kernel<D, F16, NT, CAP, FP4>;
+  static b200h::DeviceOnce attr_done;
+  if (!attr_done.test(di->ordinal)) {
+    B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    attr_done.set(di->ordinal);
+  }
+  kern<<<plan.ctas, THREADS, SMEM, a.stream>>>(tmK, tmV, p, di->status);
+  B200_CUDA_CHECK(cudaGetLastError());
+  // few items with many parts: all eight warps of a CTA share the parts of one tile; else a warp per tile
+  const unsigned x = (unsigned)(plan.by_item ? plan.items : plan.workers);
+  const bool wide = x * (D / 16) <= 8u * di->sm_count;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(x, wide ? D / 16 : 1);
+  cfg.blockDim = dim3(256);
+  cfg.stream = a.stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (wide) B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fmha_paged_merge_kernel<D, F16, NT, FP4, 8>, p));
+  else B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fmha_paged_merge_kernel<D, F16, NT, FP4, 1>, p));
+  return B200_OK;
+}
+
+}  // namespace
+}  // namespace b200
+
+// The plan depends on sizes the host knows; SM count 148 is the part's (fewer SMs run the same CTAs in turn).
+PagedSplitPlan b200_paged_split_plan(int format, int head_dim, int kv_heads, int batch, long long rows,
+                                     long long max_keys) {
+  PagedSplitPlan pl;
+  const int warps = format ? 12 : 8;
+  pl.rows_per_block = rows <= 8 ? 8 : 16;
+  const long long rb_max = (rows + pl.rows_per_block - 1) / pl.rows_per_block;
+  pl.items = (long long)batch * rb_max * kv_heads;
+  const long long steps = pl.items * ((max_keys + 15) / 16);
+  pl.ctas = (int)std::max<long long>(1, std::min<long long>(148, (steps + 1) / 2));
+  pl.workers = pl.ctas * warps;
+  pl.by_item = pl.items <= pl.workers;
+  pl.part_floats = (size_t)pl.rows_per_block * (head_dim + 2);
+  pl.desc_off = (size_t)pl.workers * 2 * pl.part_floats * sizeof(float);
+  pl.bytes = pl.desc_off + sizeof(int4) * (size_t)(pl.by_item ? pl.items : pl.workers);
+  return pl;
+}
+
+int b200_paged_split_dispatch(const PagedAttnArgs& a) {
+  using namespace b200;
+  const b200tile_paged_cache& c = *a.cache;
+  const PagedSplitPlan plan =
+      b200_paged_split_plan(c.format, c.head_dim, c.kv_heads, a.batch.batch,
+                            std::min<long long>((long long)a.batch.max_q * (a.q_heads / c.kv_heads), a.row_limit),
+                            (long long)a.batch.max_pages * c.page_size);
+#define B200_PS(D_, F_, N_, C_, Q_) return launch_split<D_, F_, N_, C_, Q_>(a, plan)
+#define B200_PS_CAP(D_, F_, N_, Q_) do { if (a.capped) B200_PS(D_, F_, N_, true, Q_); B200_PS(D_, F_, N_, false, Q_); } while (0)
+#define B200_PS_NT(D_, F_, Q_) do { if (plan.rows_per_block == 8) B200_PS_CAP(D_, F_, 1, Q_); B200_PS_CAP(D_, F_, 2, Q_); } while (0)
+#define B200_PS_FMT(D_, F_) do { if (c.format) B200_PS_NT(D_, F_, true); B200_PS_NT(D_, F_, false); } while (0)
+  if (c.head_dim == 128 && a.dtype == 0) B200_PS_FMT(128, false);
+  if (c.head_dim == 128 && a.dtype == 1) B200_PS_FMT(128, true);
+  if (c.head_dim == 64 && a.dtype == 0) B200_PS_FMT(64, false);
+  if (c.head_dim == 64 && a.dtype == 1) B200_PS_FMT(64, true);
+#undef B200_PS_FMT
+#undef B200_PS_NT
+#undef B200_PS_CAP
+#undef B200_PS
+  return b200h::set_error(B200_ERR_UNSUPPORTED, "paged_attention: no kernel for head_dim %d (64 and 128 are provided)",
+                          c.head_dim);
+}

@@ -97,6 +97,26 @@ int encode_tmap_3d(CUtensorMap* out, CUtensorMapDataType dtype, int elem_bytes, 
   return B200_OK;
 }
 
+int encode_tmap_pages(CUtensorMap* out, CUtensorMapDataType dtype, const void* base, int dim0, int slots, int heads,
+                      int pages, const int64_t strides[3], uint32_t box0, uint32_t box1) {
+  auto fn = get_encode_fn();
+  if (!fn) return set_error(B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  const uint64_t row = (uint64_t)dim0 * 2;
+  uint64_t bytes[3] = {(uint64_t)strides[2] * 2, heads > 1 ? (uint64_t)strides[1] * 2 : row,
+                       pages > 1 ? (uint64_t)strides[0] * 2 : row};
+  if (int rc = check_tma_rules(base, bytes, 3)) return rc;
+  cuuint64_t gdim[4] = {(cuuint64_t)dim0, (cuuint64_t)slots, (cuuint64_t)heads, (cuuint64_t)pages};
+  cuuint64_t gstr[3] = {bytes[0], bytes[1], bytes[2]};
+  cuuint32_t box[4] = {box0, box1, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = fn(out, dtype, 4, const_cast<void*>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(B200_ERR_CUDA, "cuTensorMapEncodeTiled(page pool) failed with CUresult %d (%d pages, %d heads, "
+                     "%d slots, page pitch %llu)", (int)r, pages, heads, slots, (unsigned long long)bytes[2]);
+  return B200_OK;
+}
+
 // ---------------------------------------------------------------------------
 // Device status record + per-device facts.
 // ---------------------------------------------------------------------------

@@ -33,6 +33,11 @@ int encode_tmap_3d(CUtensorMap* out, CUtensorMapDataType dtype, int elem_bytes, 
                    uint64_t stride2_bytes, uint32_t box0, uint32_t box1, uint32_t box2,
                    CUtensorMapSwizzle swizzle);
 
+// Page pool [pages, heads, slots, dim0], any 16-byte strides {page, head, slot} in elements of 2 bytes; the box is
+// box0 elements of `box1` slots of one head of one page.  Extents of 1 take no stride from the caller.
+int encode_tmap_pages(CUtensorMap* out, CUtensorMapDataType dtype, const void* base, int dim0, int slots, int heads,
+                      int pages, const int64_t strides[3], uint32_t box0, uint32_t box1);
+
 // Per-device first-use flag for idempotent set-up (function attributes).  Threads that race may both do
 // the set-up, which is harmless because the calls are idempotent; the flag itself is atomic.
 struct DeviceOnce {

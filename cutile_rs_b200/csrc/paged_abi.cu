@@ -1,0 +1,221 @@
+// Entry points of the paged-cache operators: argument checks, then the dispatchers.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "paged_common.cuh"
+
+using b200h::set_error;
+
+int b200_paged_append_dispatch(int dtype, const b200tile_paged_cache& c, const b200::PagedBatch& batch, const void* q,
+                               const void* k, const void* v, void* q_out, const float* inv_freq, int q_heads, int rot,
+                               const int64_t* qs, const int64_t* ks, const int64_t* vs, const int64_t* qos,
+                               cudaStream_t stream);
+int b200_paged_gather_dispatch(int dtype, const b200tile_paged_cache& c, const b200::PagedBatch& batch, void* k_out,
+                               void* v_out, const int64_t* ks, const int64_t* vs, cudaStream_t stream);
+
+namespace {
+
+bool misaligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+
+int check_dtype(const char* dtype, const char* who, int* dt) {
+  if (!dtype) return set_error(B200TILE_ERR_INVALID, "%s: dtype is null", who);
+  if (!strcmp(dtype, "bf16")) *dt = 0;
+  else if (!strcmp(dtype, "f16")) *dt = 1;
+  else return set_error(B200TILE_ERR_UNSUPPORTED, "%s: unsupported element type '%s'", who, dtype);
+  return B200TILE_OK;
+}
+
+// extents of 1 put no condition on their stride
+int check_pool(const char* who, const char* name, const void* p, const int64_t* st, const int extents[3], int unit,
+               uintptr_t align) {
+  if (!p) return set_error(B200TILE_ERR_INVALID, "%s: the %s pool is null", who, name);
+  bool bad = misaligned(p, align);
+  for (int i = 0; i < 3; ++i) {
+    if (extents[i] > 1 && st[i] <= 0)
+      return set_error(B200TILE_ERR_INVALID, "%s: strides of the %s pool must be positive", who, name);
+    bad |= extents[i] > 1 && st[i] % unit != 0;
+  }
+  if (bad)
+    return set_error(B200TILE_ERR_ALIGN, "%s: the %s pool must be %d-byte aligned with strides that are multiples of %d",
+                     who, name, (int)align, unit);
+  return B200TILE_OK;
+}
+
+int check_cache(const char* who, const b200tile_paged_cache* c) {
+  if (!c) return set_error(B200TILE_ERR_INVALID, "%s: cache is null", who);
+  if (c->format != 0 && c->format != 1)
+    return set_error(B200TILE_ERR_UNSUPPORTED, "%s: cache format %d (0: 16-bit, 1: NVFP4)", who, c->format);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return set_error(B200TILE_ERR_UNSUPPORTED, "%s: head_dim %d (64 and 128 are provided)", who, c->head_dim);
+  if (c->num_pages <= 0 || c->kv_heads <= 0 || c->page_size <= 0)
+    return set_error(B200TILE_ERR_INVALID, "%s: Shape dimensions must be positive", who);
+  if (c->page_size < 16 || (c->page_size & (c->page_size - 1)))
+    return set_error(B200TILE_ERR_UNSUPPORTED, "%s: page_size %d is not a power of two of at least 16", who, c->page_size);
+  const int ext[3] = {c->num_pages, c->kv_heads, c->page_size};
+  const int unit = c->format ? 16 : 8;
+  if (int rc = check_pool(who, "K", c->k, c->k_strides, ext, unit, 16)) return rc;
+  if (int rc = check_pool(who, "V", c->v, c->v_strides, ext, unit, 16)) return rc;
+  if (c->format) {
+    const int row = c->head_dim / 16;
+    if (int rc = check_pool(who, "K scale", c->k_scales, c->k_scale_strides, ext, row, row)) return rc;
+    if (int rc = check_pool(who, "V scale", c->v_scales, c->v_scale_strides, ext, row, row)) return rc;
+    if (!(c->k_global > 0.0f && c->v_global > 0.0f) || !isfinite(c->k_global) || !isfinite(c->v_global))
+      return set_error(B200TILE_ERR_INVALID, "%s: k_global and v_global must be positive and finite", who);
+  }
+  return B200TILE_OK;
+}
+
+int check_batch(const char* who, const b200tile_paged_cache* c, const b200tile_paged_batch* b, int tokens) {
+  if (!b) return set_error(B200TILE_ERR_INVALID, "%s: batch is null", who);
+  if (b->batch < 0 || tokens < 0) return set_error(B200TILE_ERR_INVALID, "%s: batch and tokens must not be negative", who);
+  // without sequences or tokens there is nothing to point to, and nothing to do
+  if (b->batch > 0 && tokens > 0 && (!b->block_table || !b->cu_q || !b->kv_lens))
+    return set_error(B200TILE_ERR_INVALID, "%s: block_table, cu_q and kv_lens are required", who);
+  if (misaligned(b->block_table, 4) || misaligned(b->cu_q, 4) || misaligned(b->kv_lens, 4))
+    return set_error(B200TILE_ERR_ALIGN, "%s: block_table, cu_q and kv_lens must be 4-byte aligned", who);
+  if (b->max_pages <= 0 || b->max_q_len <= 0)
+    return set_error(B200TILE_ERR_INVALID, "%s: max_pages and max_q_len must be positive", who);
+  if (b->block_table_pitch < b->max_pages && b->batch > 1)
+    return set_error(B200TILE_ERR_INVALID, "%s: block_table_pitch is shorter than max_pages", who);
+  if ((long long)b->max_pages * c->page_size > 0x7fffff00LL)
+    return set_error(B200TILE_ERR_UNSUPPORTED, "%s: %d pages of %d exceed 2^31 positions", who, b->max_pages, c->page_size);
+  return B200TILE_OK;
+}
+
+b200::PagedBatch device_batch(const b200tile_paged_cache* c, const b200tile_paged_batch* b, int tokens) {
+  b200::PagedBatch p;
+  p.table = b->block_table;
+  p.cu_q = b->cu_q;
+  p.kv_lens = b->kv_lens;
+  p.table_pitch = b->block_table_pitch;
+  p.batch = b->batch;
+  p.max_pages = b->max_pages;
+  p.num_pages = c->num_pages;
+  p.page_shift = __builtin_ctz((unsigned)c->page_size);
+  p.tokens = tokens;
+  p.max_q = std::min(b->max_q_len, tokens);
+  return p;
+}
+
+int check_rows(const char* who, const char* name, const void* p, const int64_t* st, int tokens, int unit,
+               uintptr_t align) {
+  if ((!p && tokens > 0) || !st) return set_error(B200TILE_ERR_INVALID, "%s: %s and its strides are required", who, name);
+  if (misaligned(p, align) || st[0] % unit || st[1] % unit)
+    return set_error(B200TILE_ERR_ALIGN, "%s: %s must be %d-byte aligned with strides that are multiples of %d", who, name,
+                     (int)align, unit);
+  return B200TILE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200tile_paged_kv_append(const char* dtype, const b200tile_paged_cache* cache, const b200tile_paged_batch* batch,
+                             const void* q, const void* k, const void* v, void* q_out, const float* inv_freq, int tokens,
+                             int q_heads, int rotary_dim, const int64_t q_strides[2], const int64_t k_strides[2],
+                             const int64_t v_strides[2], const int64_t q_out_strides[2], void* cu_stream) {
+  const char* who = "paged_kv_append";
+  int dt;
+  if (int rc = check_dtype(dtype, who, &dt)) return rc;
+  if (int rc = check_cache(who, cache)) return rc;
+  if (int rc = check_batch(who, cache, batch, tokens)) return rc;
+  const int unit = cache->format ? 32 : 16;
+  if (rotary_dim < 0 || rotary_dim > cache->head_dim || rotary_dim % unit)
+    return set_error(B200TILE_ERR_UNSUPPORTED, "%s: rotary_dim %d must be a multiple of %d from 0 to head_dim %d", who,
+                     rotary_dim, unit, cache->head_dim);
+  if (rotary_dim > 0 && !inv_freq) return set_error(B200TILE_ERR_INVALID, "%s: inv_freq is required for a rotation", who);
+  if (misaligned(inv_freq, 4)) return set_error(B200TILE_ERR_ALIGN, "%s: inv_freq must be 4-byte aligned", who);
+  if ((q == nullptr) != (q_out == nullptr))
+    return set_error(B200TILE_ERR_INVALID, "%s: q and q_out are given together or not at all", who);
+  if (q) {
+    if (q_heads <= 0) return set_error(B200TILE_ERR_INVALID, "%s: q_heads must be positive", who);
+    if (int rc = check_rows(who, "q", q, q_strides, tokens, 8, 16)) return rc;
+    if (int rc = check_rows(who, "q_out", q_out, q_out_strides, tokens, 8, 16)) return rc;
+  }
+  if (int rc = check_rows(who, "k", k, k_strides, tokens, 8, 16)) return rc;
+  if (int rc = check_rows(who, "v", v, v_strides, tokens, 8, 16)) return rc;
+  if (tokens == 0 || batch->batch == 0) return B200TILE_OK;
+  return b200_paged_append_dispatch(dt, *cache, device_batch(cache, batch, tokens), q, k, v, q_out, inv_freq, q_heads,
+                                    rotary_dim, q_strides, k_strides, v_strides, q_out_strides,
+                                    static_cast<cudaStream_t>(cu_stream));
+}
+
+int b200tile_paged_kv_gather(const char* dtype, const b200tile_paged_cache* cache, const b200tile_paged_batch* batch,
+                             void* k_out, void* v_out, int tokens, const int64_t k_out_strides[2],
+                             const int64_t v_out_strides[2], void* cu_stream) {
+  const char* who = "paged_kv_gather";
+  int dt;
+  if (int rc = check_dtype(dtype, who, &dt)) return rc;
+  if (int rc = check_cache(who, cache)) return rc;
+  if (int rc = check_batch(who, cache, batch, tokens)) return rc;
+  if (int rc = check_rows(who, "k_out", k_out, k_out_strides, tokens, 8, 16)) return rc;
+  if (int rc = check_rows(who, "v_out", v_out, v_out_strides, tokens, 8, 16)) return rc;
+  if (tokens == 0 || batch->batch == 0) return B200TILE_OK;
+  return b200_paged_gather_dispatch(dt, *cache, device_batch(cache, batch, tokens), k_out, v_out, k_out_strides,
+                                    v_out_strides, static_cast<cudaStream_t>(cu_stream));
+}
+
+uint64_t b200tile_paged_attention_workspace_bytes(const b200tile_paged_cache* cache, const b200tile_paged_batch* batch,
+                                                  int q_heads) {
+  if (!cache || !batch || cache->kv_heads <= 0 || q_heads <= 0 || batch->batch <= 0 || batch->max_pages <= 0 ||
+      batch->max_q_len <= 0 || cache->page_size <= 0 || cache->head_dim <= 0)
+    return 0;
+  return b200_paged_split_plan(cache->format, cache->head_dim, cache->kv_heads, batch->batch,
+                               (long long)batch->max_q_len * (q_heads / cache->kv_heads),
+                               (long long)batch->max_pages * cache->page_size).bytes;
+}
+
+int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cache, const b200tile_paged_batch* batch,
+                             const void* q, void* out, int tokens, int q_heads, const int64_t q_strides[2],
+                             const int64_t out_strides[2], float qk_scale, int causal, int window, float softcap,
+                             void* workspace, uint64_t workspace_bytes, void* cu_stream) {
+  const char* who = "paged_attention";
+  PagedAttnArgs a = {};
+  if (int rc = check_dtype(dtype, who, &a.dtype)) return rc;
+  if (int rc = check_cache(who, cache)) return rc;
+  if (int rc = check_batch(who, cache, batch, tokens)) return rc;
+  if (int rc = check_rows(who, "q", q, q_strides, tokens, 2, 4)) return rc;
+  if (int rc = check_rows(who, "out", out, out_strides, tokens, 2, 4)) return rc;
+  if (q_heads <= 0 || q_heads % cache->kv_heads)
+    return set_error(B200TILE_ERR_INVALID, "%s: q_heads %d must be a positive multiple of kv_heads %d", who, q_heads,
+                     cache->kv_heads);
+  const int group = q_heads / cache->kv_heads;
+  if ((long long)tokens * group > 0x7fffff00LL)
+    return set_error(B200TILE_ERR_UNSUPPORTED, "%s: more than 2^31 query rows per K/V head", who);
+  if (!(qk_scale > 0.0f) || !isfinite(qk_scale))
+    return set_error(B200TILE_ERR_INVALID, "%s: qk_scale must be positive and finite", who);
+  if (!(softcap >= 0.0f) || !isfinite(softcap))
+    return set_error(B200TILE_ERR_INVALID, "%s: softcap must be 0 (none) or positive and finite", who);
+  if (window < 0 || (window > 0 && !causal))
+    return set_error(B200TILE_ERR_INVALID, "%s: window must be 0 (none) or positive, and needs causal", who);
+  if (tokens == 0 || batch->batch == 0) return B200TILE_OK;
+  const uint64_t need = b200tile_paged_attention_workspace_bytes(cache, batch, q_heads);
+  if (!workspace || workspace_bytes < need)
+    return set_error(B200TILE_ERR_INVALID, "%s: a workspace of %llu bytes is required (got %llu)", who,
+                     (unsigned long long)need, (unsigned long long)(workspace ? workspace_bytes : 0));
+  if (misaligned(workspace, 16)) return set_error(B200TILE_ERR_ALIGN, "%s: workspace must be 16-byte aligned", who);
+  a.cache = cache;
+  a.batch = device_batch(cache, batch, tokens);
+  a.q = q;
+  a.out = out;
+  a.q_heads = q_heads;
+  a.q_ts = q_strides[0];
+  a.q_hs = q_strides[1];
+  a.o_ts = out_strides[0];
+  a.o_hs = out_strides[1];
+  const float log2e = 1.4426950408889634f;
+  a.score.scale_log2 = qk_scale * log2e;
+  a.capped = softcap > 0.0f;
+  a.score.cap_arg = a.capped ? 2.0f * log2e * qk_scale / softcap : 0.0f;
+  a.score.cap_out = softcap * log2e;
+  a.causal = causal != 0;
+  a.window = window;
+  a.row_limit = 0x7fffffff;
+  a.workspace = workspace;
+  a.stream = static_cast<cudaStream_t>(cu_stream);
+  return b200_paged_split_dispatch(a);
+}
+
+}  // extern "C"

@@ -19,6 +19,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
+from .paged import PagedBatch, PagedKvCache
 from .tensor import (Grid, GridBound, KernelLaunchError, MappedLaunchPartition, Partition, Tensor,
                      infer_launch_grid)
 
@@ -821,3 +822,126 @@ def linear_nvfp4_prepared(z: Tensor, x: Tensor, y: Tensor, x_scales: Tensor, y_s
     if rc:
         raise KernelLaunchError(lib.b200tile_last_error().decode())
     return z
+
+
+def _paged_rows(who: str, name: str, t: Tensor, tokens: int, heads: int, cache: PagedKvCache) -> None:
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != tokens or shape[1] != heads or shape[2] != cache.head_dim:
+        raise KernelLaunchError(f"{who}: {name} is {shape}, expected [{tokens}, {heads}, {cache.head_dim}]")
+    if t.strides[2] != 1:
+        raise KernelLaunchError(f"{who}: the head vectors of {name} must be contiguous")
+    if t.storage.device != cache.device:
+        raise KernelLaunchError(f"{who}: {name} is on {t.storage.device}, the cache on {cache.device}")
+
+
+def _paged_dtype(who: str, cache: PagedKvCache, tensors) -> str:
+    dt = tensors[0].dtype
+    if any(t.dtype != dt for t in tensors):
+        raise KernelLaunchError(f"{who}: the tensors have different element types {[t.dtype for t in tensors]}")
+    if cache.dtype is not None and cache.dtype != dt:
+        raise KernelLaunchError(f"{who}: the cache holds {cache.dtype}, the tensors {dt}")
+    return dt
+
+
+def _paged_stream(who: str, cache: PagedKvCache, batch: PagedBatch, stream: Optional[torch.cuda.Stream]) -> int:
+    if batch.device != cache.device:
+        raise KernelLaunchError(f"{who}: the batch is on {batch.device}, the cache on {cache.device}")
+    if cache.device.type != "cuda" or torch.cuda.current_device() != cache.device.index:
+        raise KernelLaunchError(f"{who}: the cache is on {cache.device}, which is not the current device")
+    if stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    if stream.device != cache.device:
+        raise KernelLaunchError(f"{who}: the stream is on {stream.device}, the cache on {cache.device}")
+    return stream.cuda_stream
+
+
+def paged_kv_append(cache: PagedKvCache, batch: PagedBatch, k: Tensor, v: Tensor, q: Optional[Tensor] = None,
+                    q_out: Optional[Tensor] = None, inv_freq: Optional[Tensor] = None,
+                    stream: Optional[torch.cuda.Stream] = None) -> None:
+    """Writes the new tokens of ``batch`` into the cache (``b200tile_paged_kv_append``): k, v [tokens, kv_heads, D] go to
+    the slots of their positions, K (and q [tokens, q_heads, D] into ``q_out``, which may be ``q``) rotated by
+    position * inv_freq [rotary_dim / 2] f32 on the way; without ``inv_freq`` nothing is rotated."""
+    who = "paged_kv_append"
+    lib = _lib.load()
+    tokens, heads = k.shape[0], cache.kv_heads
+    _paged_rows(who, "k", k, tokens, heads, cache)
+    _paged_rows(who, "v", v, tokens, heads, cache)
+    tensors, q_heads = [k, v], 0
+    if (q is None) != (q_out is None):
+        raise KernelLaunchError(f"{who}: q and q_out are given together or not at all")
+    if q is not None:
+        q_heads = q.shape[1] if len(q.shape) == 3 else 0
+        _paged_rows(who, "q", q, tokens, q_heads, cache)
+        _paged_rows(who, "q_out", q_out, tokens, q_heads, cache)
+        tensors += [q, q_out]
+    dt = _paged_dtype(who, cache, tensors)
+    rot = 0
+    if inv_freq is not None:
+        if inv_freq.dtype != "f32" or len(inv_freq.shape) != 1 or inv_freq.strides[0] != 1 or \
+                inv_freq.storage.device != cache.device:
+            raise KernelLaunchError(f"{who}: inv_freq must be a contiguous f32 vector on {cache.device}")
+        rot = 2 * inv_freq.shape[0]
+    s = _paged_stream(who, cache, batch, stream)
+    rc = lib.b200tile_paged_kv_append(
+        dt.encode(), cache.c, batch.c, q.cu_deviceptr() if q is not None else None, k.cu_deviceptr(), v.cu_deviceptr(),
+        q_out.cu_deviceptr() if q is not None else None, inv_freq.cu_deviceptr() if rot else None, tokens, q_heads, rot,
+        _i64x2(q.strides[0], q.strides[1]) if q is not None else None, _i64x2(k.strides[0], k.strides[1]),
+        _i64x2(v.strides[0], v.strides[1]), _i64x2(q_out.strides[0], q_out.strides[1]) if q is not None else None, s)
+    if rc:
+        raise KernelLaunchError(lib.b200tile_last_error().decode())
+
+
+def paged_kv_gather(k_out: Tensor, v_out: Tensor, cache: PagedKvCache, batch: PagedBatch,
+                    stream: Optional[torch.cuda.Stream] = None) -> Tuple[Tensor, Tensor]:
+    """The cached rows at the positions of the batch's tokens as k_out, v_out [tokens, kv_heads, D] in 16 bits
+    (``b200tile_paged_kv_gather``); with ``cu_q`` the running sum of ``kv_lens``, every sequence's whole cache."""
+    who = "paged_kv_gather"
+    lib = _lib.load()
+    tokens = k_out.shape[0]
+    _paged_rows(who, "k_out", k_out, tokens, cache.kv_heads, cache)
+    _paged_rows(who, "v_out", v_out, tokens, cache.kv_heads, cache)
+    dt = _paged_dtype(who, cache, [k_out, v_out])
+    s = _paged_stream(who, cache, batch, stream)
+    rc = lib.b200tile_paged_kv_gather(dt.encode(), cache.c, batch.c, k_out.cu_deviceptr(), v_out.cu_deviceptr(), tokens,
+                                      _i64x2(k_out.strides[0], k_out.strides[1]),
+                                      _i64x2(v_out.strides[0], v_out.strides[1]), s)
+    if rc:
+        raise KernelLaunchError(lib.b200tile_last_error().decode())
+    return k_out, v_out
+
+
+def paged_attention_workspace(cache: PagedKvCache, batch: PagedBatch, q_heads: int) -> torch.Tensor:
+    """Scratch for :func:`paged_attention` on a batch of these sizes (whatever its lengths are).  Calls that may run at
+    the same time, and graphs that may be replayed at the same time, need one each."""
+    need = int(_lib.load().b200tile_paged_attention_workspace_bytes(cache.c, batch.c, int(q_heads)))
+    return torch.empty(max(need, 16), dtype=torch.uint8, device=cache.device)
+
+
+def paged_attention(out: Tensor, q: Tensor, cache: PagedKvCache, batch: PagedBatch, qk_scale: float,
+                    causal: bool = True, window: int = 0, softcap: float = 0.0,
+                    workspace: Optional[torch.Tensor] = None, stream: Optional[torch.cuda.Stream] = None) -> Tensor:
+    """Attention of every token of a ragged batch (decode steps, prompt chunks, or both) over its sequence's cached rows
+    (``b200tile_paged_attention``): q, out [tokens, q_heads, D].  A token sees the keys up to its own position (all of
+    the sequence's with ``causal=False``), of those the last ``window`` if that is not 0; ``softcap`` c > 0 puts the
+    scaled scores through c tanh(s / c).  Without a ``workspace`` (uint8, from :func:`paged_attention_workspace`) one is
+    taken from the torch caching allocator."""
+    who = "paged_attention"
+    lib = _lib.load()
+    tokens = q.shape[0]
+    q_heads = q.shape[1] if len(q.shape) == 3 else 0
+    _paged_rows(who, "q", q, tokens, q_heads, cache)
+    _paged_rows(who, "out", out, tokens, q_heads, cache)
+    dt = _paged_dtype(who, cache, (q, out))
+    s = _paged_stream(who, cache, batch, stream)
+    if workspace is None:
+        with torch.cuda.stream(stream or torch.cuda.current_stream()):
+            workspace = paged_attention_workspace(cache, batch, q_heads)
+    elif workspace.device != cache.device or not workspace.is_contiguous():
+        raise KernelLaunchError(f"{who}: the workspace must be contiguous on {cache.device}")
+    rc = lib.b200tile_paged_attention(dt.encode(), cache.c, batch.c, q.cu_deviceptr(), out.cu_deviceptr(), tokens, q_heads,
+                                      _i64x2(q.strides[0], q.strides[1]), _i64x2(out.strides[0], out.strides[1]),
+                                      qk_scale, int(causal), window, softcap, workspace.data_ptr(),
+                                      workspace.numel() * workspace.element_size(), s)
+    if rc:
+        raise KernelLaunchError(lib.b200tile_last_error().decode())
+    return out

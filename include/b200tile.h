@@ -55,9 +55,10 @@ typedef struct b200tile_config {
 
 /* Device status record written by bounded waits inside the kernels. */
 typedef struct b200tile_status_t {
-  uint32_t code;  /* 0 = ok, 1 = a wait gave up, 3 = a grouped-GEMM group broke the 16-byte rule and was skipped */
+  uint32_t code;  /* 0 = ok, 1 = a wait gave up, 3 = a grouped-GEMM group broke the 16-byte rule and was skipped,
+                   * 4 = a block table named a page outside its pool */
   uint32_t block; /* blockIdx.x of the CTA that recorded it */
-  uint32_t site;  /* which wait (code 1); index of the offending group (code 3) */
+  uint32_t site;  /* which wait (code 1); index of the offending group (code 3) or sequence (code 4) */
   uint32_t aux;
 } b200tile_status_t;
 
@@ -342,6 +343,103 @@ B200TILE_API int b200tile_splitk_reduce_merge(const char* dtype, const void* att
                                               int num_kv_splits, const int64_t att_strides[2],
                                               int64_t lse_head_stride, const int64_t out_strides[2],
                                               void* cu_stream);
+
+/* ---- paged key/value cache ---------------------------------------------------------------- */
+
+/* Serving many sequences out of one pool of pages.  The reference keeps one dense cache per sequence
+ * ([kv_heads, MAX_SEQ, D], cutile-kernels/src/kv_cache.rs) and moves blocks between pools
+ * (experimental/kvbm.rs); it has no attention over pages, so these entry points extend the families
+ * `qk_norm_rope_kv_*` and `fmha_*` above rather than replace a kernel.
+ *
+ * A pool holds K or V as [num_pages, kv_heads, page_size, head_dim]; the strides say how that lies in
+ * memory (a pool stored [pages, slots, heads, D] is the same pool with other strides).
+ *   format 0   elements of the call's dtype; strides in elements, multiples of 8
+ *   format 1   NVFP4: two e2m1 codes per byte (low nibble first) and one f8e4m3fn scale per 16 values, the
+ *              operand format of b200tile_linear_nvfp4; value = code * scale * k_global (v_global).
+ *              Strides in BYTES: of k / v multiples of 16, of the scale pools multiples of head_dim / 16
+ *   head_dim   64 or 128, contiguous; page_size a power of two >= 16
+ * Pools are 16-byte aligned, the scale pools head_dim / 16 bytes.  The struct is read during the call only. */
+typedef struct b200tile_paged_cache {
+  void* k;
+  void* v;
+  void* k_scales; /* format 1 */
+  void* v_scales;
+  int64_t k_strides[3]; /* page, head, slot */
+  int64_t v_strides[3];
+  int64_t k_scale_strides[3];
+  int64_t v_scale_strides[3];
+  float k_global, v_global; /* format 1: positive */
+  int format;
+  int num_pages, kv_heads, page_size, head_dim;
+} b200tile_paged_cache;
+
+/* The sequences of a call.  The arrays are DEVICE memory and are read when the kernels run, so a captured
+ * graph can be replayed with other lengths and pages.
+ *   cu_q         i32 [batch + 1], ascending: sequence b owns the token rows [cu_q[b], cu_q[b+1])
+ *   kv_lens      i32 [batch]: length of every sequence in the cache, its new tokens INCLUDED.  Token i of
+ *                sequence b has position kv_lens[b] - (cu_q[b+1] - cu_q[b]) + i
+ *   block_table  i32 [batch, max_pages], rows `block_table_pitch` apart: page of positions
+ *                [j * page_size, (j + 1) * page_size); entries at or behind the sequence's length are not read
+ *   max_q_len    upper bound of cu_q[b+1] - cu_q[b]: attention computes no more rows of a sequence
+ * Contents cannot be checked by the call; the kernels keep to the tensors whatever they find: token rows
+ * outside every sequence are left as they are, positions outside [0, max_pages * page_size) are not written,
+ * and a page number outside the pool is recorded as status code 4 (site = sequence, aux = page), reads as zeros and
+ * is not written. */
+typedef struct b200tile_paged_batch {
+  const int32_t* block_table;
+  int64_t block_table_pitch;
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  int batch, max_pages, max_q_len;
+} b200tile_paged_batch;
+
+/* Rotary embedding of Q and K and the cache write for every new token of a ragged batch (the paged form of
+ * b200tile_qk_norm_rope_kv, without its norm):
+ *     theta = position * inv_freq[i], i in [0, rotary_dim / 2); y as in b200tile_rope_seq with D = rotary_dim
+ *     q_out[t] = rotated q[t];  K slot of the position = rotated k[t];  V slot = v[t]
+ * Dimensions from rotary_dim on are copied.  theta is taken in 64 bits: far positions keep their angle, where
+ * a 32-bit product is off by 2^-24 of it.  Format 1 writes, per 16 values, the scale e4m3(amax / (6 * global))
+ * and the codes e2m1(y / (scale * global)), ties to even, saturating; y is not rounded to 16 bits before.  A block
+ * cannot hold infinities or NaN: they become its largest code.
+ *   q [tokens, q_heads, D] or NULL (then q_out is NULL too), k / v [tokens, kv_heads, D]; strides {token, head} in
+ *   elements, multiples of 8; all tensors 16-byte aligned.  `q_out` may be `q`.
+ *   rotary_dim  0 (inv_freq NULL: no rotation) or a multiple of 16 (format 1: 32) up to D; inv_freq f32
+ *   [rotary_dim / 2]. */
+B200TILE_API int b200tile_paged_kv_append(const char* dtype, const b200tile_paged_cache* cache,
+                                          const b200tile_paged_batch* batch, const void* q, const void* k,
+                                          const void* v, void* q_out, const float* inv_freq, int tokens, int q_heads,
+                                          int rotary_dim, const int64_t q_strides[2], const int64_t k_strides[2],
+                                          const int64_t v_strides[2], const int64_t q_out_strides[2],
+                                          void* cu_stream);
+
+/* The cached rows at the positions of the batch's tokens, as 16-bit values: k_out, v_out [tokens, kv_heads, D].  With
+ * cu_q the running sum of kv_lens that is every sequence's whole cache, e.g. to hand a prefix to another pool or to
+ * b200tile_fmha_fwd.  Positions outside the cache read as zeros.  Strides {token, head} in elements, multiples of
+ * 8; outputs 16-byte aligned. */
+B200TILE_API int b200tile_paged_kv_gather(const char* dtype, const b200tile_paged_cache* cache,
+                                          const b200tile_paged_batch* batch, void* k_out, void* v_out, int tokens,
+                                          const int64_t k_out_strides[2], const int64_t v_out_strides[2],
+                                          void* cu_stream);
+
+/* Attention of every token over its sequence's cache, decode steps and prompt chunks in one ragged batch:
+ *     out[t, h] = sum_j softmax_j(s_j) v[j, h / group],   s_j = qk_scale * q[t, h] . k[j, h / group],
+ * with softcap c > 0:  s_j -> c * tanh(s_j / c).  Keys j < kv_lens[b]; causal: also j <= position of t, and with
+ * window w > 0 j > position - w.  A row that sees no key is 0.  fp32 statistics and sums.
+ *   q, out     [tokens, q_heads, D], strides {token, head} in elements, multiples of 2; 4-byte aligned
+ *   qk_scale   positive
+ *   workspace  DEVICE scratch of b200tile_paged_attention_workspace_bytes(...) bytes for the same cache and batch
+ *              (sizes only, not contents), 16-byte aligned; nothing in it outlives the call.  Calls that may overlap
+ *              on the device must not share one, nor graphs that may be replayed at the same time
+ * Cached rows at or behind kv_lens[b] and rows before every window of a block of queries are never looked at: they may hold anything, NaN
+ * included.  A NaN or infinity in V at a key that some token of the sequence sees may also reach other tokens of the
+ * same sequence in the call (it is multiplied by a probability of 0). */
+B200TILE_API uint64_t b200tile_paged_attention_workspace_bytes(const b200tile_paged_cache* cache,
+                                                               const b200tile_paged_batch* batch, int q_heads);
+B200TILE_API int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cache,
+                                          const b200tile_paged_batch* batch, const void* q, void* out, int tokens,
+                                          int q_heads, const int64_t q_strides[2], const int64_t out_strides[2],
+                                          float qk_scale, int causal, int window, float softcap, void* workspace,
+                                          uint64_t workspace_bytes, void* cu_stream);
 
 /* z[M,N] = alpha * sum over 128-deep k-blocks of  xs[m,kb] * ys[n/128,kb] * (x_q[m,kb] . y_q[n,kb]),
  * x_q [M,K] and y_q [N,K] in f8e4m3fn (bit convention cuda-core/src/dtype.rs:25-31,223), one fp32

@@ -16,7 +16,8 @@ BEGIN, END = "// --- generated: begin ---\n", "// --- generated: end ---\n"
 
 TYPES = {"int": "c_int", "unsigned": "c_uint", "float": "f32", "double": "f64", "uint64_t": "u64", "int64_t": "i64",
          "uint32_t": "u32", "int32_t": "i32", "void": "c_void", "char": "c_char", "b200tile_config": "B200Config",
-         "b200tile_status_t": "B200Status", "b200tile_compile_options": "B200CompileOptions"}
+         "b200tile_status_t": "B200Status", "b200tile_compile_options": "B200CompileOptions",
+         "b200tile_paged_cache": "B200PagedCache", "b200tile_paged_batch": "B200PagedBatch"}
 
 
 def rust_type(c: str) -> str:

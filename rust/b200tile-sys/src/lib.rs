@@ -54,6 +54,40 @@ pub struct B200Status {
     pub aux: u32,
 }
 
+/// K and V pools of a paged cache; see `b200tile_paged_cache` in the header.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct B200PagedCache {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_scales: *mut c_void,
+    pub v_scales: *mut c_void,
+    pub k_strides: [i64; 3],
+    pub v_strides: [i64; 3],
+    pub k_scale_strides: [i64; 3],
+    pub v_scale_strides: [i64; 3],
+    pub k_global: f32,
+    pub v_global: f32,
+    pub format: c_int,
+    pub num_pages: c_int,
+    pub kv_heads: c_int,
+    pub page_size: c_int,
+    pub head_dim: c_int,
+}
+
+/// The sequences of a call on a paged cache; see `b200tile_paged_batch` in the header.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct B200PagedBatch {
+    pub block_table: *const i32,
+    pub block_table_pitch: i64,
+    pub cu_q: *const i32,
+    pub kv_lens: *const i32,
+    pub batch: c_int,
+    pub max_pages: c_int,
+    pub max_q_len: c_int,
+}
+
 #[link(name = "b200tile")]
 extern "C" {
 // --- generated: begin ---
@@ -132,6 +166,20 @@ extern "C" {
         lse_partial: *const f32, out: *mut c_void, kv_heads: c_int, group: c_int, head_dim: c_int,
         num_kv_splits: c_int, att_strides: *const i64, lse_head_stride: i64, out_strides: *const i64,
         cu_stream: *mut c_void) -> c_int;
+    pub fn b200tile_paged_kv_append(dtype: *const c_char, cache: *const B200PagedCache,
+        batch: *const B200PagedBatch, q: *const c_void, k: *const c_void, v: *const c_void,
+        q_out: *mut c_void, inv_freq: *const f32, tokens: c_int, q_heads: c_int, rotary_dim: c_int,
+        q_strides: *const i64, k_strides: *const i64, v_strides: *const i64, q_out_strides: *const i64,
+        cu_stream: *mut c_void) -> c_int;
+    pub fn b200tile_paged_kv_gather(dtype: *const c_char, cache: *const B200PagedCache,
+        batch: *const B200PagedBatch, k_out: *mut c_void, v_out: *mut c_void, tokens: c_int,
+        k_out_strides: *const i64, v_out_strides: *const i64, cu_stream: *mut c_void) -> c_int;
+    pub fn b200tile_paged_attention_workspace_bytes(cache: *const B200PagedCache,
+        batch: *const B200PagedBatch, q_heads: c_int) -> u64;
+    pub fn b200tile_paged_attention(dtype: *const c_char, cache: *const B200PagedCache,
+        batch: *const B200PagedBatch, q: *const c_void, out: *mut c_void, tokens: c_int, q_heads: c_int,
+        q_strides: *const i64, out_strides: *const i64, qk_scale: f32, causal: c_int, window: c_int,
+        softcap: f32, workspace: *mut c_void, workspace_bytes: u64, cu_stream: *mut c_void) -> c_int;
     pub fn b200tile_linear_fp8_blk128(x: *const c_void, y: *const c_void, x_scales: *const f32,
         y_scales: *const f32, z: *mut c_void, out_dtype: *const c_char, m: c_int, n: c_int, k: c_int,
         ldx: i64, ldy: i64, ldz: i64, ld_xs: i64, ld_ys: i64, alpha: f32, cu_stream: *mut c_void) -> c_int;
