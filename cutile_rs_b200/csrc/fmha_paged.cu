@@ -702,6 +702,7 @@ __global__ void __launch_bounds__(256) fmha_paged_merge_kernel(const __grid_cons
   constexpr int DT = D / 16, RB = 8 * NT, CT = 8 / PW;
   __shared__ float4 s_o[8][NT][32];
   __shared__ float s_ml[8][NT][2][4][2];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the tile kernel of the same call, if there is one
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (p.by_item) {

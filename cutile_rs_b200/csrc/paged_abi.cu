@@ -17,6 +17,9 @@ int b200_paged_gather_dispatch(int dtype, const b200tile_paged_cache& c, const b
 
 namespace {
 
+// Sequences with more query rows (tokens * group) per K/V head than this go to the tile kernel.
+constexpr int kTileRows = 64;
+
 bool misaligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
 
 int check_dtype(const char* dtype, const char* who, int* dt) {
@@ -212,10 +215,14 @@ int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cach
   a.score.cap_out = softcap * log2e;
   a.causal = causal != 0;
   a.window = window;
-  a.row_limit = 0x7fffffff;
   a.workspace = workspace;
   a.stream = static_cast<cudaStream_t>(cu_stream);
-  return b200_paged_split_dispatch(a);
+  const bool tiles = (long long)a.batch.max_q * group > kTileRows && group <= 128 && !misaligned(q, 16) &&
+                     !misaligned(out, 16) && !(a.q_ts % 8) && !(a.q_hs % 8) && !(a.o_ts % 8) && !(a.o_hs % 8) &&
+                     a.q_ts > 0 && a.q_hs > 0;
+  a.row_limit = tiles ? kTileRows : 0x7fffffff;
+  if (int rc = b200_paged_split_dispatch(a)) return rc;
+  return tiles ? b200_paged_tile_dispatch(a) : B200TILE_OK;
 }
 
 }  // extern "C"

@@ -123,3 +123,5 @@ struct PagedSplitPlan {
 PagedSplitPlan b200_paged_split_plan(int format, int head_dim, int kv_heads, int batch, long long rows,
                                      long long max_keys);
 int b200_paged_split_dispatch(const PagedAttnArgs& a);
+// Launched right behind the row-block kernel, whose rows it leaves alone, and runs beside it.
+int b200_paged_tile_dispatch(const PagedAttnArgs& a);

@@ -102,15 +102,17 @@ def attention(p, scale, causal=True, window=0, softcap=0.0):
     Per row: the output's own rounding, half a step of its type; probabilities whose exponents are off by the scores'
     error (a 32-bit dot product of d terms, the score's scale and the exponential's argument: (d + 8) 2^-24 of
     sum |q k| scale, with a cap 2^-19 of it more) and which are handed over in two 16-bit pieces (2^-15 of p; one f16 piece, 2^-11,
-    for bf16 over NVFP4), all against sum p |v|; sums of n terms in 32 bits."""
+    for bf16 over NVFP4; one piece of the type, half a step, for sequences of many rows), all against sum p |v|; sums of n
+    terms in 32 bits."""
     out = torch.zeros(p.tokens, p.heads, p.d, dtype=torch.float64, device="cuda")
     tol = torch.zeros_like(out)
     group = p.heads // p.kvh
     eps = torch.finfo(p.dtype).eps
-    piece = 2.0 ** -11 if p.fmt != "16bit" and p.dtype == torch.bfloat16 else 2.0 ** -15
+    few = 2.0 ** -11 if p.fmt != "16bit" and p.dtype == torch.bfloat16 else 2.0 ** -15
     for b, (n, kv) in enumerate(zip(p.q_lens, p.kv_lens)):
         if n == 0 or kv <= 0:
             continue
+        piece = few if n * group <= 64 else eps / 2
         k, v = p.rows(b, kv)
         pos = torch.arange(kv - n, kv, device="cuda")[:, None]
         key = torch.arange(kv, device="cuda")[None, :]

@@ -82,6 +82,34 @@ def test_prompt_chunks(b200, fmt, d, dtype, heads, kvh, page, window, softcap):
     assert _status(b200)[0] == 0
 
 
+@pytest.mark.parametrize("fmt,d,dtype", [("16bit", 128, F16), ("16bit", 64, BF16), ("nvfp4", 128, BF16), ("nvfp4", 64, F16)])
+@pytest.mark.parametrize("heads,kvh,page,causal,window,softcap", [(8, 1, 64, True, 0, 0.0), (4, 4, 256, True, 700, 0.0),
+                                                                  (10, 2, 16, True, 130, 30.0), (4, 1, 32, False, 0, 0.0),
+                                                                  (4, 2, 128, False, 0, 40.0)])
+def test_long_prompts(b200, fmt, d, dtype, heads, kvh, page, causal, window, softcap):
+    """Several tiles per sequence, ends inside tiles, pages and steps, whole steps before the window, a first step in
+    which early rows see nothing yet; a sequence shorter than its tokens."""
+    p = ref.Problem([1000, 129, 257, 90], [1500, 129, 2999, 33], heads, kvh, d, page, dtype, fmt, "nhd" if page == 64 else "hnd",
+                    seed=heads + page)
+    got = _check(p, d ** -0.5, causal=causal, window=window, softcap=softcap)
+    if causal:
+        assert (got[p.cu[3]:p.cu[3] + 57] == 0).all()
+    assert _status(b200)[0] == 0
+
+
+def test_long_prompts_with_very_negative_scores(b200):
+    """Windows whose first step is empty for late rows, with scores far below zero: the reference of the running
+    exponent must come from keys that are seen."""
+    for fmt in ("16bit", "nvfp4"):
+        p = ref.Problem([400], [900], 2, 1, 128, 16, BF16, fmt, seed=30)
+        p.q.copy_(p.q.abs())
+        if fmt == "16bit":
+            p.pools[0].copy_(-p.pools[0].abs())
+        else:
+            p.pools[0].bitwise_or_(0x88)
+        _check(p, 5.0, window=100)
+
+
 def test_long_context_is_split(b200):
     """A few long sequences: every item is cut over many workers and merged."""
     for fmt in ("16bit", "nvfp4"):
