@@ -99,15 +99,12 @@ SIGNATURES = {
                                                POINTER(c_int64), c_int64, POINTER(c_int64), c_void_p]),
     "b200tile_splitk_reduce_merge": (c_int, [c_char_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                              POINTER(c_int64), c_int64, POINTER(c_int64), c_void_p]),
-    "b200tile_paged_kv_append": (c_int, [c_char_p, POINTER(PagedCacheC), POINTER(PagedBatchC), c_void_p, c_void_p,
-                                         c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, POINTER(c_int64),
-                                         POINTER(c_int64), POINTER(c_int64), POINTER(c_int64), c_void_p]),
-    "b200tile_paged_kv_gather": (c_int, [c_char_p, POINTER(PagedCacheC), POINTER(PagedBatchC), c_void_p, c_void_p,
-                                         c_int, POINTER(c_int64), POINTER(c_int64), c_void_p]),
-    "b200tile_paged_attention_workspace_bytes": (c_uint64, [POINTER(PagedCacheC), POINTER(PagedBatchC), c_int]),
-    "b200tile_paged_attention": (c_int, [c_char_p, POINTER(PagedCacheC), POINTER(PagedBatchC), c_void_p, c_void_p,
-                                         c_int, c_int, POINTER(c_int64), POINTER(c_int64), c_float, c_int, c_int,
-                                         c_float, c_void_p, c_uint64, c_void_p]),
+    # addresses as plain integers (structs and stride pairs included): these calls sit in decode loops
+    "b200tile_paged_kv_append": (c_int, [c_char_p] + [c_void_p] * 7 + [c_int, c_int, c_int] + [c_void_p] * 5),
+    "b200tile_paged_kv_gather": (c_int, [c_char_p] + [c_void_p] * 4 + [c_int, c_void_p, c_void_p, c_void_p]),
+    "b200tile_paged_attention_workspace_bytes": (c_uint64, [c_void_p, c_void_p, c_int]),
+    "b200tile_paged_attention": (c_int, [c_char_p] + [c_void_p] * 4 + [c_int, c_int, c_void_p, c_void_p, c_float, c_int,
+                                                                       c_int, c_float, c_void_p, c_uint64, c_void_p]),
     "b200tile_linear_fp8_blk128": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_char_p,
                                            c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64,
                                            c_int64, c_float, c_void_p]),

@@ -75,17 +75,19 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
   asm("{.reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t;}" : "=r"(r) : "r"(two_bytes));
   return r;
 }
-// Nibble I of each 16-bit half -> f16 with the value e2m1 * 2^-14: the sign goes to bit 15, exponent and mantissa to
-// bits 9..11, where f16 reads them with a bias that is 14 too small and its subnormals are e2m1's.
-template <int I>
-__device__ __forceinline__ uint32_t e2m1_to_f16x2(uint32_t w) {
-  const uint32_t sgn = I == 3 ? w : w << (12 - 4 * I);
-  const uint32_t mag = I == 3 ? w >> 3 : w << (9 - 4 * I);
-  return (sgn & 0x80008000u) | (mag & 0x0E000E00u);
+// The four bytes of w, two e2m1 codes each, as f16 pairs (low nibble in the low half).  One conversion instruction per
+// pair runs at 50 pairs per clock and SM against 22 for shifting the bits into place.
+__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&r)[4]) {
+  asm("{.reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4;"
+      " cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b; cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d;}"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(w));
 }
 
 constexpr int STEP = 16;             // keys per step
-constexpr float F4_UNIT = 128.0f;    // the FP4 operands are held as value * 2^-7 (scale * 2^7 stays finite in f16)
+// Warps per CTA, one CTA per SM.  16-bit, D = 128: 8 rings of 3 x 8 KB fill the shared memory; D = 64 halves the step and
+// doubles the warps.  NVFP4: what the registers allow.
+constexpr int split_warps(bool fp4, int d) { return fp4 ? 12 : d == 64 ? 16 : 8; }
+constexpr float LAZY = 8.0f;         // the running reference of the exponents may lag behind the maximum by this
 
 struct SplitParams {
   PagedBatch batch;
@@ -94,7 +96,7 @@ struct SplitParams {
   long long q_ts, q_hs, o_ts, o_hs;
   ScoreParams score;
   int kv_heads, group, causal, window, row_limit;
-  float out_scale;                   // FP4: v_global * 2^7 (the score carries k_global * 2^7)
+  float out_scale;                   // FP4: v_global (the score carries k_global)
   float* part;
   int4* desc;
   long long part_floats;
@@ -166,18 +168,19 @@ __device__ __forceinline__ RowMask<NT> row_mask(const SplitParams& p, const SeqV
 }
 
 // The online softmax of one step: s[nt] holds S^T (keys g and g + 8, rows 2t and 2t + 1 of block nt) and becomes the
-// B operand of O^T += V^T P^T.  Maximum and sum in 32 bits.  P is handed over as a 16-bit value plus the 16-bit rest
-// of it (HILO): the rounding of P alone would put an error as large as the output's own rounding beside it, and the
-// second product costs nothing next to the loads.
+// B operand of O^T += V^T P^T.  Statistics in 32 bits.  The reference m that is subtracted from the exponents is the
+// same for all lanes of a row and moves only when some score exceeds it by more than 2^8: one vote per step instead of
+// a maximum over eight lanes.  P <= 256 then, and l >= 1 for any row that saw a key.  P is handed over as a 16-bit value
+// plus the 16-bit rest of it (HILO): the rounding of P alone would put an error as large as the output's own rounding
+// beside it, and the second product costs nothing next to the loads.
 template <bool F16, int NT, int DT, bool CAP, bool HILO>
 __device__ __forceinline__ void softmax_step(const SplitParams& p, const RowMask<NT>& rm, int key0, int lane, bool ragged,
                                              float (&s)[NT][4], float (&m_run)[NT][2], float (&l_run)[NT][2],
                                              float (&o)[DT][NT][4], uint32_t (&pb)[NT][2], uint32_t (&pl)[NT][2]) {
   const int g = lane >> 2;
-  float alpha[NT][2];
-  bool grew = false;
+  bool over = false;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float x = paged_score<CAP>(p.score, s[nt][e]);
@@ -186,22 +189,36 @@ __device__ __forceinline__ void softmax_step(const SplitParams& p, const RowMask
         if (key < rm.lo[nt][e & 1] || key >= rm.hi[nt][e & 1]) x = -CUDART_INF_F;
       }
       s[nt][e] = x;
+      over |= x > m_run[nt][e & 1] + LAZY;
     }
+  if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float mx = fmaxf(s[nt][j], s[nt][2 + j]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float m_new = fmaxf(m_run[nt][j], mx);
+        const float alpha = m_new == m_run[nt][j] ? 1.0f : paged_ex2(m_run[nt][j] - m_new);
+        m_run[nt][j] = m_new;
+        l_run[nt][j] *= alpha;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          o[i][nt][j] *= alpha;
+          o[i][nt][2 + j] *= alpha;
+        }
+      }
+  }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      float mx = fmaxf(s[nt][j], s[nt][2 + j]);
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-      const float m_new = fmaxf(m_run[nt][j], mx);
-      const float m_use = m_new == -CUDART_INF_F ? 0.0f : m_new;   // nothing seen yet: keep the arguments finite
-      alpha[nt][j] = paged_ex2(m_run[nt][j] - m_use);
-      grew |= m_new != m_run[nt][j];
-      m_run[nt][j] = m_new;
-      const float a = paged_ex2(s[nt][j] - m_use), b = paged_ex2(s[nt][2 + j] - m_use);
-      s[nt][j] = a;
-      s[nt][2 + j] = b;
-      l_run[nt][j] = l_run[nt][j] * alpha[nt][j] + (a + b);
+      const float m_use = m_run[nt][j] == -CUDART_INF_F ? 0.0f : m_run[nt][j];   // nothing seen yet
+      s[nt][j] = paged_ex2(s[nt][j] - m_use);
+      s[nt][2 + j] = paged_ex2(s[nt][2 + j] - m_use);
+      l_run[nt][j] += s[nt][j] + s[nt][2 + j];
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -213,23 +230,12 @@ __device__ __forceinline__ void softmax_step(const SplitParams& p, const RowMask
       }
     }
   }
-  if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        o[i][nt][0] *= alpha[nt][0];
-        o[i][nt][1] *= alpha[nt][1];
-        o[i][nt][2] *= alpha[nt][0];
-        o[i][nt][3] *= alpha[nt][1];
-      }
-  }
 }
 
 // One 16-bit K/V step: TMA boxes of 16 keys x 64 elements with the 128-byte swizzle, in a ring of the warp's own.
 template <int D>
 struct Core16 {
-  static constexpr int WARPS = 8, STAGES = 3;
+  static constexpr int WARPS = split_warps(false, D), STAGES = 3;
   static constexpr int HALVES = D / 64, BOX = STEP * 128, TILE = HALVES * BOX, STAGE = 2 * TILE;
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int SMEM = 1024 + RING + WARPS * STAGES * 8 + 16;
@@ -237,7 +243,7 @@ struct Core16 {
 // One FP4 step: 16 keys of packed values and scales copied with cp.async into a ring of the warp's own.
 template <int D>
 struct Core4 {
-  static constexpr int WARPS = 12, STAGES = 4;
+  static constexpr int WARPS = split_warps(true, D), STAGES = 4;
   static constexpr int ROW = D / 2, SROW = D / 16;
   static constexpr int STAGE = 2 * STEP * (ROW + SROW);
   static constexpr int RING = WARPS * STAGES * STAGE;
@@ -274,7 +280,7 @@ __device__ __forceinline__ long long block_line(const SplitParams& p, long long*
 }
 
 template <int D, bool F16, int NT, bool CAP, bool FP4>
-__global__ void __launch_bounds__(FP4 ? 384 : 256, 1)
+__global__ void __launch_bounds__((FP4 ? Core4<D>::WARPS : Core16<D>::WARPS) * 32, 1)
 fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                         const __grid_constant__ SplitParams p, uint32_t* status) {
   using C16 = Core16<D>;
@@ -445,8 +451,8 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
 #pragma unroll
         for (int w = 0; w < D / 32; ++w)
 #pragma unroll
-          for (int x = 0; x < 4; ++x)                 // nibbles x and x + 4 of the word
-            qb[nt][2 * w + (x >> 1)][x & 1] = pack_f16x2(f[w * 8 + x] * inv, f[w * 8 + x + 4] * inv);
+          for (int x = 0; x < 4; ++x)                 // byte x of the word
+            qb[nt][2 * w + (x >> 1)][x & 1] = pack_f16x2(f[w * 8 + 2 * x] * inv, f[w * 8 + 2 * x + 1] * inv);
         // rows 2t and 2t + 1 sit in the lanes with g = 2t, 2t + 1
         q_unit[nt][0] = __shfl_sync(0xffffffffu, unit, 8 * t);
         q_unit[nt][1] = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
@@ -540,21 +546,20 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
             asm volatile("{.reg .b16 h; ld.shared.u8 h, [%1]; cvt.u32.u16 %0, h;}"
                          : "=r"(two) : "r"(sKs + (g + 8 * x) * C4::SROW + t));
           }
-          sc[x] = hmul2(e4m3x2_to_f16x2(two), 0x58005800u);   // * 2^7
+          sc[x] = e4m3x2_to_f16x2(two);
         }
 #pragma unroll
         for (int w = 0; w < WORDS; ++w) {
           uint32_t f0[4], f1[4];
           const uint32_t s0 = __byte_perm(sc[0], sc[0], w >= 2 ? 0x3232 : 0x1010);
           const uint32_t s1 = __byte_perm(sc[1], sc[1], w >= 2 ? 0x3232 : 0x1010);
-          f0[0] = hmul2(e2m1_to_f16x2<0>(wk[0][w]), s0);
-          f0[1] = hmul2(e2m1_to_f16x2<1>(wk[0][w]), s0);
-          f0[2] = hmul2(e2m1_to_f16x2<2>(wk[0][w]), s0);
-          f0[3] = hmul2(e2m1_to_f16x2<3>(wk[0][w]), s0);
-          f1[0] = hmul2(e2m1_to_f16x2<0>(wk[1][w]), s1);
-          f1[1] = hmul2(e2m1_to_f16x2<1>(wk[1][w]), s1);
-          f1[2] = hmul2(e2m1_to_f16x2<2>(wk[1][w]), s1);
-          f1[3] = hmul2(e2m1_to_f16x2<3>(wk[1][w]), s1);
+          e2m1x8_to_f16(wk[0][w], f0);
+          e2m1x8_to_f16(wk[1][w], f1);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {               // exact: two significant bits times four
+            f0[x] = hmul2(f0[x], s0);
+            f1[x] = hmul2(f1[x], s1);
+          }
           const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -567,8 +572,9 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[nt][e] *= q_unit[nt][e & 1];
         softmax_step<true, NT, DT, CAP, HILO>(p, rm, key0, lane, ragged, s, m_run, l_run, o, pb, pl);
-        // V: dimensions [D/8 g, D/8 (g + 1)) of keys 2t, 2t + 1, 2t + 8, 2t + 9; the halves of two keys' words side by
-        // side give (key, key + 1) pairs of one dimension per nibble.  Row m of tile c <-> dimension D/8 g + 2c (+ 1).
+        // V: dimensions [D/8 g, D/8 (g + 1)) of keys 2t, 2t + 1, 2t + 8, 2t + 9.  The operand wants two keys side by side
+        // in a register, so the codes of two keys are put into one byte first: lo holds the even dimensions, hi the odd
+        // ones.  Row m of tile c <-> dimension D/8 m + 2c, row m + 8 <-> the next one.
         constexpr int VW = D / 64;                    // words per key
         uint32_t wv[4][VW], sb[4];
 #pragma unroll
@@ -583,33 +589,41 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
           asm volatile("{.reg .b16 h; ld.shared.u8 h, [%1]; cvt.u32.u16 %0, h;}" : "=r"(sb[x]) : "r"(sat));
         }
         // a masked key's scale may be a NaN pattern: the mask clears the product, not the factor
-        const uint32_t sv0 = hmul2(e4m3x2_to_f16x2(sb[0] | (sb[1] << 8)), 0x58005800u);
-        const uint32_t sv1 = hmul2(e4m3x2_to_f16x2(sb[2] | (sb[3] << 8)), 0x58005800u);
+        const uint32_t sv0 = e4m3x2_to_f16x2(sb[0] | (sb[1] << 8)), sv1 = e4m3x2_to_f16x2(sb[2] | (sb[3] << 8));
 #pragma unroll
-        for (int w = 0; w < VW; ++w)
+        for (int w = 0; w < VW; ++w) {
+          constexpr uint32_t M = 0x0F0F0F0Fu;
+          uint32_t f[4][4];                           // lo and hi of keys 2t, 2t + 1; of keys 2t + 8, 2t + 9
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t sel = half ? 0x7632u : 0x5410u;
-            const uint32_t x0 = __byte_perm(wv[0][w], wv[1][w], sel), x1 = __byte_perm(wv[2][w], wv[3][w], sel);
-            uint32_t f0[4], f1[4];
-            f0[0] = hmul2(e2m1_to_f16x2<0>(x0), sv0) & vm0;
-            f0[1] = hmul2(e2m1_to_f16x2<1>(x0), sv0) & vm0;
-            f0[2] = hmul2(e2m1_to_f16x2<2>(x0), sv0) & vm0;
-            f0[3] = hmul2(e2m1_to_f16x2<3>(x0), sv0) & vm0;
-            f1[0] = hmul2(e2m1_to_f16x2<0>(x1), sv1) & vm1;
-            f1[1] = hmul2(e2m1_to_f16x2<1>(x1), sv1) & vm1;
-            f1[2] = hmul2(e2m1_to_f16x2<2>(x1), sv1) & vm1;
-            f1[3] = hmul2(e2m1_to_f16x2<3>(x1), sv1) & vm1;
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t ka = wv[2 * x][w], kb = wv[2 * x + 1][w], sc2 = x ? sv1 : sv0;
+            e2m1x8_to_f16((ka & M) | ((kb << 4) & ~M), f[2 * x]);
+            e2m1x8_to_f16(((ka >> 4) & M) | (kb & ~M), f[2 * x + 1]);
 #pragma unroll
-            for (int c2 = 0; c2 < 2; ++c2) {
-              const uint32_t a[4] = {f0[2 * c2], f0[2 * c2 + 1], f1[2 * c2], f1[2 * c2 + 1]};
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma_16816<true>(o[(w * 2 + half) * 2 + c2][nt], a, pb[nt][0], pb[nt][1]);
-                if (HILO) mma_16816<true>(o[(w * 2 + half) * 2 + c2][nt], a, pl[nt][0], pl[nt][1]);
-              }
+            for (int i = 0; i < 4; ++i) {
+              f[2 * x][i] = hmul2(f[2 * x][i], sc2);
+              f[2 * x + 1][i] = hmul2(f[2 * x + 1][i], sc2);
             }
           }
+          if (clear) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              f[0][i] &= vm0;
+              f[1][i] &= vm0;
+              f[2][i] &= vm1;
+              f[3][i] &= vm1;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t a[4] = {f[0][i], f[1][i], f[2][i], f[3][i]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_16816<true>(o[w * 4 + i][nt], a, pb[nt][0], pb[nt][1]);
+              if (HILO) mma_16816<true>(o[w * 4 + i][nt], a, pl[nt][0], pl[nt][1]);
+            }
+          }
+        }
       }
     }
     if (FP4 && nk > 0) {
@@ -821,9 +835,9 @@ int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
   p.min_steps = 2;
   CUtensorMap tmK = {}, tmV = {};
   if constexpr (FP4) {
-    p.score.scale_log2 *= c.k_global * F4_UNIT;
-    p.score.cap_arg *= c.k_global * F4_UNIT;
-    p.out_scale = c.v_global * F4_UNIT;
+    p.score.scale_log2 *= c.k_global ;
+    p.score.cap_arg *= c.k_global ;
+    p.out_scale = c.v_global ;
     p.k = static_cast<const uint8_t*>(c.k);
     p.v = static_cast<const uint8_t*>(c.v);
     p.ks = static_cast<const uint8_t*>(c.k_scales);
@@ -871,7 +885,7 @@ int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
 PagedSplitPlan b200_paged_split_plan(int format, int head_dim, int kv_heads, int batch, long long rows,
                                      long long max_keys) {
   PagedSplitPlan pl;
-  const int warps = format ? 12 : 8;
+  const int warps = b200::split_warps(format != 0, head_dim);
   pl.rows_per_block = rows <= 8 ? 8 : 16;
   const long long rb_max = (rows + pl.rows_per_block - 1) / pl.rows_per_block;
   pl.items = (long long)batch * rb_max * kv_heads;

@@ -1,17 +1,23 @@
 // Attention of many query rows (prompts and prompt chunks) over a paged key/value cache on the 5th-generation tensor
-// cores.  The mathematics is fmha_paged.cu's; the machine is fmha_fwd.cu's: one CTA owns two tiles of 128 query rows
+// cores.  The mathematics is fmha_paged.cu's; the machine is fmha_fwd.cu's: one CTA works on two tiles of 128 query rows
 // and walks the keys once for both, S = Q K^T and O += P V by tcgen05 with S, P and O in Tensor Memory, one softmax
 // thread per row, O rescaled only when a row's maximum grew by more than 2^8.  What differs:
 //
 //   - a tile's rows are (token, head of the group) pairs of ONE K/V head, 128 / group tokens at a time, so that K and V
 //     pass through a CTA once for all heads that share them (one TMA box {64, group, tokens} brings them in that order);
-//   - the 128 keys of a step come from 128 / page_size pages, one TMA box each; a page that no row of the CTA looks at
+//   - the 128 keys of a step come from 128 / page_size pages, one TMA box each; a page that no row of the pair looks at
 //     gets the page number just outside the pool, where TMA fills in zeros without touching memory;
 //   - V rows of a step that no row looks at (behind the length, before the window) are cleared in shared memory by the
 //     MMA warp: their probability is 0, but 0 times whatever a free slot holds need not be;
-//   - an NVFP4 cache takes four more warps: thread r expands key r of the step (64 bytes and 8 scales for D = 128) to 16
-//     bits straight into the swizzled operand tile, K and V in turn, with the next row's bytes already in registers;
-//   - which (sequence, pair of tiles) a CTA works on follows from the lengths on the device; CTAs without work leave.
+//   - the grid is one CTA per SM, and the steps of all items (sequence, pair of tiles, K/V head) form one line that is cut
+//     into equal runs, as in fmha_paged.cu: few long chunks and many short prompts fill the machine alike, and nothing
+//     about the lengths is needed on the host.  The rings run on from item to item and the next Q is fetched while the
+//     last keys of the present one are worked on.  An item that is cut leaves (m, l, O) of its parts in 32 bits for the
+//     merge kernel, at most two parts per CTA;
+//   - an NVFP4 cache takes four more warps: thread r expands key r of the step (64 bytes and 8 scales for D = 128) to f16
+//     straight into the swizzled operand tile, K and V in turn, with the next row's bytes already in registers.  The
+//     products are then f16 x f16, which holds every code * scale exactly; bf16 queries are brought to a power of two near
+//     1 row by row and converted in shared memory by two otherwise idle warps.
 //
 // What bounds it: as fmha_fwd.cu, the softmax threads and the tensor pipe together.
 #include <math_constants.h>
@@ -33,10 +39,22 @@ struct TileParams {
   uint16_t* out;
   long long o_ts, o_hs;
   float out_scale;
+  float cap_poly[6];                 // CAP_POLY * c log2e
+  float* part;                       // two slots per CTA
+  int4* desc;                        // one per CTA
   // FP4 operands: byte strides
   const uint8_t *k, *v, *ks, *vs;
   long long k_st[3], v_st[3], ks_st[3], vs_st[3];
 };
+
+// A part: O as [2 tiles][D / 4][128 rows] float4 (lanes = rows, so that stores and loads are full lines), then
+// [2][128] maxima and [2][128] sums.
+__host__ __device__ constexpr int part_floats(int d) { return 2 * 128 * (d + 2); }
+// Starting and ending an item costs about as much as this many steps of 128 keys: the line that is cut into runs counts
+// them in front of every item's steps.
+constexpr int ITEM_COST = 2;
+constexpr int MIN_RUN = 6;
+constexpr int PART_RING = 4;         // parts known ahead of their turn
 
 template <int D, bool FP4>
 struct TileSmem {
@@ -48,10 +66,12 @@ struct TileSmem {
   static constexpr int OFF_K = OFF_Q + 2 * TILE_BYTES;
   static constexpr int OFF_V = OFF_K + KV_STAGES * TILE_BYTES;
   static constexpr int OFF_BAR = OFF_V + KV_STAGES * TILE_BYTES;
-  // barriers: q_full[2], k_full[S], k_empty[S], v_full[S], v_empty[S], s_full[2], p_full[2], o_done[2]
-  static constexpr int NUM_BARS = 2 + 4 * KV_STAGES + 6;
-  static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  static constexpr int TOTAL = OFF_MISC + 16 + 1024;
+  // barriers: q_full[2], q_free[2], q_ready[2], k_full[S], k_empty[S], v_full[S], v_empty[S], s_full[2], p_full[2],
+  // o_done[2], part_full[R], part_free[R]
+  static constexpr int NUM_BARS = 6 + 4 * KV_STAGES + 6 + 2 * PART_RING;
+  static constexpr int OFF_MISC = (OFF_BAR + NUM_BARS * 8 + 15) / 16 * 16;
+  static constexpr int OFF_OUT = OFF_MISC + 16;      // 32 rows x 64 bytes per softmax warp: output on its way to memory
+  static constexpr int TOTAL = OFF_OUT + 8 * 2048 + 1024;
   static constexpr int THREADS = FP4 ? 512 : 384;
 };
 
@@ -66,49 +86,121 @@ __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.w
 __device__ __forceinline__ void st_shared_v4(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ void ld_shared_v4(uint32_t src, uint32_t (&w)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src) : "memory");
+}
 
 // Pairs of tiles that sequence b has here: none when its rows are few enough for the row-block kernel.
 __device__ __forceinline__ int seq_pairs(const TileParams& p, const SeqView& s) {
   if ((long long)s.n * p.group <= p.row_limit) return 0;
   return (s.n + 2 * p.tpt - 1) / (2 * p.tpt);
 }
+// Key range and steps of a pair; a pair that sees no key still has one step, so that its rows are written.
+struct PairSpan {
+  int lo, hi, j0, steps;
+};
+__device__ __forceinline__ PairSpan pair_span(const TileParams& p, const SeqView& s, int pair) {
+  PairSpan x;
+  const int t0 = pair * 2 * p.tpt, n = min(s.n - t0, 2 * p.tpt);
+  x.hi = p.causal ? min(s.len, s.pos0 + t0 + n) : s.len;
+  x.lo = p.causal && p.window > 0 ? max(0, s.pos0 + t0 - p.window + 1) : 0;
+  x.j0 = x.hi > x.lo ? x.lo / FA_BN : 0;
+  x.steps = x.hi > x.lo ? (x.hi + FA_BN - 1) / FA_BN - x.j0 : 1;
+  return x;
+}
 
-// 8 codes of a word and their scale (16 bits, twice; times 2^7, for bf16 2^119) -> 8 values * 2^-7 in order.
-// The codes' bits are put where the 16-bit type reads them as e2m1 * 2^-14 (bf16: 2^-126), subnormals included; the
-// product with the scale is exact (two bits times four).
-template <bool F16>
-__device__ __forceinline__ void expand8(uint32_t w, uint32_t scale, uint32_t (&o)[4]) {
-  uint32_t pr[4];                                   // (nibble i, nibble i + 4)
+// Place on the line of all steps.
+struct Walk {
+  long long u, u_end;
+  int b, pairs, pair, head;
+  SeqView sv;
+  PairSpan sp;
+  int at;                            // place in the item, ITEM_COST + step
+  int a0, a1;                        // steps of this part, relative to sp.j0
+  __device__ __forceinline__ int left() const { return (int)min((long long)(ITEM_COST + sp.steps - at), u_end - u); }
+  // steps of the part at `at`; none if the run ends within the item's cost: the next CTA begins the item then
+  __device__ __forceinline__ bool cut() {
+    a0 = max(0, at - ITEM_COST);
+    a1 = max(0, at + left() - ITEM_COST);
+    if (a1 > a0) return true;
+    u = u_end;
+    return false;
+  }
+  __device__ __forceinline__ void next(const TileParams& p) {
+    u += left();
+    if (u >= u_end) return;
+    at = 0;                          // the run goes on, so the item has ended
+    if (++head == p.kv_heads) {
+      head = 0;
+      if (++pair == pairs) {
+        pair = 0;
+        do {
+          if (++b >= p.batch.batch) {
+            u = u_end;
+            return;
+          }
+          sv = seq_view(p.batch, b);
+          pairs = seq_pairs(p, sv);
+        } while (pairs == 0);
+      }
+      sp = pair_span(p, sv, pair);
+    }
+    cut();
+  }
+};
+
+// One part of an item as the roles need it.  The loader warp walks the run and hands the parts to the others through a
+// ring in shared memory: the walk's divisions and loads happen once, ahead of time, instead of in every role between
+// two items.
+struct Part {
+  int end;                           // no more parts
+  int steps[2];                      // steps of either tile in this part
+  int tokens[2];
+  int key0, lo, hi;                  // first key of the part; keys that some row of the pair sees
+  int b, pair, head;
+  int row0, pos0, len;               // row and position of the pair's first token; cached rows of the sequence
+  int whole, slot, parts;            // the item is not cut; which slot its part takes; parts (first one only)
+};
+__device__ __forceinline__ Part make_part(const TileParams& p, const Walk& w, long long per) {
+  Part x;
+  x.end = 0;
+  x.b = w.b;
+  x.pair = w.pair;
+  x.head = w.head;
+  x.row0 = w.sv.q0 + w.pair * 2 * p.tpt;
+  x.pos0 = w.sv.pos0 + w.pair * 2 * p.tpt;
+  x.len = w.sv.len;
+  x.key0 = (w.sp.j0 + w.a0) * FA_BN;
+  x.lo = w.sp.lo;
+  x.hi = w.sp.hi;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t sgn = i == 3 ? w : w << (12 - 4 * i);
-    uint32_t mag;
-    if (F16) mag = (i == 3 ? w >> 3 : w << (9 - 4 * i)) & 0x0E000E00u;
-    else mag = (i < 2 ? w << (6 - 4 * i) : w >> (4 * i - 6)) & 0x01C001C0u;
-    const uint32_t x = (sgn & 0x80008000u) | mag;
-    if (F16) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(pr[i]) : "r"(x), "r"(scale));
-    else asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(pr[i]) : "r"(x), "r"(scale));
+  for (int t = 0; t < 2; ++t) {
+    const int n = min(max(w.sv.n - (w.pair * 2 + t) * p.tpt, 0), p.tpt);
+    const int hi = n == 0 ? 0 : p.causal ? min(w.sv.len, x.pos0 + t * p.tpt + n) : w.sv.len;
+    x.tokens[t] = n;
+    x.steps[t] = max(0, min(w.a1, (hi + FA_BN - 1) / FA_BN - w.sp.j0) - w.a0);
   }
-  o[0] = __byte_perm(pr[0], pr[1], 0x5410);
-  o[1] = __byte_perm(pr[2], pr[3], 0x5410);
-  o[2] = __byte_perm(pr[0], pr[1], 0x7632);
-  o[3] = __byte_perm(pr[2], pr[3], 0x7632);
+  x.whole = w.a0 == 0 && w.a1 == w.sp.steps;
+  x.slot = w.a0 == 0 ? 1 : 0;        // an item's first part, or the continuation of an earlier CTA's
+  x.parts = 1 + (int)((w.sp.steps - w.a1 + per - 1) / per);   // beyond the cost, every later place is a step
+  return x;
 }
-// e4m3 byte -> the scale operand of expand8
-template <bool F16>
-__device__ __forceinline__ uint32_t expand_scale(uint32_t byte) {
-  uint32_t h;
-  asm("{.reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t;}" : "=r"(h) : "r"(byte & 0xffu));
-  if (F16) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x58005800u));
-    return __byte_perm(r, r, 0x1010);
-  }
-  float f;
-  asm("{.reg .b16 a, b; mov.b32 {a, b}, %1; cvt.f32.f16 %0, a;}" : "=f"(f) : "r"(h));
-  const uint32_t r = __float_as_uint(f * 6.64613997892457936e+35f);   // 2^119; four significant bits: exact in bf16
-  return __byte_perm(r, r, 0x3232);
+
+// The four bytes of w, two e2m1 codes each, as f16 pairs times a pair of equal scales: exact (two bits times four).
+__device__ __forceinline__ void expand8(uint32_t w, uint32_t scale, uint32_t (&o)[4]) {
+  asm("{.reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4;"
+      " cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b; cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d;}"
+      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(o[i]) : "r"(o[i]), "r"(scale));
 }
+
+// c log2e tanh(s a) as an odd polynomial in s a with c log2e folded into the coefficients: the Chebyshev interpolant of tanh(sqrt u) / sqrt u on [0, 0.75^2], off by at most 4.5e-8 for |s a| <= 0.75.  Scores are a
+// small part of the cap almost always; steps with a larger one take exp2 and a reciprocal instead, which triples the load
+// of the special-function unit that bounds the softmax.
+constexpr float CAP_POLY_MAX = 0.75f;
+constexpr float CAP_POLY[6] = {1.0f, -0.33332952857017517f, 0.13325339555740356f, -0.05334111675620079f,
+                               0.019576216116547585f, -0.004711522255092859f};
 
 template <int D, bool F16, bool CAP, bool FP4>
 __global__ void __launch_bounds__(FP4 ? 512 : 384, 1)
@@ -117,93 +209,145 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   using L = TileSmem<D, FP4>;
   constexpr int STAGES = L::KV_STAGES, HALVES = L::HALVES, THREADS = L::THREADS;
   constexpr uint32_t HALF = L::HALF_BYTES, TILE = L::TILE_BYTES;
+  constexpr bool MF16 = F16 || FP4;               // element type of the products
+  constexpr bool CONVERT = FP4 && !F16;           // bf16 queries for f16 products
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int s_first[THREADS], s_warp[THREADS / 32];
+  __shared__ int s_first[THREADS];
+  __shared__ long long s_line[THREADS], s_warp[THREADS / 32], s_per;
+  __shared__ Walk s_walk;
+  __shared__ Part s_part[PART_RING];
+  __shared__ float s_unit[CONVERT ? 2 : 1][CONVERT ? 2 : 1][CONVERT ? 128 : 1];   // [item parity][tile][row]
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge, which waits for this grid
 
-  // ---- this CTA's work: pair `rank` of all sequences' pairs, one K/V head ----
-  // (launched while the row-block kernel's merge may still run: see the end of the kernel)
-  const int rank = blockIdx.x / p.kv_heads, head = blockIdx.x - rank * p.kv_heads;
-  int b, pair;
-  SeqView sv;
-  {
-    const int per = (p.batch.batch + THREADS - 1) / THREADS;
-    int mine = 0;
-    for (int i = threadIdx.x * per; i < min(p.batch.batch, (int)(threadIdx.x + 1) * per); ++i)
-      mine += seq_pairs(p, seq_view(p.batch, i));
-    int inc = mine;
+  // ---- this CTA's run ----
+  auto block_scan = [&](long long mine, long long& total) {   // exclusive prefix over the threads
+    long long inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      const long long up = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += up;
     }
+    __syncthreads();
     if (lane == 31) s_warp[warp] = inc;
     __syncthreads();
-    int before = 0, total = 0;
+    long long before = 0;
+    total = 0;
     for (int w = 0; w < THREADS / 32; ++w) {
-      before += w < warp ? s_warp[w] : 0;
+      if (w < warp) before += s_warp[w];
       total += s_warp[w];
     }
-    s_first[threadIdx.x] = before + inc - mine;
+    return before + inc - mine;
+  };
+  {
+    Walk first;
+    const int per_b = (p.batch.batch + THREADS - 1) / THREADS;
+    long long mine = 0, total;
+    for (int i = threadIdx.x * per_b; i < min(p.batch.batch, (int)(threadIdx.x + 1) * per_b); ++i)
+      mine += seq_pairs(p, seq_view(p.batch, i));
+    s_first[threadIdx.x] = (int)block_scan(mine, total);
     __syncthreads();
-    if (rank >= total) {
+    const int all_pairs = (int)total;
+    // sequence and pair at position `at` of the list of pairs
+    auto pair_at = [&](int at, Walk& w) {
+      int lo = 0, hi = THREADS - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_first[mid] <= at) lo = mid;
+        else hi = mid - 1;
+      }
+      int seen = s_first[lo];
+      w.b = lo * per_b;
+      w.sv = seq_view(p.batch, w.b);
+      w.pairs = seq_pairs(p, w.sv);
+      while (seen + w.pairs <= at && w.b + 1 < p.batch.batch) {
+        seen += w.pairs;
+        w.sv = seq_view(p.batch, ++w.b);
+        w.pairs = seq_pairs(p, w.sv);
+      }
+      w.pair = at - seen;
+    };
+    auto step_pair = [&](Walk& w) {                // to the next pair of the list, if there is one
+      if (++w.pair < w.pairs) return;
+      w.pair = 0;
+      do {
+        if (w.b + 1 >= p.batch.batch) return;
+        w.sv = seq_view(p.batch, ++w.b);
+        w.pairs = seq_pairs(p, w.sv);
+      } while (w.pairs == 0);
+    };
+    const int per_p = (all_pairs + THREADS - 1) / THREADS;
+    const int p_begin = threadIdx.x * per_p, p_end = min(all_pairs, p_begin + per_p);
+    mine = 0;
+    if (p_begin < p_end) {
+      Walk w;
+      pair_at(p_begin, w);
+      for (int i = p_begin; i < p_end; ++i) {
+        mine += (long long)(ITEM_COST + pair_span(p, w.sv, w.pair).steps) * p.kv_heads;
+        step_pair(w);
+      }
+    }
+    s_line[threadIdx.x] = block_scan(mine, total);
+    __syncthreads();
+    long long per = (total + gridDim.x - 1) / gridDim.x;
+    if (per < MIN_RUN) per = MIN_RUN;
+    first.u = blockIdx.x * per;
+    first.u_end = min(total, first.u + per);
+    if (threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (first.u >= first.u_end) {
       grid_dep_wait();
       return;
     }
     int lo = 0, hi = THREADS - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (s_first[mid] <= rank) lo = mid;
+      if (s_line[mid] <= first.u) lo = mid;
       else hi = mid - 1;
     }
-    b = lo * per;
-    int at = s_first[lo];
-    sv = seq_view(p.batch, b);
-    int n = seq_pairs(p, sv);
-    while (at + n <= rank) {
-      at += n;
-      if (++b >= p.batch.batch) {
-        grid_dep_wait();
-        return;
-      }
-      sv = seq_view(p.batch, b);
-      n = seq_pairs(p, sv);
+    long long line = s_line[lo];
+    pair_at(lo * per_p, first);
+    first.sp = pair_span(p, first.sv, first.pair);
+    while (line + (long long)(ITEM_COST + first.sp.steps) * p.kv_heads <= first.u) {
+      line += (long long)(ITEM_COST + first.sp.steps) * p.kv_heads;
+      step_pair(first);
+      first.sp = pair_span(p, first.sv, first.pair);
     }
-    pair = rank - at;
-    if (p.causal) pair = n - 1 - pair;             // the longest first
+    const long long rel = first.u - line;
+    first.head = (int)(rel / (ITEM_COST + first.sp.steps));
+    first.at = (int)(rel - (long long)first.head * (ITEM_COST + first.sp.steps));
+    if (!first.cut()) {                            // every thread finds the same
+      grid_dep_wait();
+      return;
+    }
+    if (threadIdx.x == 0) {
+      s_walk = first;
+      s_per = per;
+    }
   }
-  // tokens and keys of the two tiles; steps of 128 keys from step j0
-  int tok0[2], ntok[2], hi_key[2], n_kv[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    tok0[t] = (pair * 2 + t) * p.tpt;
-    ntok[t] = min(max(sv.n - tok0[t], 0), p.tpt);
-    hi_key[t] = ntok[t] == 0 ? 0 : p.causal ? min(sv.len, sv.pos0 + tok0[t] + ntok[t]) : sv.len;
-  }
-  const int lo_key = p.causal && p.window > 0 ? max(0, sv.pos0 + tok0[0] - p.window + 1) : 0;
-  const int hi_all = max(hi_key[0], hi_key[1]);
-  const int j0 = lo_key / FA_BN;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) n_kv[t] = max(0, (hi_key[t] + FA_BN - 1) / FA_BN - j0);
-  const int n_max = max(n_kv[0], n_kv[1]);
 
   const uint32_t sQ = base + L::OFF_Q, sK = base + L::OFF_K, sV = base + L::OFF_V;
   const uint32_t bar_q_full = base + L::OFF_BAR;
-  const uint32_t bar_k_full = bar_q_full + 2 * 8;
+  const uint32_t bar_q_free = bar_q_full + 2 * 8;
+  const uint32_t bar_q_ready = bar_q_free + 2 * 8;
+  const uint32_t bar_k_full = bar_q_ready + 2 * 8;
   const uint32_t bar_k_empty = bar_k_full + STAGES * 8;
   const uint32_t bar_v_full = bar_k_empty + STAGES * 8;
   const uint32_t bar_v_empty = bar_v_full + STAGES * 8;
   const uint32_t bar_s_full = bar_v_empty + STAGES * 8;
   const uint32_t bar_p_full = bar_s_full + 2 * 8;
   const uint32_t bar_o_done = bar_p_full + 2 * 8;
+  const uint32_t bar_part_full = bar_o_done + 2 * 8;
+  const uint32_t bar_part_free = bar_part_full + PART_RING * 8;
   volatile uint32_t* misc = reinterpret_cast<volatile uint32_t*>(gen_base + L::OFF_MISC);
   WaitCtx wctx{misc + 1, status};
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_q_full + i * 8, 1);
+      mbar_init(bar_q_free + i * 8, 1);
+      mbar_init(bar_q_ready + i * 8, 1);
       mbar_init(bar_s_full + i * 8, 1);
       mbar_init(bar_p_full + i * 8, 4);
       mbar_init(bar_o_done + i * 8, 1);
@@ -213,6 +357,10 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       mbar_init(bar_k_empty + s * 8, 1);
       mbar_init(bar_v_full + s * 8, FP4 ? 4 : 1);
       mbar_init(bar_v_empty + s * 8, 1);
+    }
+    for (int i = 0; i < PART_RING; ++i) {
+      mbar_init(bar_part_full + i * 8, 1);
+      mbar_init(bar_part_free + i * 8, THREADS / 32 - 1);    // every warp but the loader's
     }
     misc[1] = 0;
     fence_mbar_init();
@@ -232,123 +380,151 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   const uint32_t tmem_base = misc[0];
   auto S_COL = [](int t) { return (uint32_t)(t * 128); };
   auto O_COL = [](int t) { return (uint32_t)(256 + t * 128); };
+  auto wait_all = [&](uint32_t bar, uint32_t parity, uint32_t site) {
+    return __all_sync(0xffffffffu, mbar_wait(wctx, bar, parity, site)) != 0;
+  };
+
+  // the i-th part, once it is there (all lanes of the warp together); false when the run has ended or a wait gave up
+  auto have_part = [&](int i) {
+    return wait_all(bar_part_full + (i % PART_RING) * 8, (i / PART_RING) & 1, 16) && !s_part[i % PART_RING].end;
+  };
+  auto done_part = [&](int i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_part_free + (i % PART_RING) * 8);
+  };
 
   if (warp < 4) reg_dealloc<FP4 ? 40 : FA_OTHER_REGS>();
   if (warp == 0) {
-    // ------------------------------- loader -------------------------------
-    if (lane == 0) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (n_kv[t] == 0) continue;
-        mbar_expect_tx(bar_q_full + t * 8, (uint32_t)(HALVES * 128 * p.tpt * p.group));
-#pragma unroll
-        for (int h = 0; h < HALVES; ++h)
-          tma_load_3d(sQ + t * TILE + h * HALF, &tmQ, bar_q_full + t * 8, h * 64, head * p.group, sv.q0 + tok0[t]);
+    // ------------------------------- parts, K and V -------------------------------
+    const int boxes = FA_BN / p.box_rows;
+    const int slot_mask = (1 << p.batch.page_shift) - 1;
+    int armed_k = 0, armed_v = 0;        // K and V steps fetched so far: stage and phase of the ring
+    bool ok = true;
+    for (int i = 0;; ++i) {
+      const int at = i % PART_RING;
+      if (i >= PART_RING && !wait_all(bar_part_free + at * 8, (i / PART_RING - 1) & 1, 17)) { ok = false; break; }
+      if (lane == 0) {
+        if (i > 0) s_walk.next(p);
+        if (s_walk.u < s_walk.u_end) s_part[at] = make_part(p, s_walk, s_per);
+        else s_part[at].end = 1;
+        mbar_arrive(bar_part_full + at * 8);
       }
-    }
-    if (!FP4) {
-      const int boxes = FA_BN / p.box_rows;
-      const int slot_mask = (1 << p.batch.page_shift) - 1;
+      __syncwarp();
+      const Part& w = s_part[at];
+      if (w.end) break;
+      if (FP4) continue;
       // lane i < boxes: page of box i; lane i < boxes * HALVES issues box i % boxes of half i / boxes
+      const int n = max(w.steps[0], w.steps[1]), key0 = w.key0, lo = w.lo, hi = w.hi, b = w.b, head = w.head;
       auto page_for = [&](int j) {
-        const int key = (j0 + j) * FA_BN + lane * p.box_rows;
-        const bool used = j < n_max && lane < boxes && key < hi_all && key + p.box_rows > lo_key;
+        const int key = key0 + j * FA_BN + lane * p.box_rows;
+        const bool used = j < n && lane < boxes && key < hi && key + p.box_rows > lo;
         return used ? page_of(p.batch, b, key, status) : p.batch.num_pages;
       };
-      uint32_t stage = 0, phase = 0;
-      int pages = page_for(0), k_armed = 0, v_armed = 0;
-      for (int j = 0; j < n_max; ++j) {
+      int pages = n > 0 ? page_for(0) : 0;
+      for (int j = 0; j < n; ++j) {
         const int next = page_for(j + 1);
         const int box = lane % boxes, half = lane / boxes;
         const int pg = __shfl_sync(0xffffffffu, pages, box);
-        const int slot = ((j0 + j) * FA_BN + box * p.box_rows) & slot_mask;
+        const int slot = (key0 + j * FA_BN + box * p.box_rows) & slot_mask;
+        const uint32_t stage = armed_k % STAGES, phase = (armed_k / STAGES) & 1;
         const uint32_t off = stage * TILE + half * HALF + box * p.box_rows * 128;
-        if (!__all_sync(0xffffffffu, mbar_wait(wctx, bar_k_empty + stage * 8, phase ^ 1, 10))) break;
+        if (!wait_all(bar_k_empty + stage * 8, phase ^ 1, 10)) { ok = false; break; }
         if (lane == 0) mbar_expect_tx(bar_k_full + stage * 8, TILE);
         __syncwarp();
         if (half < HALVES) tma_load_4d_tile(sK + off, &tmK, bar_k_full + stage * 8, half * 64, slot, head, pg);
-        ++k_armed;
-        if (!__all_sync(0xffffffffu, mbar_wait(wctx, bar_v_empty + stage * 8, phase ^ 1, 11))) break;
+        ++armed_k;
+        if (!wait_all(bar_v_empty + stage * 8, phase ^ 1, 11)) { ok = false; break; }
         if (lane == 0) mbar_expect_tx(bar_v_full + stage * 8, TILE);
         __syncwarp();
         if (half < HALVES) tma_load_4d_tile(sV + off, &tmV, bar_v_full + stage * 8, half * 64, slot, head, pg);
-        ++v_armed;
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        ++armed_v;
         pages = next;
       }
-      if (v_armed < n_max) {
-        // a wait gave up: the copies still in flight get their (bounded) time before the shared memory goes
-        for (int i = max(0, k_armed - STAGES); i < k_armed; ++i)
-          mbar_wait(wctx, bar_k_full + (i % STAGES) * 8, (i / STAGES) & 1, 12);
-        for (int i = max(0, v_armed - STAGES); i < v_armed; ++i)
-          mbar_wait(wctx, bar_v_full + (i % STAGES) * 8, (i / STAGES) & 1, 13);
-      }
+      if (!ok) break;
+    }
+    if (!ok) {
+      // a wait gave up: the copies still in flight get their (bounded) time before the shared memory goes
+      for (int i = max(0, armed_k - STAGES); i < armed_k; ++i)
+        mbar_wait(wctx, bar_k_full + (i % STAGES) * 8, (i / STAGES) & 1, 12);
+      for (int i = max(0, armed_v - STAGES); i < armed_v; ++i)
+        mbar_wait(wctx, bar_v_full + (i % STAGES) * 8, (i / STAGES) & 1, 13);
     }
   } else if (warp == 1) {
     // ------------------------------- MMA issuer --------------------------------
     // the whole warp runs the control flow, one elected lane issues (fmha_fwd.cu says why)
-    if (n_max > 0) {
-      const bool me = elect_one() != 0;
-      constexpr uint32_t fmt = F16 ? FMT_F16 : FMT_BF16;
-      constexpr uint32_t idesc_qk = make_idesc(fmt, fmt, 0, 0, FA_BM, FA_BN);
-      constexpr uint32_t idesc_pv = make_idesc(fmt, fmt, 0, 1, FA_BM, D);
-      auto issue_qk = [&](int t, uint32_t k_addr) {
+    const bool me = elect_one() != 0;
+    constexpr uint32_t fmt = MF16 ? FMT_F16 : FMT_BF16;
+    constexpr uint32_t idesc_qk = make_idesc(fmt, fmt, 0, 0, FA_BM, FA_BN);
+    constexpr uint32_t idesc_pv = make_idesc(fmt, fmt, 0, 1, FA_BM, D);
+    auto issue_qk = [&](int t, uint32_t k_addr) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = (kk / 4) * HALF + (kk % 4) * 32;
-          const uint64_t a = make_smem_desc(sQ + t * TILE + off, 16, 1024, SWZ_128B);
-          const uint64_t bd = make_smem_desc(k_addr + off, 16, 1024, SWZ_128B);
-          if (me) umma_f16_ss(tmem_base + S_COL(t), a, bd, idesc_qk, kk != 0);
-        }
-      };
-      auto issue_pv = [&](int t, uint32_t v_addr, bool acc) {
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t off = (kk / 4) * HALF + (kk % 4) * 32;
+        const uint64_t a = make_smem_desc(sQ + t * TILE + off, 16, 1024, SWZ_128B);
+        const uint64_t bd = make_smem_desc(k_addr + off, 16, 1024, SWZ_128B);
+        if (me) umma_f16_ss(tmem_base + S_COL(t), a, bd, idesc_qk, kk != 0);
+      }
+    };
+    auto issue_pv = [&](int t, uint32_t v_addr, bool acc) {
 #pragma unroll
-        for (int kk = 0; kk < FA_BN / 16; ++kk) {
-          const uint64_t bd = make_smem_desc(v_addr + kk * 2048, HALF, 1024, SWZ_128B);
-          if (me) umma_f16_ts(tmem_base + O_COL(t), tmem_base + S_COL(t) + kk * 8, bd, idesc_pv, acc || kk != 0);
-        }
-      };
-      // V rows of the step that no row of the CTA sees
-      auto clear_v = [&](int j, uint32_t v_addr) {
-        const int key0 = (j0 + j) * FA_BN;
-        const int from = max(lo_key - key0, 0), to = min(hi_all - key0, FA_BN);
-        if (from <= 0 && to >= FA_BN) return;
-        for (int i = lane; i < FA_BN * HALVES * 8; i += 32) {
-          const int r = i / (HALVES * 8), c = i % (HALVES * 8);
-          if (r < from || r >= to) st_shared_v4(v_addr + (c >> 3) * HALF + r * 128 + (c & 7) * 16, 0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-      };
-      bool ok = __all_sync(0xffffffffu, mbar_wait(wctx, bar_k_full + 0, 0, 20));
+      for (int kk = 0; kk < FA_BN / 16; ++kk) {
+        const uint64_t bd = make_smem_desc(v_addr + kk * 2048, HALF, 1024, SWZ_128B);
+        if (me) umma_f16_ts(tmem_base + O_COL(t), tmem_base + S_COL(t) + kk * 8, bd, idesc_pv, acc || kk != 0);
+      }
+    };
+    // V rows of a step that no row of the pair sees
+    auto clear_v = [&](int key0, int lo, int hi, uint32_t v_addr) {
+      const int from = max(lo - key0, 0), to = min(hi - key0, FA_BN);
+      if (from <= 0 && to >= FA_BN) return;
+      for (int i = lane; i < FA_BN * HALVES * 8; i += 32) {
+        const int r = i / (HALVES * 8), c = i % (HALVES * 8);
+        if (r < from || r >= to) st_shared_v4(v_addr + (c >> 3) * HALF + r * 128 + (c & 7) * 16, 0, 0, 0, 0);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    int it = 0;                          // steps through the rings so far
+    uint32_t q_items[2] = {0, 0}, steps[2] = {0, 0};   // items and steps of each tile so far
+    bool ok = true;
+    for (int i = 0; ok && have_part(i); ++i) {
+      const Part& w = s_part[i % PART_RING];
+      const int cnt[2] = {w.steps[0], w.steps[1]};
+      const int n = max(cnt[0], cnt[1]), key0 = w.key0, lo = w.lo, hi = w.hi;
+      done_part(i);
+      if (n == 0) continue;
+      if (!wait_all(bar_k_full + (it % STAGES) * 8, (it / STAGES) & 1, 20)) { ok = false; break; }
 #pragma unroll
       for (int t = 0; t < 2 && ok; ++t) {
-        if (n_kv[t] == 0) continue;
-        if (!__all_sync(0xffffffffu, mbar_wait(wctx, bar_q_full + t * 8, 0, 21))) { ok = false; break; }
+        if (cnt[t] == 0) continue;
+        if (!wait_all((CONVERT ? bar_q_ready : bar_q_full) + t * 8, q_items[t] & 1, 21)) { ok = false; break; }
         tc_fence_after_sync();
-        issue_qk(t, sK);
+        issue_qk(t, sK + (it % STAGES) * TILE);
         if (me) umma_commit(bar_s_full + t * 8);
+        if (cnt[t] == 1 && me) umma_commit(bar_q_free + t * 8);
+        ++q_items[t];
       }
-      if (ok && me) umma_commit(bar_k_empty + 0);
-      for (int j = 0; j < n_max && ok; ++j) {
-        const uint32_t vs = j % STAGES, vph = (j / STAGES) & 1;
-        const uint32_t ks = (j + 1) % STAGES, kph = ((j + 1) / STAGES) & 1;
-        const bool have_next = j + 1 < n_max;
-        if (!__all_sync(0xffffffffu, mbar_wait(wctx, bar_v_full + vs * 8, vph, 22))) { ok = false; break; }
-        if constexpr (!FP4) clear_v(j, sV + vs * TILE);
-        if (have_next && !__all_sync(0xffffffffu, mbar_wait(wctx, bar_k_full + ks * 8, kph, 23))) { ok = false; break; }
+      if (ok && me) umma_commit(bar_k_empty + (it % STAGES) * 8);
+      for (int j = 0; j < n && ok; ++j, ++it) {
+        const uint32_t vs = it % STAGES, vph = (it / STAGES) & 1;
+        const uint32_t ks = (it + 1) % STAGES, kph = ((it + 1) / STAGES) & 1;
+        const bool have_next = j + 1 < n;
+        if (!wait_all(bar_v_full + vs * 8, vph, 22)) { ok = false; break; }
+        if constexpr (!FP4) clear_v(key0 + j * FA_BN, lo, hi, sV + vs * TILE);
+        if (have_next && !wait_all(bar_k_full + ks * 8, kph, 23)) { ok = false; break; }
         tc_fence_after_sync();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (j < n_kv[t]) {
-            if (!__all_sync(0xffffffffu, mbar_wait(wctx, bar_p_full + t * 8, j & 1, 24))) { ok = false; break; }
+          if (j < cnt[t]) {
+            if (!wait_all(bar_p_full + t * 8, steps[t] & 1, 24)) { ok = false; break; }
             tc_fence_after_sync();
             issue_pv(t, sV + vs * TILE, j > 0);
-            if (j == n_kv[t] - 1 && me) umma_commit(bar_o_done + t * 8);
+            ++steps[t];
+            if (j == cnt[t] - 1 && me) umma_commit(bar_o_done + t * 8);
           }
-          if (j + 1 < n_kv[t]) {
+          if (j + 1 < cnt[t]) {
             issue_qk(t, sK + ks * TILE);
             if (me) umma_commit(bar_s_full + t * 8);
+            if (j + 2 == cnt[t] && me) umma_commit(bar_q_free + t * 8);
           }
         }
         if (!ok) break;
@@ -356,6 +532,66 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         if (have_next && me) umma_commit(bar_k_empty + ks * 8);
       }
     }
+  } else if (warp < 4) {
+    // ------- Q of tile `warp - 2`; bf16 queries for f16 products: converted, a power of two per row taken out -------
+    const int t = warp - 2;
+    uint32_t items = 0;
+    for (int i = 0; have_part(i); ++i) {
+      const Part& w = s_part[i % PART_RING];
+      const int n = w.steps[t], q_head = w.head * p.group, q_row = w.row0 + t * p.tpt;
+      done_part(i);
+      if (n == 0) continue;
+      // the products of the last item with this tile's Q have been read
+      if (items > 0 && !wait_all(bar_q_free + t * 8, (items - 1) & 1, 14)) break;
+      if (lane == 0) {
+        mbar_expect_tx(bar_q_full + t * 8, (uint32_t)(HALVES * 128 * p.tpt * p.group));
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+          tma_load_3d(sQ + t * TILE + h * HALF, &tmQ, bar_q_full + t * 8, h * 64, q_head, q_row);
+      }
+      if (!CONVERT) {
+        ++items;
+        continue;
+      }
+      if (!wait_all(bar_q_full + t * 8, items & 1, 25)) break;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 32 + lane;
+        const uint32_t row = sQ + t * TILE + r * 128;
+        float mx = 0.0f;
+#pragma unroll 4
+        for (int c = 0; c < HALVES * 8; ++c) {
+          uint32_t x[4];
+          ld_shared_v4(row + (c >> 3) * HALF + (((c & 7) ^ (r & 7)) << 4), x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = paged_unpack16<false>(x[e]);
+            mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+        const uint32_t e = __float_as_uint(mx) & 0x7f800000u;
+        const bool scaled = e > (27u << 23) && e < (227u << 23);   // not for rows of zeros, infinities or NaN
+        const float inv = scaled ? __uint_as_float((254u << 23) - e) : 1.0f;
+        s_unit[items & 1][t][r] = scaled ? __uint_as_float(e) : 1.0f;
+#pragma unroll 4
+        for (int c = 0; c < HALVES * 8; ++c) {
+          const uint32_t at = row + (c >> 3) * HALF + (((c & 7) ^ (r & 7)) << 4);
+          uint32_t x[4];
+          ld_shared_v4(at, x);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = paged_unpack16<false>(x[k]);
+            x[k] = pack_f16x2(f.x * inv, f.y * inv);
+          }
+          st_shared_v4(at, x[0], x[1], x[2], x[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q_ready + t * 8);
+      ++items;
+    }
+    if (items > 0) mbar_wait(wctx, bar_q_full + t * 8, (items - 1) & 1, 15);   // nothing in flight when this warp leaves
   } else if (warp >= 4 && warp < 12) {
     // -------------------------------- softmax ----------------------------------
     reg_alloc<FA_SOFTMAX_REGS>();
@@ -366,210 +602,303 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     const uint32_t lane_base = tmem_base + ((uint32_t)(q * 32) << 16);
     const uint32_t tS = lane_base + S_COL(t);
     const uint32_t tO = lane_base + O_COL(t);
-    const int n_mine = n_kv[t];
-    // keys this row sees (rows that are no token's see none)
-    int row_lo = 0, row_hi = 0;
-    if (tok < ntok[t]) {
-      const int pos = sv.pos0 + tok0[t] + tok;
-      row_hi = p.causal ? min(sv.len, pos + 1) : sv.len;
-      if (p.causal && p.window > 0) row_lo = max(0, pos - p.window + 1);
-    }
-    float m_run = -CUDART_INF_F, l_run = 0.0f;
+    uint32_t steps = 0, items = 0;
+    const uint32_t s_out = base + L::OFF_OUT + (warp - 4) * 2048;
     bool ok = true;
-    for (int j = 0; j < n_mine && ok; ++j) {
-      if (!mbar_wait(wctx, bar_s_full + t * 8, j & 1, 30)) { ok = false; break; }
-      tc_fence_after_sync();
-      uint32_t v[FA_BN];
-#pragma unroll
-      for (int c = 0; c < FA_BN / 32; ++c)
-        tmem_ld_32x32b_x32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&v[c * 32]));
-      const int key0 = (j0 + j) * FA_BN;
-      const int c_hi = row_hi - 1 - key0, c_lo = row_lo - key0;    // first and last column seen
-      const bool masked_tile = __any_sync(0xffffffffu, c_hi < FA_BN - 1 || c_lo > 0);
-      tmem_wait_ld();
-      if (masked_tile) {
-#pragma unroll
-        for (int i = 0; i < FA_BN; ++i)
-          if (i > c_hi || i < c_lo) v[i] = 0xff800000u;  // -inf
+    for (int i = 0; ok && have_part(i); ++i) {
+      const Part& w = s_part[i % PART_RING];
+      const int n_mine = w.steps[t], key_base = w.key0;
+      // keys this row sees (rows that are no token's see none)
+      int row_lo = 0, row_hi = 0;
+      if (tok < w.tokens[t]) {
+        const int pos = w.pos0 + t * p.tpt + tok;
+        row_hi = p.causal ? min(w.len, pos + 1) : w.len;
+        if (p.causal && p.window > 0) row_lo = max(0, pos - p.window + 1);
       }
-      float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-      for (int i = 0; i < FA_BN; i += 8) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          mx[u] = max3(mx[u], __uint_as_float(v[i + 2 * u]), __uint_as_float(v[i + 2 * u + 1]));
-      }
-      const float rmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      // the score grows with s: the largest s has the largest score (the cap maps -inf to -cap: kept apart)
-      const float m_tile = rmax == -CUDART_INF_F ? rmax : paged_score<CAP>(p.score, rmax);
-      const float m_new = fmaxf(m_run, m_tile);
-      bool need = false;
-      float alpha = 1.0f;
-      if (m_run == -CUDART_INF_F) {
-        m_run = m_new;                       // nothing seen before: O and l are zero
-      } else if (m_new - m_run > FA_RESCALE_THRESHOLD) {
-        need = true;
-        alpha = ex2_approx(m_run - m_new);
-        l_run *= alpha;
-        m_run = m_new;
-      }
-      if (__any_sync(0xffffffffu, need)) {
-        // S_t(j) complete implies O_t += P_t(j-1) V(j-1) complete (MMAs retire in issue order)
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(tO + c * 32, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st_32x32b_x32(tO + c * 32, o);
+      const bool blind = row_hi <= row_lo;
+      float scale = p.score.scale_log2, cap_arg = p.score.cap_arg;
+      float m_run = -CUDART_INF_F, l_run = 0.0f;
+      for (int j = 0; j < n_mine; ++j, ++steps) {
+        if (!wait_all(bar_s_full + t * 8, steps & 1, 30)) { ok = false; break; }
+        tc_fence_after_sync();
+        if (CONVERT && j == 0) {
+          const float unit = s_unit[items & 1][t][row];
+          scale *= unit;
+          cap_arg *= unit;
         }
-      }
-      const float neg_m = m_run == -CUDART_INF_F ? 0.0f : -m_run;
-      uint64_t ls2[4] = {0ull, 0ull, 0ull, 0ull};
-      const uint64_t scale2 = CAP ? pack2(p.score.cap_arg, p.score.cap_arg) : pack2(p.score.scale_log2, p.score.scale_log2);
-      const uint64_t negm2 = pack2(neg_m, neg_m);
+        uint32_t v[FA_BN];
 #pragma unroll
-      for (int c = 0; c < FA_BN / 32; ++c) {
-        uint32_t pk[16];
+        for (int c = 0; c < FA_BN / 32; ++c)
+          tmem_ld_32x32b_x32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&v[c * 32]));
+        const int key0 = key_base + j * FA_BN;
+        const int c_hi = row_hi - 1 - key0, c_lo = row_lo - key0;    // first and last column seen
+        const bool masked_tile = __any_sync(0xffffffffu, c_hi < FA_BN - 1 || c_lo > 0);
+        tmem_wait_ld();
+        if (masked_tile) {
+          // a row that sees nothing at all would keep the cap's polynomial from the others: it holds zeros there
+          const uint32_t hidden = CAP && blind ? 0u : 0xff800000u;   // -inf
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float a, d;
-          const float sa = __uint_as_float(v[c * 32 + 2 * i]), sd = __uint_as_float(v[c * 32 + 2 * i + 1]);
-          if (CAP) {
-            // a masked entry keeps its -inf through the cap
-            float xa, xd;
-            unpack2(fma2(pack2(sa, sd), scale2, 0ull), xa, xd);
-            const float off = p.score.cap_out + neg_m;
-            a = ex2_approx(fmaf(-2.0f * p.score.cap_out, paged_rcp(1.0f + ex2_approx(xa)), off));
-            d = ex2_approx(fmaf(-2.0f * p.score.cap_out, paged_rcp(1.0f + ex2_approx(xd)), off));
-            if (masked_tile) {
-              a = sa == -CUDART_INF_F ? 0.0f : a;
-              d = sd == -CUDART_INF_F ? 0.0f : d;
-            }
-          } else {
-            float xa, xd;
-            unpack2(fma2(pack2(sa, sd), scale2, negm2), xa, xd);
-            a = ex2_approx(xa);
-            d = ex2_approx(xd);
+          for (int c = 0; c < FA_BN / 32; ++c) {
+            // bits of the columns [c_lo, c_hi] among these 32
+            const int h = c_hi - c * 32, l = c_lo - c * 32;
+            uint32_t bits = h >= 31 ? ~0u : h < 0 ? 0u : (2u << h) - 1u;
+            bits &= l <= 0 ? ~0u : l > 31 ? 0u : ~0u << l;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((bits >> i) & 1u)) v[c * 32 + i] = hidden;
           }
-          ls2[i & 3] = add2(ls2[i & 3], pack2(a, d));
-          pk[i] = F16 ? pack_f16x2(a, d) : pack_bf16x2(a, d);
         }
-        tmem_st_32x32b_x16(tS + c * 16, pk);
+        float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+        for (int i = 0; i < FA_BN; i += 8) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            mx[u] = max3(mx[u], __uint_as_float(v[i + 2 * u]), __uint_as_float(v[i + 2 * u + 1]));
+        }
+        const float rmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        bool poly = false;                    // the cap's polynomial serves every score of the warp's rows
+        if (CAP) {
+          float mn[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < FA_BN; i += 4)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) mn[u] = fminf(mn[u], __uint_as_float(v[i + u]));
+          const float big = fmaxf(rmax, -fminf(fminf(mn[0], mn[1]), fminf(mn[2], mn[3])));
+          poly = __all_sync(0xffffffffu, big * cap_arg <= 2.0f * 1.4426950408889634f * CAP_POLY_MAX);
+        }
+        // the score grows with s: the largest s has the largest score (the cap maps -inf to -cap: kept apart)
+        const float m_tile = rmax == -CUDART_INF_F ? rmax
+                             : CAP             ? paged_score<true>(ScoreParams{scale, cap_arg, p.score.cap_out}, rmax)
+                                               : rmax * scale;
+        const float m_new = fmaxf(m_run, m_tile);
+        bool need = false;
+        float alpha = 1.0f;
+        if (m_run == -CUDART_INF_F) {
+          m_run = m_new;                       // nothing seen before: O and l are zero
+        } else if (m_new - m_run > FA_RESCALE_THRESHOLD) {
+          need = true;
+          alpha = ex2_approx(m_run - m_new);
+          l_run *= alpha;
+          m_run = m_new;
+        }
+        if (__any_sync(0xffffffffu, need)) {
+          // S_t(j) complete implies O_t += P_t(j-1) V(j-1) complete (MMAs retire in issue order)
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(tO + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x32b_x32(tO + c * 32, o);
+          }
+        }
+        const float neg_m = m_run == -CUDART_INF_F ? 0.0f : -m_run;
+        uint64_t ls2[4] = {0ull, 0ull, 0ull, 0ull};
+        // P = exp2(score - m) of 32 columns at a time, to 16 bits, over S's columns
+        auto probabilities = [&](auto&& score_minus_m) {
+#pragma unroll
+          for (int c = 0; c < FA_BN / 32; ++c) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float xa, xd;
+              unpack2(score_minus_m(pack2(__uint_as_float(v[c * 32 + 2 * i]), __uint_as_float(v[c * 32 + 2 * i + 1]))), xa, xd);
+              const float a = ex2_approx(xa), d = ex2_approx(xd);
+              ls2[i & 3] = add2(ls2[i & 3], pack2(a, d));
+              pk[i] = MF16 ? pack_f16x2(a, d) : pack_bf16x2(a, d);
+            }
+            tmem_st_32x32b_x16(tS + c * 16, pk);
+          }
+        };
+        const uint64_t negm2 = pack2(neg_m, neg_m);
+        if (!CAP) {
+          const uint64_t scale2 = pack2(scale, scale);
+          probabilities([&](uint64_t s2) { return fma2(s2, scale2, negm2); });
+        } else if (poly) {
+          const float a = cap_arg * (0.5f / 1.4426950408889634f);      // scale / c
+          const uint64_t a2 = pack2(a, a), zero2 = 0ull;
+          uint64_t k2[6];
+#pragma unroll
+          for (int i = 0; i < 6; ++i) k2[i] = pack2(p.cap_poly[i], p.cap_poly[i]);
+          probabilities([&](uint64_t s2) {
+            const uint64_t x = fma2(s2, a2, zero2), y = fma2(x, x, zero2);
+            uint64_t h = fma2(k2[5], y, k2[4]);
+            h = fma2(h, y, k2[3]);
+            h = fma2(h, y, k2[2]);
+            h = fma2(h, y, k2[1]);
+            h = fma2(h, y, k2[0]);
+            return fma2(x, h, negm2);
+          });
+        } else {
+          const float off = p.score.cap_out + neg_m;
+          probabilities([&](uint64_t s2) {
+            float sa, sd;
+            unpack2(s2, sa, sd);
+            float xa = fmaf(-2.0f * p.score.cap_out, paged_rcp(1.0f + ex2_approx(sa * cap_arg)), off);
+            float xd = fmaf(-2.0f * p.score.cap_out, paged_rcp(1.0f + ex2_approx(sd * cap_arg)), off);
+            if (sa == -CUDART_INF_F) xa = -CUDART_INF_F;               // masked: stays out, cap or not
+            if (sd == -CUDART_INF_F) xd = -CUDART_INF_F;
+            return pack2(xa, xd);
+          });
+        }
+        float ls[4];
+        {
+          const uint64_t s01 = add2(ls2[0], ls2[1]), s23 = add2(ls2[2], ls2[3]);
+          unpack2(s01, ls[0], ls[1]);
+          unpack2(s23, ls[2], ls[3]);
+        }
+        l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        tmem_wait_st();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p_full + t * 8);
       }
-      float ls[4];
-      {
-        const uint64_t s01 = add2(ls2[0], ls2[1]), s23 = add2(ls2[2], ls2[3]);
-        unpack2(s01, ls[0], ls[1]);
-        unpack2(s23, ls[2], ls[3]);
-      }
-      l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-      tmem_wait_st();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_p_full + t * 8);
-    }
-    // ------------------------------- epilogue ----------------------------------
-    // rows of this warp that are tokens, staged in Q_t's shared memory (free: all S_t MMAs retired) and copied out
-    // 16 lanes (D = 64: 8) to a row
-    if (ok && n_mine > 0) ok = mbar_wait(wctx, bar_o_done + t * 8, 0, 31);
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
+      // ------------------------------- the part's result ----------------------------------
+      if (ok && n_mine > 0) ok = wait_all(bar_o_done + t * 8, items & 1, 31);
+      if (!ok) break;
       tc_fence_after_sync();
-      const float inv_l = l_run == 0.0f ? 0.0f : (FP4 ? p.out_scale : 1.0f) / l_run;
-      const uint32_t stage_row = sQ + t * TILE + (uint32_t)row * 128;
+      if (blind) {
+        m_run = -CUDART_INF_F;
+        l_run = 0.0f;
+      }
+      const bool whole = w.whole;
+      const float inv_l = !whole ? 1.0f : l_run == 0.0f ? 0.0f : (FP4 ? p.out_scale : 1.0f) / l_run;
+      float* part = p.part + ((long long)blockIdx.x * 2 + w.slot) * part_floats(D);
+      const int ntok = w.tokens[t];
+      const long long out_row = w.row0 + t * p.tpt;
+      const int out_head = w.head * p.group;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         if (n_mine > 0) {
           tmem_ld_32x32b_x32(tO + c * 32, o);
           tmem_wait_ld();
-        } else {
+        }
+        if (n_mine == 0 || l_run == 0.0f) {        // whatever stands there, a row without a key is zero
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
+        if (whole) {
+          // to 16 bits, through shared memory, so that a store covers 64 neighbouring bytes of 8 rows and not 16 of 32
+          __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t w[4];
+          for (int e = 0; e < 4; ++e) {
+            uint32_t x[4];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float lo = __uint_as_float(o[e * 8 + 2 * x]) * inv_l;
-            const float hi = __uint_as_float(o[e * 8 + 2 * x + 1]) * inv_l;
-            w[x] = F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+            for (int k = 0; k < 4; ++k) {
+              const float lo = __uint_as_float(o[e * 8 + 2 * k]) * inv_l;
+              const float hi = __uint_as_float(o[e * 8 + 2 * k + 1]) * inv_l;
+              x[k] = F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+            }
+            st_shared_v4(s_out + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4), x[0], x[1], x[2], x[3]);
           }
-          const uint32_t chunk = (uint32_t)((c & 1) * 4 + e);
-          st_shared_v4(stage_row + (c >> 1) * HALF + ((chunk ^ (uint32_t)(lane & 7)) << 4), w[0], w[1], w[2], w[3]);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int r = k * 8 + (lane >> 2), e = lane & 3, rt = (q * 32 + r) / p.group;
+            uint32_t x[4];
+            ld_shared_v4(s_out + r * 64 + ((e ^ ((r >> 1) & 3)) << 4), x);
+            if (rt < ntok)
+              *reinterpret_cast<uint4*>(p.out + (out_row + rt) * p.o_ts +
+                                        (long long)(out_head + q * 32 + r - rt * p.group) * p.o_hs + c * 32 + e * 8) =
+                  make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            reinterpret_cast<uint4*>(part)[(t * (D / 4) + c * 8 + e) * 128 + row] =
+                make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
         }
       }
-      __syncwarp();
-      constexpr int LPR = D / 8;                    // lanes per row
-      for (int i = lane / LPR; i < 32; i += 32 / LPR) {
-        const int r = q * 32 + i, rt = r / p.group;
-        if (rt >= ntok[t]) break;
-        const int c = lane % LPR;
-        uint32_t w[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "r"(sQ + t * TILE + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)));
-        uint16_t* dst = p.out + (long long)(sv.q0 + tok0[t] + rt) * p.o_ts +
-                        (long long)(head * p.group + r - rt * p.group) * p.o_hs + c * 8;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (!whole) {
+        float* ml = part + 2 * 128 * D;
+        ml[t * 128 + row] = m_run;
+        ml[256 + t * 128 + row] = l_run;
+        // the parts of this item: this CTA's and the next ones' first
+        if (w.slot == 1 && warp == 4 && lane == 0) p.desc[blockIdx.x] = make_int4(w.parts, w.b, w.pair, w.head);
       }
+      done_part(i);
+      if (n_mine > 0) ++items;
+      tc_fence_before_sync();
     }
   } else if (FP4 && warp >= 12) {
-    // ---------------------- NVFP4 rows to 16-bit operand tiles ----------------------
+    // ---------------------- NVFP4 rows to f16 operand tiles ----------------------
     reg_dealloc<56>();
     const int r = threadIdx.x - 384;                // key of the step
     constexpr int WORDS = D / 8;                    // packed words per row
     uint32_t wk[WORDS], wv[WORDS], sk[D / 64], sw[D / 64];
     const int slot_mask = (1 << p.batch.page_shift) - 1;
-    auto fetch = [&](int j, const uint8_t* pool, const long long (&st)[3], const uint8_t* spool, const long long (&sst)[3],
-                     uint32_t (&w)[WORDS], uint32_t (&s)[D / 64]) {
+    auto fetch = [&](const Part& w, int j, const uint8_t* pool, const long long (&st)[3], const uint8_t* spool,
+                     const long long (&sst)[3], uint32_t (&x)[WORDS], uint32_t (&s)[D / 64]) {
 #pragma unroll
-      for (int i = 0; i < WORDS; ++i) w[i] = 0;
+      for (int i = 0; i < WORDS; ++i) x[i] = 0;
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) s[i] = 0;
-      const int key = (j0 + j) * FA_BN + r;
-      if (j >= n_max || key < lo_key || key >= hi_all) return;    // unseen: zeros
-      const int pg = page_of(p.batch, b, key, status);
+      const int key = w.key0 + j * FA_BN + r;
+      if (key < w.lo || key >= w.hi) return;        // unseen: zeros
+      const int pg = page_of(p.batch, w.b, key, status);
       if (pg >= p.batch.num_pages) return;
-      const uint8_t* row = pool + pg * st[0] + head * st[1] + (key & slot_mask) * st[2];
-      const uint8_t* srow = spool + pg * sst[0] + head * sst[1] + (key & slot_mask) * sst[2];
+      const uint8_t* src = pool + pg * st[0] + w.head * st[1] + (key & slot_mask) * st[2];
+      const uint8_t* ssrc = spool + pg * sst[0] + w.head * sst[1] + (key & slot_mask) * sst[2];
 #pragma unroll
       for (int i = 0; i < WORDS / 4; ++i) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(row) + i);
-        w[4 * i] = x.x;
-        w[4 * i + 1] = x.y;
-        w[4 * i + 2] = x.z;
-        w[4 * i + 3] = x.w;
+        const uint4 y = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        x[4 * i] = y.x;
+        x[4 * i + 1] = y.y;
+        x[4 * i + 2] = y.z;
+        x[4 * i + 3] = y.w;
       }
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) s[i] = __ldg(reinterpret_cast<const uint32_t*>(srow) + i);
+      for (int i = 0; i < D / 64; ++i) s[i] = __ldg(reinterpret_cast<const uint32_t*>(ssrc) + i);
     };
-    auto expand = [&](uint32_t dst, const uint32_t (&w)[WORDS], const uint32_t (&s)[D / 64]) {
+    auto expand = [&](uint32_t dst, const uint32_t (&x)[WORDS], const uint32_t (&s)[D / 64]) {
 #pragma unroll
-      for (int i = 0; i < WORDS; ++i) {
-        const uint32_t sc = expand_scale<F16>(s[i / 8] >> (8 * ((i / 2) & 3)));
-        uint32_t o[4];
-        expand8<F16>(w[i], sc, o);
-        st_shared_v4(dst + (i >> 3) * HALF + r * 128 + (((i & 7) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+      for (int i = 0; i < WORDS; i += 4) {           // two scales
+        uint32_t two;
+        asm("{.reg .b16 h; cvt.u16.u32 h, %1; cvt.rn.f16x2.e4m3x2 %0, h;}" : "=r"(two) : "r"((s[i / 8] >> (4 * (i & 4))) & 0xffffu));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t o[4];
+          expand8(x[i + k], __byte_perm(two, two, k < 2 ? 0x1010 : 0x3232), o);
+          const int c = i + k;
+          st_shared_v4(dst + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
     };
-    fetch(0, p.k, p.k_st, p.ks, p.ks_st, wk, sk);
-    fetch(0, p.v, p.v_st, p.vs, p.vs_st, wv, sw);
-    uint32_t stage = 0, phase = 0;
-    for (int j = 0; j < n_max; ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait(wctx, bar_k_empty + stage * 8, phase ^ 1, 10))) break;
-      expand(sK + stage * TILE, wk, sk);
-      if (lane == 0) mbar_arrive(bar_k_full + stage * 8);
-      fetch(j + 1, p.k, p.k_st, p.ks, p.ks_st, wk, sk);
-      if (!__all_sync(0xffffffffu, mbar_wait(wctx, bar_v_empty + stage * 8, phase ^ 1, 11))) break;
-      expand(sV + stage * TILE, wv, sw);
-      if (lane == 0) mbar_arrive(bar_v_full + stage * 8);
-      fetch(j + 1, p.v, p.v_st, p.vs, p.vs_st, wv, sw);
-      if (++stage == STAGES) { stage = 0; phase ^= 1; }
+    int it = 0;
+    bool ok = true;
+    int i = 0, n = 0;
+    auto open_part = [&]() {
+      for (; have_part(i); ++i) {
+        const Part& w = s_part[i % PART_RING];
+        n = max(w.steps[0], w.steps[1]);
+        if (n > 0) {
+          fetch(w, 0, p.k, p.k_st, p.ks, p.ks_st, wk, sk);
+          fetch(w, 0, p.v, p.v_st, p.vs, p.vs_st, wv, sw);
+          return true;
+        }
+        done_part(i);
+      }
+      return false;
+    };
+    while (ok && open_part()) {
+      const Part& w = s_part[i % PART_RING];
+      for (int j = 0; j < n; ++j, ++it) {
+        const uint32_t stage = it % STAGES, phase = (it / STAGES) & 1;
+        if (!wait_all(bar_k_empty + stage * 8, phase ^ 1, 10)) { ok = false; break; }
+        expand(sK + stage * TILE, wk, sk);
+        if (lane == 0) mbar_arrive(bar_k_full + stage * 8);
+        const bool more = j + 1 < n;
+        if (more) fetch(w, j + 1, p.k, p.k_st, p.ks, p.ks_st, wk, sk);
+        if (!wait_all(bar_v_empty + stage * 8, phase ^ 1, 11)) { ok = false; break; }
+        expand(sV + stage * TILE, wv, sw);
+        if (lane == 0) mbar_arrive(bar_v_full + stage * 8);
+        if (more) fetch(w, j + 1, p.v, p.v_st, p.vs, p.vs_st, wv, sw);
+      }
+      done_part(i++);
     }
   }
 
@@ -580,12 +909,57 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     tmem_dealloc(tmem_base, 512);
   }
   // The row-block kernel of the same call runs beside this one and writes other rows.  Whatever follows in the stream
-  // waits for this kernel only, so no CTA of it ends before that one has.
+  // waits for the last kernel of the call only, so no CTA here ends before that one has.
   grid_dep_wait();
 }
 
+// Adds the parts of the items that were cut, as the row-block kernel's merge does.  Thread = row; blockIdx.y = tile and
+// a quarter of the dimensions.
+template <int D, bool F16>
+__global__ void __launch_bounds__(128) fmha_paged_tile_merge_kernel(const __grid_constant__ TileParams p) {
+  grid_dep_wait();
+  const int4 d = p.desc[blockIdx.x];
+  if (d.x == 0) return;
+  const int t = blockIdx.y & 1, c0 = (blockIdx.y >> 1) * (D / 16);       // float4 columns c0 .. c0 + D / 16
+  const int row = threadIdx.x, tok = row / p.group;
+  const SeqView sv = seq_view(p.batch, d.y);
+  const int tok0 = (d.z * 2 + t) * p.tpt;
+  if (tok >= min(max(sv.n - tok0, 0), p.tpt)) return;
+  float m = -CUDART_INF_F, l = 0.0f;
+  float4 o[D / 16];
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+  for (int i = 0; i < d.x; ++i) {
+    const float* part = p.part + ((long long)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * part_floats(D);
+    const float pm = part[2 * 128 * D + t * 128 + row], pl = part[2 * 128 * D + 256 + t * 128 + row];
+    float4 v[D / 16];
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) v[c] = reinterpret_cast<const float4*>(part)[(t * (D / 4) + c0 + c) * 128 + row];
+    const float mn = fmaxf(m, pm), mu = mn == -CUDART_INF_F ? 0.0f : mn;
+    const float wa = ex2_approx(m - mu), wb = ex2_approx(pm - mu);
+    m = mn;
+    l = l * wa + pl * wb;
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      o[c].x = o[c].x * wa + v[c].x * wb;
+      o[c].y = o[c].y * wa + v[c].y * wb;
+      o[c].z = o[c].z * wa + v[c].z * wb;
+      o[c].w = o[c].w * wa + v[c].w * wb;
+    }
+  }
+  const float inv = l == 0.0f ? 0.0f : p.out_scale / l;
+  uint16_t* dst = p.out + (long long)(sv.q0 + tok0 + tok) * p.o_ts +
+                  (long long)(d.w * p.group + row - tok * p.group) * p.o_hs + c0 * 4;
+#pragma unroll
+  for (int c = 0; c < D / 16; c += 2)
+    *reinterpret_cast<uint4*>(dst + c * 4) =
+        make_uint4(paged_pack16<F16>(o[c].x * inv, o[c].y * inv), paged_pack16<F16>(o[c].z * inv, o[c].w * inv),
+                   paged_pack16<F16>(o[c + 1].x * inv, o[c + 1].y * inv), paged_pack16<F16>(o[c + 1].z * inv, o[c + 1].w * inv));
+}
+
 template <int D, bool F16, bool CAP, bool FP4>
-int launch_tile(const PagedAttnArgs& a) {
+int launch_tile(const PagedAttnArgs& a, const PagedTilePlan& plan) {
   using L = TileSmem<D, FP4>;
   const b200h::DeviceInfo* di = b200h::device_info();
   if (!di) return B200_ERR_CUDA;
@@ -603,6 +977,10 @@ int launch_tile(const PagedAttnArgs& a) {
   p.out = static_cast<uint16_t*>(a.out);
   p.o_ts = a.o_ts;
   p.o_hs = a.o_hs;
+  p.out_scale = 1.0f;
+  for (int i = 0; i < 6; ++i) p.cap_poly[i] = CAP_POLY[i] * a.score.cap_out;
+  p.part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + a.tile_off);
+  p.desc = reinterpret_cast<int4*>(static_cast<char*>(a.workspace) + a.tile_off + plan.desc_off);
   const CUtensorMapDataType dt = F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap tmQ, tmK = {}, tmV = {};
   const uint64_t row = (uint64_t)D * 2;
@@ -612,9 +990,9 @@ int launch_tile(const PagedAttnArgs& a) {
                                      CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   if constexpr (FP4) {
-    p.score.scale_log2 *= c.k_global * 128.0f;      // the expanded operands are value * 2^-7
-    p.score.cap_arg *= c.k_global * 128.0f;
-    p.out_scale = c.v_global * 128.0f;
+    p.score.scale_log2 *= c.k_global;
+    p.score.cap_arg *= c.k_global;
+    p.out_scale = c.v_global;
     p.k = static_cast<const uint8_t*>(c.k);
     p.v = static_cast<const uint8_t*>(c.v);
     p.ks = static_cast<const uint8_t*>(c.k_scales);
@@ -635,14 +1013,8 @@ int launch_tile(const PagedAttnArgs& a) {
     B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
     attr_done.set(di->ordinal);
   }
-  // at most one partly filled pair per sequence that has rows for this kernel
-  const long long tokens = a.batch.tokens;
-  const long long some = std::min<long long>(a.batch.batch, tokens * p.group / (a.row_limit + 1LL));
-  const long long ctas = (tokens / (2 * p.tpt) + some) * p.kv_heads;
-  if (ctas > 0x7fffffffLL) return b200h::set_error(B200_ERR_INVALID, "paged_attention: grid too large");
-  if (ctas == 0) return B200_OK;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.gridDim = dim3(plan.ctas);
   cfg.blockDim = dim3(L::THREADS);
   cfg.dynamicSmemBytes = L::TOTAL;
   cfg.stream = a.stream;
@@ -652,16 +1024,29 @@ int launch_tile(const PagedAttnArgs& a) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tmQ, tmK, tmV, p, di->status));
+  cfg.gridDim = dim3(plan.ctas, 8);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = 0;
+  B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fmha_paged_tile_merge_kernel<D, F16>, p));
   return B200_OK;
 }
 
 }  // namespace
 }  // namespace b200
 
+PagedTilePlan b200_paged_tile_plan(int head_dim) {
+  PagedTilePlan pl;
+  pl.ctas = 148;
+  pl.desc_off = (size_t)pl.ctas * 2 * b200::part_floats(head_dim) * sizeof(float);
+  pl.bytes = pl.desc_off + (size_t)pl.ctas * sizeof(int4);
+  return pl;
+}
+
 int b200_paged_tile_dispatch(const PagedAttnArgs& a) {
   using namespace b200;
   const b200tile_paged_cache& c = *a.cache;
-#define B200_PT(D_, F_, C_, Q_) return launch_tile<D_, F_, C_, Q_>(a)
+  const PagedTilePlan plan = b200_paged_tile_plan(c.head_dim);
+#define B200_PT(D_, F_, C_, Q_) return launch_tile<D_, F_, C_, Q_>(a, plan)
 #define B200_PT_CAP(D_, F_, Q_) do { if (a.capped) B200_PT(D_, F_, true, Q_); B200_PT(D_, F_, false, Q_); } while (0)
 #define B200_PT_FMT(D_, F_) do { if (c.format) B200_PT_CAP(D_, F_, true); B200_PT_CAP(D_, F_, false); } while (0)
   if (c.head_dim == 128 && a.dtype == 0) B200_PT_FMT(128, false);

@@ -110,7 +110,9 @@ int encode_tmap_pages(CUtensorMap* out, CUtensorMapDataType dtype, const void* b
   cuuint32_t box[4] = {box0, box1, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = fn(out, dtype, 4, const_cast<void*>(base), gdim, gstr, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  CU_TENSOR_MAP_SWIZZLE_128B,
+                  row >= 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return set_error(B200_ERR_CUDA, "cuTensorMapEncodeTiled(page pool) failed with CUresult %d (%d pages, %d heads, "
                      "%d slots, page pitch %llu)", (int)r, pages, heads, slots, (unsigned long long)bytes[2]);

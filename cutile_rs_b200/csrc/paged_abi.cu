@@ -87,6 +87,15 @@ int check_batch(const char* who, const b200tile_paged_cache* c, const b200tile_p
   return B200TILE_OK;
 }
 
+bool may_tile(long long max_q, int group) { return max_q * group > kTileRows && group <= 128; }
+
+// Workspace of the row-block kernel for sequences of up to `rows` query rows, a multiple of 256 bytes.
+size_t split_bytes(const b200tile_paged_cache* c, const b200tile_paged_batch* b, long long rows) {
+  const size_t n = b200_paged_split_plan(c->format, c->head_dim, c->kv_heads, b->batch, rows,
+                                         (long long)b->max_pages * c->page_size).bytes;
+  return (n + 255) & ~(size_t)255;
+}
+
 b200::PagedBatch device_batch(const b200tile_paged_cache* c, const b200tile_paged_batch* b, int tokens) {
   b200::PagedBatch p;
   p.table = b->block_table;
@@ -165,9 +174,11 @@ uint64_t b200tile_paged_attention_workspace_bytes(const b200tile_paged_cache* ca
   if (!cache || !batch || cache->kv_heads <= 0 || q_heads <= 0 || batch->batch <= 0 || batch->max_pages <= 0 ||
       batch->max_q_len <= 0 || cache->page_size <= 0 || cache->head_dim <= 0)
     return 0;
-  return b200_paged_split_plan(cache->format, cache->head_dim, cache->kv_heads, batch->batch,
-                               (long long)batch->max_q_len * (q_heads / cache->kv_heads),
-                               (long long)batch->max_pages * cache->page_size).bytes;
+  const int group = q_heads / cache->kv_heads;
+  const size_t all = split_bytes(cache, batch, (long long)batch->max_q_len * group);
+  if (!may_tile(batch->max_q_len, group)) return all;
+  // the tile kernel's part lies behind the row-block kernel's; without it (rows it cannot move) the latter takes all rows
+  return std::max(all, split_bytes(cache, batch, kTileRows) + b200_paged_tile_plan(cache->head_dim).bytes);
 }
 
 int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cache, const b200tile_paged_batch* batch,
@@ -217,9 +228,10 @@ int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cach
   a.window = window;
   a.workspace = workspace;
   a.stream = static_cast<cudaStream_t>(cu_stream);
-  const bool tiles = (long long)a.batch.max_q * group > kTileRows && group <= 128 && !misaligned(q, 16) &&
-                     !misaligned(out, 16) && !(a.q_ts % 8) && !(a.q_hs % 8) && !(a.o_ts % 8) && !(a.o_hs % 8) &&
-                     a.q_ts > 0 && a.q_hs > 0;
+  // the tile kernel moves rows by TMA and in 16-byte pieces; rows that do not lie so take row blocks, whatever their number
+  const bool tiles = may_tile(batch->max_q_len, group) && !misaligned(q, 16) && !misaligned(out, 16) && !(a.q_ts % 8) &&
+                     !(a.q_hs % 8) && !(a.o_ts % 8) && !(a.o_hs % 8) && a.q_ts > 0 && a.q_hs > 0;
+  a.tile_off = tiles ? split_bytes(cache, batch, kTileRows) : 0;
   a.row_limit = tiles ? kTileRows : 0x7fffffff;
   if (int rc = b200_paged_split_dispatch(a)) return rc;
   return tiles ? b200_paged_tile_dispatch(a) : B200TILE_OK;

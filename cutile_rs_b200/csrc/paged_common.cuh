@@ -108,6 +108,7 @@ struct PagedAttnArgs {
   int causal, window;
   int row_limit;                     // sequences with more query rows per K/V head are another kernel's
   void* workspace;
+  size_t tile_off;                   // the tile kernel's part of the workspace
   cudaStream_t stream;
 };
 
@@ -123,5 +124,10 @@ struct PagedSplitPlan {
 PagedSplitPlan b200_paged_split_plan(int format, int head_dim, int kv_heads, int batch, long long rows,
                                      long long max_keys);
 int b200_paged_split_dispatch(const PagedAttnArgs& a);
+struct PagedTilePlan {
+  int ctas;
+  size_t desc_off, bytes;
+};
+PagedTilePlan b200_paged_tile_plan(int head_dim);
 // Launched right behind the row-block kernel, whose rows it leaves alone, and runs beside it.
 int b200_paged_tile_dispatch(const PagedAttnArgs& a);

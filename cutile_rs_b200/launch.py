@@ -824,34 +824,41 @@ def linear_nvfp4_prepared(z: Tensor, x: Tensor, y: Tensor, x_scales: Tensor, y_s
     return z
 
 
-def _paged_rows(who: str, name: str, t: Tensor, tokens: int, heads: int, cache: PagedKvCache) -> None:
-    shape = t.shape
-    if len(shape) != 3 or shape[0] != tokens or shape[1] != heads or shape[2] != cache.head_dim:
-        raise KernelLaunchError(f"{who}: {name} is {shape}, expected [{tokens}, {heads}, {cache.head_dim}]")
+# The paged calls sit in decode loops, where a kernel takes a few microseconds: one comparison per tensor decides whether
+# it is what the call needs, and only a mismatch looks for the reason.
+def _paged_rows(who: str, name: str, t: Tensor, tokens: int, heads: int, cache: PagedKvCache, dt: str) -> int:
+    """Checks that ``t`` is [tokens, heads, D] of type ``dt`` beside the cache; the address of its {token, head} strides."""
+    if t.shape != [tokens, heads, cache.head_dim]:
+        raise KernelLaunchError(f"{who}: {name} is {t.shape}, expected [{tokens}, {heads}, {cache.head_dim}]")
     if t.strides[2] != 1:
         raise KernelLaunchError(f"{who}: the head vectors of {name} must be contiguous")
+    if t.dtype != dt:
+        raise KernelLaunchError(f"{who}: the tensors have different element types, {name} is {t.dtype} beside {dt}")
     if t.storage.device != cache.device:
         raise KernelLaunchError(f"{who}: {name} is on {t.storage.device}, the cache on {cache.device}")
+    pair = t.__dict__.get("_row_strides")
+    if pair is None:
+        pair = t._row_strides = _i64x2(t.strides[0], t.strides[1])
+        t._row_strides_at = ctypes.addressof(pair)
+    return t._row_strides_at
 
 
-def _paged_dtype(who: str, cache: PagedKvCache, tensors) -> str:
-    dt = tensors[0].dtype
-    if any(t.dtype != dt for t in tensors):
-        raise KernelLaunchError(f"{who}: the tensors have different element types {[t.dtype for t in tensors]}")
+def _paged_dtype(who: str, cache: PagedKvCache, dt: str) -> bytes:
     if cache.dtype is not None and cache.dtype != dt:
         raise KernelLaunchError(f"{who}: the cache holds {cache.dtype}, the tensors {dt}")
-    return dt
+    return dt.encode()
 
 
 def _paged_stream(who: str, cache: PagedKvCache, batch: PagedBatch, stream: Optional[torch.cuda.Stream]) -> int:
-    if batch.device != cache.device:
-        raise KernelLaunchError(f"{who}: the batch is on {batch.device}, the cache on {cache.device}")
-    if cache.device.type != "cuda" or torch.cuda.current_device() != cache.device.index:
-        raise KernelLaunchError(f"{who}: the cache is on {cache.device}, which is not the current device")
+    dev = cache.device
+    if batch.device != dev:
+        raise KernelLaunchError(f"{who}: the batch is on {batch.device}, the cache on {dev}")
+    if dev.type != "cuda" or torch.cuda.current_device() != dev.index:
+        raise KernelLaunchError(f"{who}: the cache is on {dev}, which is not the current device")
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
-    if stream.device != cache.device:
-        raise KernelLaunchError(f"{who}: the stream is on {stream.device}, the cache on {cache.device}")
+        return torch._C._cuda_getCurrentRawStream(dev.index)
+    if stream.device != dev:
+        raise KernelLaunchError(f"{who}: the stream is on {stream.device}, the cache on {dev}")
     return stream.cuda_stream
 
 
@@ -863,30 +870,26 @@ def paged_kv_append(cache: PagedKvCache, batch: PagedBatch, k: Tensor, v: Tensor
     position * inv_freq [rotary_dim / 2] f32 on the way; without ``inv_freq`` nothing is rotated."""
     who = "paged_kv_append"
     lib = _lib.load()
-    tokens, heads = k.shape[0], cache.kv_heads
-    _paged_rows(who, "k", k, tokens, heads, cache)
-    _paged_rows(who, "v", v, tokens, heads, cache)
-    tensors, q_heads = [k, v], 0
+    tokens, heads, dt = k.shape[0], cache.kv_heads, k.dtype
+    ks, vs = _paged_rows(who, "k", k, tokens, heads, cache, dt), _paged_rows(who, "v", v, tokens, heads, cache, dt)
+    qp = qop = qs = qos = f = None
+    q_heads = rot = 0
     if (q is None) != (q_out is None):
         raise KernelLaunchError(f"{who}: q and q_out are given together or not at all")
     if q is not None:
         q_heads = q.shape[1] if len(q.shape) == 3 else 0
-        _paged_rows(who, "q", q, tokens, q_heads, cache)
-        _paged_rows(who, "q_out", q_out, tokens, q_heads, cache)
-        tensors += [q, q_out]
-    dt = _paged_dtype(who, cache, tensors)
-    rot = 0
+        qs, qos = _paged_rows(who, "q", q, tokens, q_heads, cache, dt), _paged_rows(who, "q_out", q_out, tokens, q_heads,
+                                                                                   cache, dt)
+        qp, qop = q.storage.data_ptr(), q_out.storage.data_ptr()
     if inv_freq is not None:
         if inv_freq.dtype != "f32" or len(inv_freq.shape) != 1 or inv_freq.strides[0] != 1 or \
                 inv_freq.storage.device != cache.device:
             raise KernelLaunchError(f"{who}: inv_freq must be a contiguous f32 vector on {cache.device}")
         rot = 2 * inv_freq.shape[0]
-    s = _paged_stream(who, cache, batch, stream)
-    rc = lib.b200tile_paged_kv_append(
-        dt.encode(), cache.c, batch.c, q.cu_deviceptr() if q is not None else None, k.cu_deviceptr(), v.cu_deviceptr(),
-        q_out.cu_deviceptr() if q is not None else None, inv_freq.cu_deviceptr() if rot else None, tokens, q_heads, rot,
-        _i64x2(q.strides[0], q.strides[1]) if q is not None else None, _i64x2(k.strides[0], k.strides[1]),
-        _i64x2(v.strides[0], v.strides[1]), _i64x2(q_out.strides[0], q_out.strides[1]) if q is not None else None, s)
+        f = inv_freq.storage.data_ptr()
+    dt = _paged_dtype(who, cache, dt)
+    rc = lib.b200tile_paged_kv_append(dt, cache.c, batch.c, qp, k.storage.data_ptr(), v.storage.data_ptr(), qop, f, tokens,
+                                      q_heads, rot, qs, ks, vs, qos, _paged_stream(who, cache, batch, stream))
     if rc:
         raise KernelLaunchError(lib.b200tile_last_error().decode())
 
@@ -897,14 +900,11 @@ def paged_kv_gather(k_out: Tensor, v_out: Tensor, cache: PagedKvCache, batch: Pa
     (``b200tile_paged_kv_gather``); with ``cu_q`` the running sum of ``kv_lens``, every sequence's whole cache."""
     who = "paged_kv_gather"
     lib = _lib.load()
-    tokens = k_out.shape[0]
-    _paged_rows(who, "k_out", k_out, tokens, cache.kv_heads, cache)
-    _paged_rows(who, "v_out", v_out, tokens, cache.kv_heads, cache)
-    dt = _paged_dtype(who, cache, [k_out, v_out])
-    s = _paged_stream(who, cache, batch, stream)
-    rc = lib.b200tile_paged_kv_gather(dt.encode(), cache.c, batch.c, k_out.cu_deviceptr(), v_out.cu_deviceptr(), tokens,
-                                      _i64x2(k_out.strides[0], k_out.strides[1]),
-                                      _i64x2(v_out.strides[0], v_out.strides[1]), s)
+    tokens, heads, dt = k_out.shape[0], cache.kv_heads, k_out.dtype
+    ks = _paged_rows(who, "k_out", k_out, tokens, heads, cache, dt)
+    vs = _paged_rows(who, "v_out", v_out, tokens, heads, cache, dt)
+    rc = lib.b200tile_paged_kv_gather(_paged_dtype(who, cache, dt), cache.c, batch.c, k_out.storage.data_ptr(),
+                                      v_out.storage.data_ptr(), tokens, ks, vs, _paged_stream(who, cache, batch, stream))
     if rc:
         raise KernelLaunchError(lib.b200tile_last_error().decode())
     return k_out, v_out
@@ -927,21 +927,20 @@ def paged_attention(out: Tensor, q: Tensor, cache: PagedKvCache, batch: PagedBat
     taken from the torch caching allocator."""
     who = "paged_attention"
     lib = _lib.load()
-    tokens = q.shape[0]
+    tokens, dt = q.shape[0], q.dtype
     q_heads = q.shape[1] if len(q.shape) == 3 else 0
-    _paged_rows(who, "q", q, tokens, q_heads, cache)
-    _paged_rows(who, "out", out, tokens, q_heads, cache)
-    dt = _paged_dtype(who, cache, (q, out))
+    qs = _paged_rows(who, "q", q, tokens, q_heads, cache, dt)
+    os = _paged_rows(who, "out", out, tokens, q_heads, cache, dt)
+    dt = _paged_dtype(who, cache, dt)
     s = _paged_stream(who, cache, batch, stream)
     if workspace is None:
         with torch.cuda.stream(stream or torch.cuda.current_stream()):
             workspace = paged_attention_workspace(cache, batch, q_heads)
     elif workspace.device != cache.device or not workspace.is_contiguous():
         raise KernelLaunchError(f"{who}: the workspace must be contiguous on {cache.device}")
-    rc = lib.b200tile_paged_attention(dt.encode(), cache.c, batch.c, q.cu_deviceptr(), out.cu_deviceptr(), tokens, q_heads,
-                                      _i64x2(q.strides[0], q.strides[1]), _i64x2(out.strides[0], out.strides[1]),
-                                      qk_scale, int(causal), window, softcap, workspace.data_ptr(),
-                                      workspace.numel() * workspace.element_size(), s)
+    rc = lib.b200tile_paged_attention(dt, cache.c, batch.c, q.storage.data_ptr(), out.storage.data_ptr(), tokens, q_heads,
+                                      qs, os, qk_scale, int(causal), window, softcap, workspace.data_ptr(),
+                                      workspace.nbytes, s)
     if rc:
         raise KernelLaunchError(lib.b200tile_last_error().decode())
     return out

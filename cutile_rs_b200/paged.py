@@ -58,7 +58,7 @@ class PagedKvCache:
         c.k_global, c.v_global, c.format = float(k_global), float(v_global), int(fp4)
         c.num_pages, c.kv_heads, c.page_size, c.head_dim = self.num_pages, self.kv_heads, self.page_size, self.head_dim
         self._struct = c
-        self.c = ctypes.pointer(c)
+        self.c = ctypes.addressof(c)      # what the C ABI takes
 
 
 class PagedBatch:
@@ -83,4 +83,4 @@ class PagedBatch:
         c.cu_q, c.kv_lens = cu_q.data_ptr(), kv_lens.data_ptr()
         c.batch, c.max_pages, c.max_q_len = self.batch, self.max_pages, self.max_q_len
         self._struct = c
-        self.c = ctypes.pointer(c)
+        self.c = ctypes.addressof(c)      # what the C ABI takes

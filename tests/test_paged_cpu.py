@@ -16,13 +16,13 @@ def _cache(**kw):
              k_scale_strides=I3(512, 128, 8), v_scale_strides=I3(512, 128, 8), k_global=1.0, v_global=1.0, format=0,
              num_pages=4, kv_heads=4, page_size=16, head_dim=128)
     d.update(kw)
-    return _lib.PagedCacheC(**d)
+    return ctypes.pointer(_lib.PagedCacheC(**d))
 
 
 def _batch(**kw):
     d = dict(block_table=P, block_table_pitch=8, cu_q=P, kv_lens=P, batch=2, max_pages=8, max_q_len=4)
     d.update(kw)
-    return _lib.PagedBatchC(**d)
+    return ctypes.pointer(_lib.PagedBatchC(**d))
 
 
 def _attend(c, b, dtype=b"bf16", q=P, out=P, tokens=4, heads=8, qs=I2(1024, 128), os=I2(1024, 128), scale=0.1, causal=1,
