@@ -30,6 +30,15 @@
 namespace b200 {
 namespace {
 
+// c log2e tanh(x), x = s scale / c, as an odd polynomial in x with c log2e folded into the coefficients: the Chebyshev
+// interpolant of tanh(sqrt u) / sqrt u on [0, 0.4^2], off by at most 4.5e-8 for |x| <= 0.4.  Scores are a small part of the
+// cap almost always; steps with a larger one take exp2 and a reciprocal instead, which triples the load of the
+// special-function unit that bounds the softmax (8.2 against 2.6 thousand cycles a step).
+constexpr float CAP_POLY_MAX = 0.4f;
+constexpr int CAP_POLY_N = 4;
+constexpr float CAP_POLY[CAP_POLY_N] = {0.9999998807907104f, -0.33331355452537537f, 0.13270874321460724f,
+                                        -0.04754934832453728f};
+
 struct TileParams {
   PagedBatch batch;
   ScoreParams score;
@@ -38,8 +47,9 @@ struct TileParams {
   int box_rows;                      // keys per K/V box
   uint16_t* out;
   long long o_ts, o_hs;
+  int wide_out;                      // the output's rows lie on 32-byte boundaries
   float out_scale;
-  float cap_poly[6];                 // CAP_POLY * c log2e
+  float cap_poly[CAP_POLY_N];        // CAP_POLY * c log2e
   float* part;                       // two slots per CTA
   int4* desc;                        // one per CTA
   // FP4 operands: byte strides
@@ -50,10 +60,9 @@ struct TileParams {
 // A part: O as [2 tiles][D / 4][128 rows] float4 (lanes = rows, so that stores and loads are full lines), then
 // [2][128] maxima and [2][128] sums.
 __host__ __device__ constexpr int part_floats(int d) { return 2 * 128 * (d + 2); }
-// Starting and ending an item costs about as much as this many steps of 128 keys: the line that is cut into runs counts
-// them in front of every item's steps.
-constexpr int ITEM_COST = 2;
-constexpr int MIN_RUN = 6;
+// Starting and ending an item costs about as much as this many keys.
+constexpr int ITEM_COST = 256;
+constexpr int MIN_RUN = 768;         // keys: a shorter run would be mostly start-up
 constexpr int PART_RING = 4;         // parts known ahead of their turn
 
 template <int D, bool FP4>
@@ -70,8 +79,7 @@ struct TileSmem {
   // o_done[2], part_full[R], part_free[R]
   static constexpr int NUM_BARS = 6 + 4 * KV_STAGES + 6 + 2 * PART_RING;
   static constexpr int OFF_MISC = (OFF_BAR + NUM_BARS * 8 + 15) / 16 * 16;
-  static constexpr int OFF_OUT = OFF_MISC + 16;      // 32 rows x 64 bytes per softmax warp: output on its way to memory
-  static constexpr int TOTAL = OFF_OUT + 8 * 2048 + 1024;
+  static constexpr int TOTAL = OFF_MISC + 16 + 1024;
   static constexpr int THREADS = FP4 ? 512 : 384;
 };
 
@@ -81,6 +89,11 @@ __device__ __forceinline__ void tma_load_4d_tile(uint32_t dst, const void* desc,
       " [%0], [%1, {%3, %4, %5, %6}], [%2];"
       ::"r"(dst), "l"(desc), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
+}
+__device__ __forceinline__ float absmax3(float a, float b, float c) {
+  float d;
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void st_shared_v4(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -109,22 +122,53 @@ __device__ __forceinline__ PairSpan pair_span(const TileParams& p, const SeqView
   return x;
 }
 
-// Place on the line of all steps.
+// The line that is cut into runs is measured in keys: an item of pair i is ITEM_COST plus the keys its rows can see at
+// most, span(i) = min(base + (i + 1) tokens, top) for a causal sequence, whose sums have a closed form; so a warp finds
+// any place on the line with a few divisions, whatever the number of pairs.  A part's share of the item's length is its
+// share of the item's steps.
+struct SeqLine {
+  long long base, slope, top;        // span(i) = min(base + i slope, top)
+  int pairs;
+  int bend;                          // pairs below the top
+};
+__device__ __forceinline__ SeqLine seq_line(const TileParams& p, const SeqView& s) {
+  SeqLine x;
+  x.pairs = seq_pairs(p, s);
+  const int tokens = 2 * p.tpt;
+  x.slope = p.causal ? tokens : 0;
+  x.base = p.causal ? max(0, s.pos0) + tokens : s.len;
+  x.top = p.causal && p.window > 0 ? (long long)p.window + tokens : (1ll << 40);
+  x.bend = x.top <= x.base ? 0 : x.slope == 0 ? x.pairs : (int)min((long long)x.pairs, (x.top - x.base) / x.slope + 1);
+  return x;
+}
+__device__ __forceinline__ long long line_len(const SeqLine& x, int i) {    // of one item of pair i
+  return ITEM_COST + (i < x.bend ? x.base + i * x.slope : x.top);
+}
+__device__ __forceinline__ long long line_sum(const SeqLine& x, int n) {    // of the first n pairs, one item each
+  const long long k = min(n, x.bend);
+  return (long long)n * ITEM_COST + k * x.base + x.slope * (k * (k - 1) / 2) + (n - k) * x.top;
+}
+
+// Place on the line.
 struct Walk {
   long long u, u_end;
-  int b, pairs, pair, head;
+  long long at, len;                 // place in the item and the item's length
+  int b, pair, head;
   SeqView sv;
+  SeqLine line;
   PairSpan sp;
-  int at;                            // place in the item, ITEM_COST + step
   int a0, a1;                        // steps of this part, relative to sp.j0
-  __device__ __forceinline__ int left() const { return (int)min((long long)(ITEM_COST + sp.steps - at), u_end - u); }
-  // steps of the part at `at`; none if the run ends within the item's cost: the next CTA begins the item then
+  __device__ __forceinline__ long long left() const { return min(len - at, u_end - u); }
+  // steps of the part at `at`; false if it is an item's beginning too short for a step: the next CTA begins it then
   __device__ __forceinline__ bool cut() {
-    a0 = max(0, at - ITEM_COST);
-    a1 = max(0, at + left() - ITEM_COST);
-    if (a1 > a0) return true;
-    u = u_end;
-    return false;
+    a0 = (int)(at * sp.steps / len);
+    a1 = (int)((at + left()) * sp.steps / len);
+    return a1 > 0;
+  }
+  __device__ __forceinline__ void open(const TileParams& p) {
+    sp = pair_span(p, sv, pair);
+    len = line_len(line, pair);
+    at = 0;
   }
   __device__ __forceinline__ void next(const TileParams& p) {
     u += left();
@@ -132,7 +176,7 @@ struct Walk {
     at = 0;                          // the run goes on, so the item has ended
     if (++head == p.kv_heads) {
       head = 0;
-      if (++pair == pairs) {
+      if (++pair == line.pairs) {
         pair = 0;
         do {
           if (++b >= p.batch.batch) {
@@ -140,14 +184,65 @@ struct Walk {
             return;
           }
           sv = seq_view(p.batch, b);
-          pairs = seq_pairs(p, sv);
-        } while (pairs == 0);
+          line = seq_line(p, sv);
+        } while (line.pairs == 0);
       }
-      sp = pair_span(p, sv, pair);
+      open(p);
     }
-    cut();
+    if (!cut()) u = u_end;
   }
 };
+
+// The line's length, by one warp.
+__device__ __forceinline__ long long whole_line(const TileParams& p, int lane) {
+  long long mine = 0;
+  for (int b = lane; b < p.batch.batch; b += 32) {
+    const SeqLine x = seq_line(p, seq_view(p.batch, b));
+    mine += line_sum(x, x.pairs);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  return mine * p.kv_heads;
+}
+// The item at place u < u_end <= the line's length; all lanes together, the result in all of them.
+__device__ __forceinline__ void find_place(const TileParams& p, int lane, Walk& w) {
+  long long before = 0;                            // of the sequences already passed
+  for (int b0 = 0; b0 < p.batch.batch; b0 += 32) {
+    long long mine = 0;
+    if (b0 + lane < p.batch.batch) {
+      const SeqLine x = seq_line(p, seq_view(p.batch, b0 + lane));
+      mine = line_sum(x, x.pairs) * p.kv_heads;
+    }
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    const uint32_t past = __ballot_sync(0xffffffffu, before + inc > w.u);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      before += __shfl_sync(0xffffffffu, inc - mine, l);
+      w.b = b0 + l;
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  w.sv = seq_view(p.batch, w.b);
+  w.line = seq_line(p, w.sv);
+  const long long rel = w.u - before;
+  int lo = 0, hi = w.line.pairs - 1;               // the last pair that begins at or before rel
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (line_sum(w.line, mid) * p.kv_heads <= rel) lo = mid;
+    else hi = mid - 1;
+  }
+  w.pair = lo;
+  w.open(p);
+  const long long in_pair = rel - line_sum(w.line, lo) * p.kv_heads;
+  w.head = (int)(in_pair / w.len);
+  w.at = in_pair - w.head * w.len;
+}
 
 // One part of an item as the roles need it.  The loader warp walks the run and hands the parts to the others through a
 // ring in shared memory: the walk's divisions and loads happen once, ahead of time, instead of in every role between
@@ -182,7 +277,7 @@ __device__ __forceinline__ Part make_part(const TileParams& p, const Walk& w, lo
   }
   x.whole = w.a0 == 0 && w.a1 == w.sp.steps;
   x.slot = w.a0 == 0 ? 1 : 0;        // an item's first part, or the continuation of an earlier CTA's
-  x.parts = 1 + (int)((w.sp.steps - w.a1 + per - 1) / per);   // beyond the cost, every later place is a step
+  x.parts = 1 + (int)((w.len - w.at - w.left() + per - 1) / per);
   return x;
 }
 
@@ -195,12 +290,6 @@ __device__ __forceinline__ void expand8(uint32_t w, uint32_t scale, uint32_t (&o
   for (int i = 0; i < 4; ++i) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(o[i]) : "r"(o[i]), "r"(scale));
 }
 
-// c log2e tanh(s a) as an odd polynomial in s a with c log2e folded into the coefficients: the Chebyshev interpolant of tanh(sqrt u) / sqrt u on [0, 0.75^2], off by at most 4.5e-8 for |s a| <= 0.75.  Scores are a
-// small part of the cap almost always; steps with a larger one take exp2 and a reciprocal instead, which triples the load
-// of the special-function unit that bounds the softmax.
-constexpr float CAP_POLY_MAX = 0.75f;
-constexpr float CAP_POLY[6] = {1.0f, -0.33332952857017517f, 0.13325339555740356f, -0.05334111675620079f,
-                               0.019576216116547585f, -0.004711522255092859f};
 
 template <int D, bool F16, bool CAP, bool FP4>
 __global__ void __launch_bounds__(FP4 ? 512 : 384, 1)
@@ -212,121 +301,21 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   constexpr bool MF16 = F16 || FP4;               // element type of the products
   constexpr bool CONVERT = FP4 && !F16;           // bf16 queries for f16 products
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int s_first[THREADS];
-  __shared__ long long s_line[THREADS], s_warp[THREADS / 32], s_per;
   __shared__ Walk s_walk;
   __shared__ Part s_part[PART_RING];
+  __shared__ long long s_row_off[FA_BM];          // element offset of a tile's row in the output, from its first token
+  __shared__ int s_row_tok[FA_BM];                // its token
   __shared__ float s_unit[CONVERT ? 2 : 1][CONVERT ? 2 : 1][CONVERT ? 128 : 1];   // [item parity][tile][row]
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge, which waits for this grid
 
-  // ---- this CTA's run ----
-  auto block_scan = [&](long long mine, long long& total) {   // exclusive prefix over the threads
-    long long inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
-    }
-    __syncthreads();
-    if (lane == 31) s_warp[warp] = inc;
-    __syncthreads();
-    long long before = 0;
-    total = 0;
-    for (int w = 0; w < THREADS / 32; ++w) {
-      if (w < warp) before += s_warp[w];
-      total += s_warp[w];
-    }
-    return before + inc - mine;
-  };
-  {
-    Walk first;
-    const int per_b = (p.batch.batch + THREADS - 1) / THREADS;
-    long long mine = 0, total;
-    for (int i = threadIdx.x * per_b; i < min(p.batch.batch, (int)(threadIdx.x + 1) * per_b); ++i)
-      mine += seq_pairs(p, seq_view(p.batch, i));
-    s_first[threadIdx.x] = (int)block_scan(mine, total);
-    __syncthreads();
-    const int all_pairs = (int)total;
-    // sequence and pair at position `at` of the list of pairs
-    auto pair_at = [&](int at, Walk& w) {
-      int lo = 0, hi = THREADS - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s_first[mid] <= at) lo = mid;
-        else hi = mid - 1;
-      }
-      int seen = s_first[lo];
-      w.b = lo * per_b;
-      w.sv = seq_view(p.batch, w.b);
-      w.pairs = seq_pairs(p, w.sv);
-      while (seen + w.pairs <= at && w.b + 1 < p.batch.batch) {
-        seen += w.pairs;
-        w.sv = seq_view(p.batch, ++w.b);
-        w.pairs = seq_pairs(p, w.sv);
-      }
-      w.pair = at - seen;
-    };
-    auto step_pair = [&](Walk& w) {                // to the next pair of the list, if there is one
-      if (++w.pair < w.pairs) return;
-      w.pair = 0;
-      do {
-        if (w.b + 1 >= p.batch.batch) return;
-        w.sv = seq_view(p.batch, ++w.b);
-        w.pairs = seq_pairs(p, w.sv);
-      } while (w.pairs == 0);
-    };
-    const int per_p = (all_pairs + THREADS - 1) / THREADS;
-    const int p_begin = threadIdx.x * per_p, p_end = min(all_pairs, p_begin + per_p);
-    mine = 0;
-    if (p_begin < p_end) {
-      Walk w;
-      pair_at(p_begin, w);
-      for (int i = p_begin; i < p_end; ++i) {
-        mine += (long long)(ITEM_COST + pair_span(p, w.sv, w.pair).steps) * p.kv_heads;
-        step_pair(w);
-      }
-    }
-    s_line[threadIdx.x] = block_scan(mine, total);
-    __syncthreads();
-    long long per = (total + gridDim.x - 1) / gridDim.x;
-    if (per < MIN_RUN) per = MIN_RUN;
-    first.u = blockIdx.x * per;
-    first.u_end = min(total, first.u + per);
-    if (threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
-    if (first.u >= first.u_end) {
-      grid_dep_wait();
-      return;
-    }
-    int lo = 0, hi = THREADS - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_line[mid] <= first.u) lo = mid;
-      else hi = mid - 1;
-    }
-    long long line = s_line[lo];
-    pair_at(lo * per_p, first);
-    first.sp = pair_span(p, first.sv, first.pair);
-    while (line + (long long)(ITEM_COST + first.sp.steps) * p.kv_heads <= first.u) {
-      line += (long long)(ITEM_COST + first.sp.steps) * p.kv_heads;
-      step_pair(first);
-      first.sp = pair_span(p, first.sv, first.pair);
-    }
-    const long long rel = first.u - line;
-    first.head = (int)(rel / (ITEM_COST + first.sp.steps));
-    first.at = (int)(rel - (long long)first.head * (ITEM_COST + first.sp.steps));
-    if (!first.cut()) {                            // every thread finds the same
-      grid_dep_wait();
-      return;
-    }
-    if (threadIdx.x == 0) {
-      s_walk = first;
-      s_per = per;
-    }
+  if (threadIdx.x < FA_BM) {
+    const int tok = threadIdx.x / p.group;
+    s_row_tok[threadIdx.x] = tok;
+    s_row_off[threadIdx.x] = tok * p.o_ts + (long long)(threadIdx.x - tok * p.group) * p.o_hs;
   }
-
   const uint32_t sQ = base + L::OFF_Q, sK = base + L::OFF_K, sV = base + L::OFF_V;
   const uint32_t bar_q_full = base + L::OFF_BAR;
   const uint32_t bar_q_free = bar_q_full + 2 * 8;
@@ -393,6 +382,24 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     if (lane == 0) mbar_arrive(bar_part_free + (i % PART_RING) * 8);
   };
 
+  // the run of this CTA, found by the loader warp before it gives up its registers
+  long long per = 0;
+  if (warp == 0) {
+    const long long total = whole_line(p, lane);
+    per = max((long long)MIN_RUN, (total + gridDim.x - 1) / gridDim.x);
+    Walk first;
+    first.u = blockIdx.x * per;
+    first.u_end = min(total, first.u + per);
+    if (first.u < first.u_end) {
+      find_place(p, lane, first);
+      if (!first.cut()) first.u = first.u_end;
+    }
+    if (lane == 0) {
+      p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+      s_walk = first;
+    }
+    __syncwarp();
+  }
   if (warp < 4) reg_dealloc<FP4 ? 40 : FA_OTHER_REGS>();
   if (warp == 0) {
     // ------------------------------- parts, K and V -------------------------------
@@ -405,7 +412,7 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       if (i >= PART_RING && !wait_all(bar_part_free + at * 8, (i / PART_RING - 1) & 1, 17)) { ok = false; break; }
       if (lane == 0) {
         if (i > 0) s_walk.next(p);
-        if (s_walk.u < s_walk.u_end) s_part[at] = make_part(p, s_walk, s_per);
+        if (s_walk.u < s_walk.u_end) s_part[at] = make_part(p, s_walk, per);
         else s_part[at].end = 1;
         mbar_arrive(bar_part_full + at * 8);
       }
@@ -594,16 +601,15 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     if (items > 0) mbar_wait(wctx, bar_q_full + t * 8, (items - 1) & 1, 15);   // nothing in flight when this warp leaves
   } else if (warp >= 4 && warp < 12) {
     // -------------------------------- softmax ----------------------------------
-    reg_alloc<FA_SOFTMAX_REGS>();
+    reg_alloc<FP4 ? 208 : 216>();       // 216 x 256 + 56 x 128 = 62464 <= 168 x 384; with NVFP4 208 x 256 + (40 + 56) x 128 = 65536
     const int t = (warp - 4) >> 2;
     const int q = warp & 3;
     const int row = q * 32 + lane;          // row inside the tile == TMEM lane
-    const int tok = row / p.group;
+    const int tok = s_row_tok[row];
     const uint32_t lane_base = tmem_base + ((uint32_t)(q * 32) << 16);
     const uint32_t tS = lane_base + S_COL(t);
     const uint32_t tO = lane_base + O_COL(t);
     uint32_t steps = 0, items = 0;
-    const uint32_t s_out = base + L::OFF_OUT + (warp - 4) * 2048;
     bool ok = true;
     for (int i = 0; ok && have_part(i); ++i) {
       const Part& w = s_part[i % PART_RING];
@@ -616,6 +622,8 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         if (p.causal && p.window > 0) row_lo = max(0, pos - p.window + 1);
       }
       const bool blind = row_hi <= row_lo;
+      float poly_max = 0.0f;
+      uint64_t k2[CAP_POLY_N];             // the polynomial in s itself
       float scale = p.score.scale_log2, cap_arg = p.score.cap_arg;
       float m_run = -CUDART_INF_F, l_run = 0.0f;
       for (int j = 0; j < n_mine; ++j, ++steps) {
@@ -626,17 +634,37 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           scale *= unit;
           cap_arg *= unit;
         }
+        if (CAP && j == 0) {
+          const float a = cap_arg * (0.5f / 1.4426950408889634f), aa = a * a;      // scale / c and its powers, if f32 holds them
+          poly_max = a > 0x1p-14f && a < 0x1p14f ? CAP_POLY_MAX / a : -1.0f;
+          float f = a;
+#pragma unroll
+          for (int i = 0; i < CAP_POLY_N; ++i) {
+            k2[i] = pack2(p.cap_poly[i] * f, p.cap_poly[i] * f);
+            f *= aa;
+          }
+        }
         uint32_t v[FA_BN];
 #pragma unroll
         for (int c = 0; c < FA_BN / 32; ++c)
           tmem_ld_32x32b_x32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&v[c * 32]));
         const int key0 = key_base + j * FA_BN;
         const int c_hi = row_hi - 1 - key0, c_lo = row_lo - key0;    // first and last column seen
-        const bool masked_tile = __any_sync(0xffffffffu, c_hi < FA_BN - 1 || c_lo > 0);
+        // rows that see nothing (no token's, mostly) hold what they like: nothing of it is written
+        const bool masked_tile = __any_sync(0xffffffffu, !blind && (c_hi < FA_BN - 1 || c_lo > 0));
         tmem_wait_ld();
+        bool poly = false;                    // the cap's polynomial serves every score of the warp's rows
+        if (CAP) {
+          float mp[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < FA_BN; i += 8)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              mp[u] = absmax3(mp[u], __uint_as_float(v[i + 2 * u]), __uint_as_float(v[i + 2 * u + 1]));
+          const float big = fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3]));
+          poly = __all_sync(0xffffffffu, blind || big <= poly_max);
+        }
         if (masked_tile) {
-          // a row that sees nothing at all would keep the cap's polynomial from the others: it holds zeros there
-          const uint32_t hidden = CAP && blind ? 0u : 0xff800000u;   // -inf
 #pragma unroll
           for (int c = 0; c < FA_BN / 32; ++c) {
             // bits of the columns [c_lo, c_hi] among these 32
@@ -645,7 +673,7 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             bits &= l <= 0 ? ~0u : l > 31 ? 0u : ~0u << l;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (!((bits >> i) & 1u)) v[c * 32 + i] = hidden;
+              if (!((bits >> i) & 1u)) v[c * 32 + i] = 0xff800000u;  // -inf
           }
         }
         float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
@@ -656,18 +684,8 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             mx[u] = max3(mx[u], __uint_as_float(v[i + 2 * u]), __uint_as_float(v[i + 2 * u + 1]));
         }
         const float rmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        bool poly = false;                    // the cap's polynomial serves every score of the warp's rows
-        if (CAP) {
-          float mn[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int i = 0; i < FA_BN; i += 4)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) mn[u] = fminf(mn[u], __uint_as_float(v[i + u]));
-          const float big = fmaxf(rmax, -fminf(fminf(mn[0], mn[1]), fminf(mn[2], mn[3])));
-          poly = __all_sync(0xffffffffu, big * cap_arg <= 2.0f * 1.4426950408889634f * CAP_POLY_MAX);
-        }
         // the score grows with s: the largest s has the largest score (the cap maps -inf to -cap: kept apart)
-        const float m_tile = rmax == -CUDART_INF_F ? rmax
+        const float m_tile = blind || rmax == -CUDART_INF_F ? -CUDART_INF_F
                              : CAP             ? paged_score<true>(ScoreParams{scale, cap_arg, p.score.cap_out}, rmax)
                                                : rmax * scale;
         const float m_new = fmaxf(m_run, m_tile);
@@ -716,20 +734,25 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           const uint64_t scale2 = pack2(scale, scale);
           probabilities([&](uint64_t s2) { return fma2(s2, scale2, negm2); });
         } else if (poly) {
-          const float a = cap_arg * (0.5f / 1.4426950408889634f);      // scale / c
-          const uint64_t a2 = pack2(a, a), zero2 = 0ull;
-          uint64_t k2[6];
-#pragma unroll
-          for (int i = 0; i < 6; ++i) k2[i] = pack2(p.cap_poly[i], p.cap_poly[i]);
-          probabilities([&](uint64_t s2) {
-            const uint64_t x = fma2(s2, a2, zero2), y = fma2(x, x, zero2);
-            uint64_t h = fma2(k2[5], y, k2[4]);
-            h = fma2(h, y, k2[3]);
-            h = fma2(h, y, k2[2]);
+          auto capped = [&](uint64_t s2) {
+            const uint64_t y = fma2(s2, s2, 0ull);
+            uint64_t h = fma2(k2[3], y, k2[2]);
             h = fma2(h, y, k2[1]);
             h = fma2(h, y, k2[0]);
-            return fma2(x, h, negm2);
-          });
+            return fma2(s2, h, negm2);
+          };
+          if (!masked_tile) {
+            probabilities(capped);
+          } else {
+            probabilities([&](uint64_t s2) {
+              float sa, sd, xa, xd;
+              unpack2(s2, sa, sd);
+              unpack2(capped(s2), xa, xd);
+              if (sa == -CUDART_INF_F) xa = -CUDART_INF_F;             // masked: stays out, cap or not
+              if (sd == -CUDART_INF_F) xd = -CUDART_INF_F;
+              return pack2(xa, xd);
+            });
+          }
         } else {
           const float off = p.score.cap_out + neg_m;
           probabilities([&](uint64_t s2) {
@@ -737,7 +760,7 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             unpack2(s2, sa, sd);
             float xa = fmaf(-2.0f * p.score.cap_out, paged_rcp(1.0f + ex2_approx(sa * cap_arg)), off);
             float xd = fmaf(-2.0f * p.score.cap_out, paged_rcp(1.0f + ex2_approx(sd * cap_arg)), off);
-            if (sa == -CUDART_INF_F) xa = -CUDART_INF_F;               // masked: stays out, cap or not
+            if (sa == -CUDART_INF_F) xa = -CUDART_INF_F;
             if (sd == -CUDART_INF_F) xd = -CUDART_INF_F;
             return pack2(xa, xd);
           });
@@ -766,10 +789,10 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       const float inv_l = !whole ? 1.0f : l_run == 0.0f ? 0.0f : (FP4 ? p.out_scale : 1.0f) / l_run;
       float* part = p.part + ((long long)blockIdx.x * 2 + w.slot) * part_floats(D);
       const int ntok = w.tokens[t];
-      const long long out_row = w.row0 + t * p.tpt;
-      const int out_head = w.head * p.group;
+      uint16_t* out = p.out + (long long)(w.row0 + t * p.tpt) * p.o_ts + (long long)(w.head * p.group) * p.o_hs;
+      uint16_t* dst = out + s_row_off[row];
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = 0; c < D / 32; ++c) {           // 32 columns at a time: more spill the softmax loop's registers
         uint32_t o[32];
         if (n_mine > 0) {
           tmem_ld_32x32b_x32(tO + c * 32, o);
@@ -777,32 +800,28 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         }
         if (n_mine == 0 || l_run == 0.0f) {        // whatever stands there, a row without a key is zero
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0u;
+          for (int k = 0; k < 32; ++k) o[k] = 0u;
         }
         if (whole) {
-          // to 16 bits, through shared memory, so that a store covers 64 neighbouring bytes of 8 rows and not 16 of 32
-          __syncwarp();
+          if (tok < ntok) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t x[4];
+            for (int e = 0; e < 2; ++e) {
+              uint32_t x[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float lo = __uint_as_float(o[e * 8 + 2 * k]) * inv_l;
-              const float hi = __uint_as_float(o[e * 8 + 2 * k + 1]) * inv_l;
-              x[k] = F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+              for (int k = 0; k < 8; ++k) {
+                const float lo = __uint_as_float(o[e * 16 + 2 * k]) * inv_l;
+                const float hi = __uint_as_float(o[e * 16 + 2 * k + 1]) * inv_l;
+                x[k] = F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+              }
+              if (p.wide_out) {                    // a full 32-byte sector per lane
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                             ::"l"(dst + c * 32 + e * 16), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]),
+                               "r"(x[6]), "r"(x[7]) : "memory");
+              } else {
+                *reinterpret_cast<uint4*>(dst + c * 32 + e * 16) = make_uint4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<uint4*>(dst + c * 32 + e * 16 + 8) = make_uint4(x[4], x[5], x[6], x[7]);
+              }
             }
-            st_shared_v4(s_out + lane * 64 + ((e ^ ((lane >> 1) & 3)) << 4), x[0], x[1], x[2], x[3]);
-          }
-          __syncwarp();
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int r = k * 8 + (lane >> 2), e = lane & 3, rt = (q * 32 + r) / p.group;
-            uint32_t x[4];
-            ld_shared_v4(s_out + r * 64 + ((e ^ ((r >> 1) & 3)) << 4), x);
-            if (rt < ntok)
-              *reinterpret_cast<uint4*>(p.out + (out_row + rt) * p.o_ts +
-                                        (long long)(out_head + q * 32 + r - rt * p.group) * p.o_hs + c * 32 + e * 8) =
-                  make_uint4(x[0], x[1], x[2], x[3]);
           }
         } else {
 #pragma unroll
@@ -977,8 +996,9 @@ int launch_tile(const PagedAttnArgs& a, const PagedTilePlan& plan) {
   p.out = static_cast<uint16_t*>(a.out);
   p.o_ts = a.o_ts;
   p.o_hs = a.o_hs;
+  p.wide_out = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.o_ts % 16 == 0 && a.o_hs % 16 == 0;
   p.out_scale = 1.0f;
-  for (int i = 0; i < 6; ++i) p.cap_poly[i] = CAP_POLY[i] * a.score.cap_out;
+  for (int i = 0; i < CAP_POLY_N; ++i) p.cap_poly[i] = CAP_POLY[i] * a.score.cap_out;
   p.part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + a.tile_off);
   p.desc = reinterpret_cast<int4*>(static_cast<char*>(a.workspace) + a.tile_off + plan.desc_off);
   const CUtensorMapDataType dt = F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
