@@ -61,7 +61,7 @@ struct TileParams {
 // [2][128] maxima and [2][128] sums.
 __host__ __device__ constexpr int part_floats(int d) { return 2 * 128 * (d + 2); }
 // Starting and ending an item costs about as much as this many keys.
-constexpr int ITEM_COST = 256;
+constexpr int ITEM_COST = 384;
 constexpr int MIN_RUN = 768;         // keys: a shorter run would be mostly start-up
 constexpr int PART_RING = 4;         // parts known ahead of their turn
 
@@ -601,7 +601,7 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     if (items > 0) mbar_wait(wctx, bar_q_full + t * 8, (items - 1) & 1, 15);   // nothing in flight when this warp leaves
   } else if (warp >= 4 && warp < 12) {
     // -------------------------------- softmax ----------------------------------
-    reg_alloc<FP4 ? 208 : 216>();       // 216 x 256 + 56 x 128 = 62464 <= 168 x 384; with NVFP4 208 x 256 + (40 + 56) x 128 = 65536
+    reg_alloc<FP4 ? 208 : 224>();       // 224 x 256 + 56 x 128 = 168 x 384; with NVFP4 208 x 256 + (40 + 56) x 128 = 128 x 512
     const int t = (warp - 4) >> 2;
     const int q = warp & 3;
     const int row = q * 32 + lane;          // row inside the tile == TMEM lane
@@ -933,34 +933,34 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 }
 
 // Adds the parts of the items that were cut, as the row-block kernel's merge does.  Thread = row; blockIdx.y = tile and
-// a quarter of the dimensions.
+// an eighth of the dimensions.
 template <int D, bool F16>
 __global__ void __launch_bounds__(128) fmha_paged_tile_merge_kernel(const __grid_constant__ TileParams p) {
   grid_dep_wait();
   const int4 d = p.desc[blockIdx.x];
   if (d.x == 0) return;
-  const int t = blockIdx.y & 1, c0 = (blockIdx.y >> 1) * (D / 16);       // float4 columns c0 .. c0 + D / 16
+  const int t = blockIdx.y & 1, c0 = (blockIdx.y >> 1) * (D / 32);       // float4 columns c0 .. c0 + D / 32
   const int row = threadIdx.x, tok = row / p.group;
   const SeqView sv = seq_view(p.batch, d.y);
   const int tok0 = (d.z * 2 + t) * p.tpt;
   if (tok >= min(max(sv.n - tok0, 0), p.tpt)) return;
   float m = -CUDART_INF_F, l = 0.0f;
-  float4 o[D / 16];
+  float4 o[D / 32];
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 2
+  for (int i = 0; i < D / 32; ++i) o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
   for (int i = 0; i < d.x; ++i) {
     const float* part = p.part + ((long long)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * part_floats(D);
     const float pm = part[2 * 128 * D + t * 128 + row], pl = part[2 * 128 * D + 256 + t * 128 + row];
-    float4 v[D / 16];
+    float4 v[D / 32];
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) v[c] = reinterpret_cast<const float4*>(part)[(t * (D / 4) + c0 + c) * 128 + row];
+    for (int c = 0; c < D / 32; ++c) v[c] = reinterpret_cast<const float4*>(part)[(t * (D / 4) + c0 + c) * 128 + row];
     const float mn = fmaxf(m, pm), mu = mn == -CUDART_INF_F ? 0.0f : mn;
     const float wa = ex2_approx(m - mu), wb = ex2_approx(pm - mu);
     m = mn;
     l = l * wa + pl * wb;
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
+    for (int c = 0; c < D / 32; ++c) {
       o[c].x = o[c].x * wa + v[c].x * wb;
       o[c].y = o[c].y * wa + v[c].y * wb;
       o[c].z = o[c].z * wa + v[c].z * wb;
@@ -971,7 +971,7 @@ __global__ void __launch_bounds__(128) fmha_paged_tile_merge_kernel(const __grid
   uint16_t* dst = p.out + (long long)(sv.q0 + tok0 + tok) * p.o_ts +
                   (long long)(d.w * p.group + row - tok * p.group) * p.o_hs + c0 * 4;
 #pragma unroll
-  for (int c = 0; c < D / 16; c += 2)
+  for (int c = 0; c < D / 32; c += 2)
     *reinterpret_cast<uint4*>(dst + c * 4) =
         make_uint4(paged_pack16<F16>(o[c].x * inv, o[c].y * inv), paged_pack16<F16>(o[c].z * inv, o[c].w * inv),
                    paged_pack16<F16>(o[c + 1].x * inv, o[c + 1].y * inv), paged_pack16<F16>(o[c + 1].z * inv, o[c + 1].w * inv));
@@ -1044,7 +1044,7 @@ int launch_tile(const PagedAttnArgs& a, const PagedTilePlan& plan) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tmQ, tmK, tmV, p, di->status));
-  cfg.gridDim = dim3(plan.ctas, 8);
+  cfg.gridDim = dim3(plan.ctas, 16);
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 0;
   B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fmha_paged_tile_merge_kernel<D, F16>, p));
