@@ -102,9 +102,10 @@ struct SplitParams {
   long long part_floats;
   int workers, by_item, rb_max;
   int min_steps;
-  // FP4 operands: byte strides
+  // FP4 operands, strides in bytes: those that are multiplied in every step fit in 32 bits
   const uint8_t *k, *v, *ks, *vs;
-  long long k_st[3], v_st[3], ks_st[3], vs_st[3];
+  long long k_head, v_head, ks_head, vs_head;
+  uint32_t k_page, v_page, ks_page, vs_page, k_slot, v_slot, ks_slot, vs_slot;
 };
 
 // Steps of one item of the sequence, from key step `base`; 0 for a sequence without rows here, and at least 1 for one
@@ -174,8 +175,8 @@ __device__ __forceinline__ RowMask<NT> row_mask(const SplitParams& p, const SeqV
 // plus the 16-bit rest of it (HILO): the rounding of P alone would put an error as large as the output's own rounding
 // beside it, and the second product costs nothing next to the loads.
 template <bool F16, int NT, int DT, bool CAP, bool HILO>
-__device__ __forceinline__ void softmax_step(const SplitParams& p, const RowMask<NT>& rm, int key0, int lane, bool ragged,
-                                             float (&s)[NT][4], float (&m_run)[NT][2], float (&l_run)[NT][2],
+__device__ __forceinline__ void softmax_step(const ScoreParams (&sp)[NT][2], const RowMask<NT>& rm, int key0, int lane,
+                                             bool ragged, float (&s)[NT][4], float (&m_run)[NT][2], float (&l_run)[NT][2],
                                              float (&o)[DT][NT][4], uint32_t (&pb)[NT][2], uint32_t (&pl)[NT][2]) {
   const int g = lane >> 2;
   bool over = false;
@@ -183,7 +184,7 @@ __device__ __forceinline__ void softmax_step(const SplitParams& p, const RowMask
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      float x = paged_score<CAP>(p.score, s[nt][e]);
+      float x = paged_score<CAP>(sp[nt][e & 1], s[nt][e]);
       if (ragged) {
         const int key = key0 + g + (e >> 1) * 8;
         if (key < rm.lo[nt][e & 1] || key >= rm.hi[nt][e & 1]) x = -CUDART_INF_F;
@@ -368,6 +369,18 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
       pages = i + lane < nk ? page_of(p.batch, b, key, status) : 0;
     };
     const int slot_mask = (1 << p.batch.page_shift) - 1;
+    // FP4: where this lane's pieces of a step lie in the pools, for page 0 and slot 0 of this head
+    const uint8_t *k_lane = nullptr, *v_lane = nullptr, *s_lane = nullptr;
+    uint32_t s_page = 0, s_slot = 0;
+    if constexpr (FP4) {
+      constexpr int CH = C4::ROW / 16;
+      k_lane = p.k + (long long)h * p.k_head + (long long)(lane / CH) * p.k_slot + (lane % CH) * 16;
+      v_lane = p.v + (long long)h * p.v_head + (long long)(lane / CH) * p.v_slot + (lane % CH) * 16;
+      const bool is_v = lane >= 16;                   // scales: K's rows in the first half of the lanes, V's in the second
+      s_page = is_v ? p.vs_page : p.ks_page;
+      s_slot = is_v ? p.vs_slot : p.ks_slot;
+      s_lane = (is_v ? p.vs : p.ks) + (long long)h * (is_v ? p.vs_head : p.ks_head) + (long long)(lane & 15) * s_slot;
+    }
     auto issue = [&](int i) {
       if (i >= nk) return;                            // warp-uniform
       if (i - pages_at >= 32) fetch_pages(i);
@@ -386,21 +399,17 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
         }
       } else {
         const bool ok = pg < p.batch.num_pages;
-        const int pgc = ok ? pg : 0;                  // a valid address for the copies that read nothing
-        const uint8_t* kp = p.k + (long long)pgc * p.k_st[0] + (long long)h * p.k_st[1] + (long long)slot * p.k_st[2];
-        const uint8_t* vp = p.v + (long long)pgc * p.v_st[0] + (long long)h * p.v_st[1] + (long long)slot * p.v_st[2];
-        constexpr int CH = C4::ROW / 16;              // 16-byte chunks per row
+        const uint32_t pgc = ok ? pg : 0;             // a valid address for the copies that read nothing
+        const uint8_t* kp = k_lane + (uint64_t)pgc * p.k_page + (uint64_t)(uint32_t)slot * p.k_slot;
+        const uint8_t* vp = v_lane + (uint64_t)pgc * p.v_page + (uint64_t)(uint32_t)slot * p.v_slot;
+        const uint8_t* sp_ = s_lane + (uint64_t)pgc * s_page + (uint64_t)(uint32_t)slot * s_slot;
+        constexpr int CH = C4::ROW / 16, ROWS = 32 / CH;   // 16-byte chunks per row; rows a pass of the warp covers
 #pragma unroll
-        for (int c = 0; c < STEP * CH / 32; ++c) {
-          const int x = c * 32 + lane, r = x / CH, o = (x % CH) * 16;
-          cp_async_16(dst + r * C4::ROW + o, kp + r * p.k_st[2] + o, ok);
-          cp_async_16(dst + STEP * C4::ROW + r * C4::ROW + o, vp + r * p.v_st[2] + o, ok);
+        for (int c = 0; c < STEP / ROWS; ++c) {
+          cp_async_16(dst + c * 512 + lane * 16, kp + (uint64_t)(c * ROWS) * p.k_slot, ok);
+          cp_async_16(dst + STEP * C4::ROW + c * 512 + lane * 16, vp + (uint64_t)(c * ROWS) * p.v_slot, ok);
         }
-        const int r = lane & 15;
-        const bool is_v = lane >= 16;
-        const uint8_t* sp = is_v ? p.vs + (long long)pgc * p.vs_st[0] + (long long)h * p.vs_st[1] + (slot + r) * p.vs_st[2]
-                                 : p.ks + (long long)pgc * p.ks_st[0] + (long long)h * p.ks_st[1] + (slot + r) * p.ks_st[2];
-        cp_async_small<C4::SROW>(dst + 2 * STEP * C4::ROW + (is_v ? STEP * C4::SROW : 0) + r * C4::SROW, sp, ok);
+        cp_async_small<C4::SROW>(dst + 2 * STEP * C4::ROW + lane * C4::SROW, sp_, ok);
       }
     };
     if (nk > 0) {
@@ -415,9 +424,10 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
     // Q^T as the B operand: query row 8 nt + g, two adjacent dimensions per register (FP4: the pairs that the K words
     // unpack to, see below; the row is brought to a power of two near 1 first, so that f16 holds it whatever its size)
     uint32_t qb[NT][DT][2];
-    float q_unit[NT][2];                              // what the rows 2t, 2t + 1 were divided by
+    ScoreParams sp[NT][2];                            // of the rows 2t, 2t + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      sp[nt][0] = sp[nt][1] = p.score;
       const int row = rb * RB + nt * 8 + g;
       const int tok = row / p.group;
       const bool ok = tok < sv.n;
@@ -454,8 +464,12 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
           for (int x = 0; x < 4; ++x)                 // byte x of the word
             qb[nt][2 * w + (x >> 1)][x & 1] = pack_f16x2(f[w * 8 + 2 * x] * inv, f[w * 8 + 2 * x + 1] * inv);
         // rows 2t and 2t + 1 sit in the lanes with g = 2t, 2t + 1
-        q_unit[nt][0] = __shfl_sync(0xffffffffu, unit, 8 * t);
-        q_unit[nt][1] = __shfl_sync(0xffffffffu, unit, 8 * t + 4);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float f = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * j);
+          sp[nt][j].scale_log2 *= f;
+          sp[nt][j].cap_arg *= f;
+        }
       }
     }
 
@@ -500,7 +514,7 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(s[nt], a, qb[nt][ks][0], qb[nt][ks][1]);
         }
-        softmax_step<F16, NT, DT, CAP, HILO>(p, rm, key0, lane, ragged, s, m_run, l_run, o, pb, pl);
+        softmax_step<F16, NT, DT, CAP, HILO>(sp, rm, key0, lane, ragged, s, m_run, l_run, o, pb, pl);
 #pragma unroll
         for (int c = 0; c < DT; ++c) {
           uint32_t a[4];
@@ -567,11 +581,7 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
             mma_16816<true>(s[nt], a1, qb[nt][2 * w + 1][0], qb[nt][2 * w + 1][1]);
           }
         }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[nt][e] *= q_unit[nt][e & 1];
-        softmax_step<true, NT, DT, CAP, HILO>(p, rm, key0, lane, ragged, s, m_run, l_run, o, pb, pl);
+        softmax_step<true, NT, DT, CAP, HILO>(sp, rm, key0, lane, ragged, s, m_run, l_run, o, pb, pl);
         // V: dimensions [D/8 g, D/8 (g + 1)) of keys 2t, 2t + 1, 2t + 8, 2t + 9.  The operand wants two keys side by side
         // in a register, so the codes of two keys are put into one byte first: lo holds the even dimensions, hi the odd
         // ones.  Row m of tile c <-> dimension D/8 m + 2c, row m + 8 <-> the next one.
@@ -717,13 +727,15 @@ __global__ void __launch_bounds__(256) fmha_paged_merge_kernel(const __grid_cons
   __shared__ float4 s_o[8][NT][32];
   __shared__ float s_ml[8][NT][2][4][2];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the tile kernel of the same call, if there is one
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  bool exists = true;
   if (p.by_item) {
-    // items that do not exist in this launch have no descriptor
+    // items that do not exist in this launch have no descriptor (lengths are the call's inputs: known before the wait)
     const int b = blockIdx.x / (p.rb_max * p.kv_heads), rb = (blockIdx.x / p.kv_heads) % p.rb_max;
-    if (rb >= seq_work<RB>(p, b).rbs) return;
+    exists = rb < seq_work<RB>(p, b).rbs;
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!exists) return;
   const int4 d = p.desc[blockIdx.x];
   if (d.x == 0) return;
   const int pw = warp % PW, c = blockIdx.y * CT + warp / PW;
@@ -749,18 +761,30 @@ __global__ void __launch_bounds__(256) fmha_paged_merge_kernel(const __grid_cons
     }
   };
   if (c < DT) {
-#pragma unroll 4
-    for (int i = pw; i < d.x; i += PW) {
-      const float* src = p.part + ((long long)(d.y + i) * 2 + (i == 0 ? 1 : 0)) * p.part_floats;
-      const float* ml = src + DT * NT * 128;
+    constexpr int U = NT == 1 ? 8 : 4;               // parts whose loads are in flight together
+    for (int i0 = pw; i0 < d.x; i0 += U * PW) {
+      float4 v[U][NT];
+      float2 pm[U][NT], pl[U][NT];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float4 v = reinterpret_cast<const float4*>(src)[(c * NT + nt) * 32 + lane];
-        const float2 pm = *reinterpret_cast<const float2*>(ml + nt * 8 + 2 * t);
-        const float2 pl = *reinterpret_cast<const float2*>(ml + RB + nt * 8 + 2 * t);
-        const float a[2] = {pm.x, pm.y}, q[2] = {pl.x, pl.y};
-        add(nt, a, q, v);
+      for (int x = 0; x < U; ++x) {
+        const int i = i0 + x * PW;
+        const float* src = p.part + ((long long)(d.y + i) * 2 + (i == 0 ? 1 : 0)) * p.part_floats;
+        const float* ml = src + DT * NT * 128;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const bool there = i < d.x;
+          v[x][nt] = there ? reinterpret_cast<const float4*>(src)[(c * NT + nt) * 32 + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          pm[x][nt] = there ? *reinterpret_cast<const float2*>(ml + nt * 8 + 2 * t) : make_float2(-CUDART_INF_F, -CUDART_INF_F);
+          pl[x][nt] = there ? *reinterpret_cast<const float2*>(ml + RB + nt * 8 + 2 * t) : make_float2(0.0f, 0.0f);
+        }
       }
+#pragma unroll
+      for (int x = 0; x < U; ++x)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float a[2] = {pm[x][nt].x, pm[x][nt].y}, q[2] = {pl[x][nt].x, pl[x][nt].y};
+          add(nt, a, q, v[x][nt]);
+        }
     }
   }
   if (PW > 1) {
@@ -842,10 +866,10 @@ int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
     p.v = static_cast<const uint8_t*>(c.v);
     p.ks = static_cast<const uint8_t*>(c.k_scales);
     p.vs = static_cast<const uint8_t*>(c.v_scales);
-    for (int i = 0; i < 3; ++i) {
-      p.k_st[i] = c.k_strides[i]; p.v_st[i] = c.v_strides[i];
-      p.ks_st[i] = c.k_scale_strides[i]; p.vs_st[i] = c.v_scale_strides[i];
-    }
+    p.k_page = (uint32_t)c.k_strides[0]; p.k_head = c.k_strides[1]; p.k_slot = (uint32_t)c.k_strides[2];
+    p.v_page = (uint32_t)c.v_strides[0]; p.v_head = c.v_strides[1]; p.v_slot = (uint32_t)c.v_strides[2];
+    p.ks_page = (uint32_t)c.k_scale_strides[0]; p.ks_head = c.k_scale_strides[1]; p.ks_slot = (uint32_t)c.k_scale_strides[2];
+    p.vs_page = (uint32_t)c.v_scale_strides[0]; p.vs_head = c.v_scale_strides[1]; p.vs_slot = (uint32_t)c.v_scale_strides[2];
   } else {
     const CUtensorMapDataType dt = F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     if (int rc = b200h::encode_tmap_pages(&tmK, dt, c.k, D, c.page_size, c.kv_heads, c.num_pages, c.k_strides, 64, STEP))

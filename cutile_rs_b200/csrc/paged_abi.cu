@@ -32,13 +32,15 @@ int check_dtype(const char* dtype, const char* who, int* dt) {
 
 // extents of 1 put no condition on their stride
 int check_pool(const char* who, const char* name, const void* p, const int64_t* st, const int extents[3], int unit,
-               uintptr_t align) {
+               uintptr_t align, bool bytes) {
   if (!p) return set_error(B200TILE_ERR_INVALID, "%s: the %s pool is null", who, name);
   bool bad = misaligned(p, align);
   for (int i = 0; i < 3; ++i) {
     if (extents[i] > 1 && st[i] <= 0)
       return set_error(B200TILE_ERR_INVALID, "%s: strides of the %s pool must be positive", who, name);
     bad |= extents[i] > 1 && st[i] % unit != 0;
+    if (bytes && i != 1 && extents[i] > 1 && st[i] > 0x7fffffff)
+      return set_error(B200TILE_ERR_UNSUPPORTED, "%s: page and slot strides of the %s pool must be below 2^31 bytes", who, name);
   }
   if (bad)
     return set_error(B200TILE_ERR_ALIGN, "%s: the %s pool must be %d-byte aligned with strides that are multiples of %d",
@@ -58,12 +60,12 @@ int check_cache(const char* who, const b200tile_paged_cache* c) {
     return set_error(B200TILE_ERR_UNSUPPORTED, "%s: page_size %d is not a power of two of at least 16", who, c->page_size);
   const int ext[3] = {c->num_pages, c->kv_heads, c->page_size};
   const int unit = c->format ? 16 : 8;
-  if (int rc = check_pool(who, "K", c->k, c->k_strides, ext, unit, 16)) return rc;
-  if (int rc = check_pool(who, "V", c->v, c->v_strides, ext, unit, 16)) return rc;
+  if (int rc = check_pool(who, "K", c->k, c->k_strides, ext, unit, 16, c->format == 1)) return rc;
+  if (int rc = check_pool(who, "V", c->v, c->v_strides, ext, unit, 16, c->format == 1)) return rc;
   if (c->format) {
     const int row = c->head_dim / 16;
-    if (int rc = check_pool(who, "K scale", c->k_scales, c->k_scale_strides, ext, row, row)) return rc;
-    if (int rc = check_pool(who, "V scale", c->v_scales, c->v_scale_strides, ext, row, row)) return rc;
+    if (int rc = check_pool(who, "K scale", c->k_scales, c->k_scale_strides, ext, row, row, true)) return rc;
+    if (int rc = check_pool(who, "V scale", c->v_scales, c->v_scale_strides, ext, row, row, true)) return rc;
     if (!(c->k_global > 0.0f && c->v_global > 0.0f) || !isfinite(c->k_global) || !isfinite(c->v_global))
       return set_error(B200TILE_ERR_INVALID, "%s: k_global and v_global must be positive and finite", who);
   }

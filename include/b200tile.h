@@ -356,7 +356,8 @@ B200TILE_API int b200tile_splitk_reduce_merge(const char* dtype, const void* att
  *   format 0   elements of the call's dtype; strides in elements, multiples of 8
  *   format 1   NVFP4: two e2m1 codes per byte (low nibble first) and one f8e4m3fn scale per 16 values, the
  *              operand format of b200tile_linear_nvfp4; value = code * scale * k_global (v_global).
- *              Strides in BYTES: of k / v multiples of 16, of the scale pools multiples of head_dim / 16
+ *              Strides in BYTES: of k / v multiples of 16, of the scale pools multiples of head_dim / 16;
+ *              page and slot strides below 2^31
  *   head_dim   64 or 128, contiguous; page_size a power of two >= 16
  * Pools are 16-byte aligned, the scale pools head_dim / 16 bytes.  The struct is read during the call only. */
 typedef struct b200tile_paged_cache {

@@ -51,6 +51,7 @@ CACHE_FAULTS = [
     (dict(format=1, k_global=0.0), _lib.ERR_INVALID, "k_global"),
     (dict(format=1, v_global=float("nan")), _lib.ERR_INVALID, "v_global"),
     (dict(format=1, k_strides=I3(8192, 2048, 72)), _lib.ERR_ALIGN, "K pool"),
+    (dict(format=1, v_strides=I3(1 << 31, 2048, 128)), _lib.ERR_UNSUPPORTED, "2^31"),
 ]
 
 
