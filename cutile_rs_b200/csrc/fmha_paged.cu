@@ -85,8 +85,8 @@ __device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&r)[4]) {
 
 constexpr int STEP = 16;             // keys per step
 // Warps per CTA, one CTA per SM.  16-bit, D = 128: 8 rings of 3 x 8 KB fill the shared memory; D = 64 halves the step and
-// doubles the warps.  NVFP4: what the registers allow.
-constexpr int split_warps(bool fp4, int d) { return fp4 ? 12 : d == 64 ? 16 : 8; }
+// takes half again as many warps.  NVFP4: what the registers allow.
+constexpr int split_warps(bool fp4, int d) { return fp4 ? 12 : d == 64 ? 12 : 8; }
 constexpr float LAZY = 8.0f;         // the running reference of the exponents may lag behind the maximum by this
 
 struct SplitParams {
@@ -174,30 +174,35 @@ __device__ __forceinline__ RowMask<NT> row_mask(const SplitParams& p, const SeqV
 // a maximum over eight lanes.  P <= 256 then, and l >= 1 for any row that saw a key.  P is handed over as a 16-bit value
 // plus the 16-bit rest of it (HILO): the rounding of P alone would put an error as large as the output's own rounding
 // beside it, and the second product costs nothing next to the loads.
-template <bool F16, int NT, int DT, bool CAP, bool HILO>
+template <bool F16, int KS, int NT, int DT, bool CAP, bool HILO>
 __device__ __forceinline__ void softmax_step(const ScoreParams (&sp)[NT][2], const RowMask<NT>& rm, int key0, int lane,
-                                             bool ragged, float (&s)[NT][4], float (&m_run)[NT][2], float (&l_run)[NT][2],
-                                             float (&o)[DT][NT][4], uint32_t (&pb)[NT][2], uint32_t (&pl)[NT][2]) {
+                                             bool ragged, float (&s)[KS][NT][4], float (&m_run)[NT][2],
+                                             float (&l_run)[NT][2], float (&o)[DT][NT][4], uint32_t (&pb)[KS][NT][2],
+                                             uint32_t (&pl)[KS][NT][2]) {
   const int g = lane >> 2;
   bool over = false;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float x = paged_score<CAP>(sp[nt][e & 1], s[nt][e]);
-      if (ragged) {
-        const int key = key0 + g + (e >> 1) * 8;
-        if (key < rm.lo[nt][e & 1] || key >= rm.hi[nt][e & 1]) x = -CUDART_INF_F;
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = paged_score<CAP>(sp[nt][e & 1], s[ks][nt][e]);
+        if (ragged) {
+          const int key = key0 + ks * STEP + g + (e >> 1) * 8;
+          if (key < rm.lo[nt][e & 1] || key >= rm.hi[nt][e & 1]) x = -CUDART_INF_F;
+        }
+        s[ks][nt][e] = x;
+        over |= x > m_run[nt][e & 1] + LAZY;
       }
-      s[nt][e] = x;
-      over |= x > m_run[nt][e & 1] + LAZY;
-    }
   if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float mx = fmaxf(s[nt][j], s[nt][2 + j]);
+        float mx = fmaxf(s[0][nt][j], s[0][nt][2 + j]);
+#pragma unroll
+        for (int ks = 1; ks < KS; ++ks) mx = fmaxf(mx, fmaxf(s[ks][nt][j], s[ks][nt][2 + j]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -214,20 +219,25 @@ __device__ __forceinline__ void softmax_step(const ScoreParams (&sp)[NT][2], con
   }
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+    float m_use[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float m_use = m_run[nt][j] == -CUDART_INF_F ? 0.0f : m_run[nt][j];   // nothing seen yet
-      s[nt][j] = paged_ex2(s[nt][j] - m_use);
-      s[nt][2 + j] = paged_ex2(s[nt][2 + j] - m_use);
-      l_run[nt][j] += s[nt][j] + s[nt][2 + j];
-    }
+    for (int j = 0; j < 2; ++j) m_use[j] = m_run[nt][j] == -CUDART_INF_F ? 0.0f : m_run[nt][j];   // nothing seen yet
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t hi = paged_pack16<F16>(s[nt][2 * h], s[nt][2 * h + 1]);
-      pb[nt][h] = mat_trans(hi);
-      if (HILO) {
-        const float2 f = paged_unpack16<F16>(hi);
-        pl[nt][h] = mat_trans(paged_pack16<F16>(s[nt][2 * h] - f.x, s[nt][2 * h + 1] - f.y));
+    for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        s[ks][nt][j] = paged_ex2(s[ks][nt][j] - m_use[j]);
+        s[ks][nt][2 + j] = paged_ex2(s[ks][nt][2 + j] - m_use[j]);
+        l_run[nt][j] += s[ks][nt][j] + s[ks][nt][2 + j];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t hi = paged_pack16<F16>(s[ks][nt][2 * h], s[ks][nt][2 * h + 1]);
+        pb[ks][nt][h] = mat_trans(hi);
+        if (HILO) {
+          const float2 f = paged_unpack16<F16>(hi);
+          pl[ks][nt][h] = mat_trans(paged_pack16<F16>(s[ks][nt][2 * h] - f.x, s[ks][nt][2 * h + 1] - f.y));
+        }
       }
     }
   }
@@ -236,7 +246,8 @@ __device__ __forceinline__ void softmax_step(const ScoreParams (&sp)[NT][2], con
 // One 16-bit K/V step: TMA boxes of 16 keys x 64 elements with the 128-byte swizzle, in a ring of the warp's own.
 template <int D>
 struct Core16 {
-  static constexpr int WARPS = split_warps(false, D), STAGES = 3;
+  static constexpr int WARPS = split_warps(false, D), STAGES = D == 64 ? 4 : 3;
+  static constexpr int KS = D == 64 ? 2 : 1;           // steps per iteration
   static constexpr int HALVES = D / 64, BOX = STEP * 128, TILE = HALVES * BOX, STAGE = 2 * TILE;
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int SMEM = 1024 + RING + WARPS * STAGES * 8 + 16;
@@ -244,7 +255,8 @@ struct Core16 {
 // One FP4 step: 16 keys of packed values and scales copied with cp.async into a ring of the warp's own.
 template <int D>
 struct Core4 {
-  static constexpr int WARPS = split_warps(true, D), STAGES = 4;
+  static constexpr int WARPS = split_warps(true, D), STAGES = 6;
+  static constexpr int KS = 2;
   static constexpr int ROW = D / 2, SROW = D / 16;
   static constexpr int STAGE = 2 * STEP * (ROW + SROW);
   static constexpr int RING = WARPS * STAGES * STAGE;
@@ -288,6 +300,8 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
   using C4 = Core4<D>;
   constexpr int WARPS = FP4 ? C4::WARPS : C16::WARPS, THREADS = WARPS * 32;
   constexpr int STAGES = FP4 ? C4::STAGES : C16::STAGES;
+  constexpr int KS = FP4 ? C4::KS : C16::KS;
+  static_assert(!FP4 || STAGES % KS == 0, "a group of copies is KS steps");
   constexpr int DT = D / 16, RB = 8 * NT;
   constexpr bool HILO = !FP4 || F16;         // bf16 output over f16 probabilities needs no second product
   extern __shared__ uint8_t smem_raw[];
@@ -355,11 +369,21 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
     const int rb = item / p.kv_heads, h = item - rb * p.kv_heads;
     const SeqView& sv = sw.s;
     const int rows = min(RB, sv.n * p.group - rb * RB);
-    const RowMask<NT> rm = row_mask<NT>(p, sv, rb, lane);
+    RowMask<NT> rm = row_mask<NT>(p, sv, rb, lane);
     // the part's key steps, cut to what the block's rows can see
     const int k0 = max(sw.base + st0, rm.lo_min / STEP);
     const int k1 = rm.hi_max > rm.lo_min ? min(sw.base + st1, (rm.hi_max + STEP - 1) / STEP) : 0;
     const int nk = k1 - k0;
+    // with two steps per iteration an odd number leaves the last one without a partner: what stands in its place is
+    // another worker's or nobody's, and lies behind every row's range
+    if (KS > 1 && nk > 0) {
+      rm.hi_max = min(rm.hi_max, k1 * STEP);
+      rm.hi_min = min(rm.hi_min, k1 * STEP);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) rm.hi[nt][j] = min(rm.hi[nt][j], k1 * STEP);
+    }
 
     // page numbers of 32 steps at a time, one per lane
     int pages = 0, pages_at = 0;
@@ -415,9 +439,9 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
     if (nk > 0) {
       fetch_pages(0);
 #pragma unroll
-      for (int s = 0; s < STAGES - (FP4 ? 1 : 0); ++s) {
+      for (int s = 0; s < STAGES - (FP4 ? KS : 0); ++s) {
         issue(s);
-        if (FP4) asm volatile("cp.async.commit_group;" ::: "memory");
+        if (FP4 && s % KS == KS - 1) asm volatile("cp.async.commit_group;" ::: "memory");
       }
     }
 
@@ -482,155 +506,177 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
       for (int i = 0; i < DT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
     }
 
-    for (int i = 0; i < nk; ++i) {
+    for (int i = 0; i < nk; i += KS) {
       const int key0 = (k0 + i) * STEP;
-      const bool ragged = key0 < rm.lo_max || key0 + STEP > rm.hi_min;
-      const uint32_t slot_at = (ring_at + i) % STAGES;
-      float s[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+      const bool ragged = key0 < rm.lo_max || key0 + KS * STEP > rm.hi_min;
+      const bool clear = key0 < rm.lo_min || key0 + KS * STEP > rm.hi_max;
       // keys of this lane's V operand that no row of the block sees hold anything at all: cleared bit by bit
-      uint32_t vm0 = 0xffffffffu, vm1 = 0xffffffffu;
-      const bool clear = key0 < rm.lo_min || key0 + STEP > rm.hi_max;
-      if (clear) {
+      auto v_mask = [&](int ks, uint32_t& vm0, uint32_t& vm1) {
         auto seen = [&](int key) { return key >= rm.lo_min && key < rm.hi_max; };
-        const int ka = key0 + 2 * t;
+        const int ka = key0 + ks * STEP + 2 * t;
         vm0 = (seen(ka) ? 0xffffu : 0u) | (seen(ka + 1) ? 0xffff0000u : 0u);
         vm1 = (seen(ka + 8) ? 0xffffu : 0u) | (seen(ka + 9) ? 0xffff0000u : 0u);
-      }
-      uint32_t pb[NT][2], pl[NT][2];
+      };
+      float s[KS][NT][4];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[ks][nt][0] = s[ks][nt][1] = s[ks][nt][2] = s[ks][nt][3] = 0.0f;
+      uint32_t pb[KS][NT][2], pl[KS][NT][2];
       if constexpr (!FP4) {
-        if (!__all_sync(0xffffffffu, mbar_wait(wctx, bars + slot_at * 8, ((ring_at + i) / STAGES) & 1u, 90u + slot_at))) {
-          // gave up: the copies still in flight get their (bounded) time before the shared memory goes
-          for (int x = 1; x < STAGES && i + x < nk; ++x)
-            mbar_wait(wctx, bars + ((ring_at + i + x) % STAGES) * 8, ((ring_at + i + x) / STAGES) & 1u, 99u);
-          return;
-        }
-        const uint32_t sK = ring + slot_at * C16::STAGE, sV = sK + C16::TILE;
+        uint32_t at[KS];
 #pragma unroll
-        for (int ks = 0; ks < DT; ++ks) {
-          uint32_t a[4];
-          ldm_x4(sK + (ks >> 2) * C16::BOX + rowk * 128 + ((((ks & 3) * 2 + ck) ^ (lane & 7)) << 4), a);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(s[nt], a, qb[nt][ks][0], qb[nt][ks][1]);
-        }
-        softmax_step<F16, NT, DT, CAP, HILO>(sp, rm, key0, lane, ragged, s, m_run, l_run, o, pb, pl);
-#pragma unroll
-        for (int c = 0; c < DT; ++c) {
-          uint32_t a[4];
-          ldm_x4_trans(sV + (c >> 2) * C16::BOX + rowv * 128 + ((((c & 3) * 2 + cv) ^ (lane & 7)) << 4), a);
-          if (clear) {
-            a[0] &= vm0;
-            a[1] &= vm0;
-            a[2] &= vm1;
-            a[3] &= vm1;
+        for (int ks = 0; ks < KS; ++ks) {
+          const uint32_t slot_at = (ring_at + i + ks) % STAGES;
+          at[ks] = ring + slot_at * C16::STAGE;
+          if (i + ks < nk &&
+              !__all_sync(0xffffffffu, mbar_wait(wctx, bars + slot_at * 8, ((ring_at + i + ks) / STAGES) & 1u, 90u + slot_at))) {
+            // gave up: the copies still in flight get their (bounded) time before the shared memory goes
+            for (int x = ks + 1; x < STAGES && i + x < nk; ++x)
+              mbar_wait(wctx, bars + ((ring_at + i + x) % STAGES) * 8, ((ring_at + i + x) / STAGES) & 1u, 99u);
+            return;
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_16816<F16>(o[c][nt], a, pb[nt][0], pb[nt][1]);
-            mma_16816<F16>(o[c][nt], a, pl[nt][0], pl[nt][1]);
+          for (int c = 0; c < DT; ++c) {
+            uint32_t a[4];
+            ldm_x4(at[ks] + (c >> 2) * C16::BOX + rowk * 128 + ((((c & 3) * 2 + ck) ^ (lane & 7)) << 4), a);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_16816<F16>(s[ks][nt], a, qb[nt][c][0], qb[nt][c][1]);
           }
         }
-        __syncwarp();                                 // every lane is done with the slot before it is filled again
-        issue(i + STAGES);
+        softmax_step<F16, KS, NT, DT, CAP, HILO>(sp, rm, key0, lane, ragged, s, m_run, l_run, o, pb, pl);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t vm0 = ~0u, vm1 = ~0u;
+          if (clear) v_mask(ks, vm0, vm1);
+#pragma unroll
+          for (int c = 0; c < DT; ++c) {
+            uint32_t a[4];
+            ldm_x4_trans(at[ks] + C16::TILE + (c >> 2) * C16::BOX + rowv * 128 + ((((c & 3) * 2 + cv) ^ (lane & 7)) << 4), a);
+            if (clear) {
+              a[0] &= vm0;
+              a[1] &= vm0;
+              a[2] &= vm1;
+              a[3] &= vm1;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_16816<F16>(o[c][nt], a, pb[ks][nt][0], pb[ks][nt][1]);
+              mma_16816<F16>(o[c][nt], a, pl[ks][nt][0], pl[ks][nt][1]);
+            }
+          }
+        }
+        __syncwarp();                                 // every lane is done with the slots before they are filled again
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) issue(i + STAGES + ks);
       } else {
-        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        // one group per iteration: KS steps
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES / KS - 2) : "memory");
         __syncwarp();
-        issue(i + STAGES - 1);                        // into the slot that the last step was done with
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) issue(i + STAGES - KS + ks);   // into the slots that the last iteration was done with
         asm volatile("cp.async.commit_group;" ::: "memory");
-        const uint32_t sK = ring + slot_at * C4::STAGE, sV = sK + STEP * C4::ROW;
-        const uint32_t sKs = sV + STEP * C4::ROW, sVs = sKs + STEP * C4::SROW;
-        // K: keys g and g + 8, D/4 dimensions of each (D/8 bytes), one scale per two words
-        constexpr int WORDS = D / 32;
-        uint32_t wk[2][WORDS];
-        uint32_t sc[2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const uint32_t at = sK + (g + 8 * x) * C4::ROW + t * (D / 8);
-          if constexpr (WORDS == 4)
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(wk[x][0]), "=r"(wk[x][1]), "=r"(wk[x][2]), "=r"(wk[x][3]) : "r"(at));
-          else
-            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(wk[x][0]), "=r"(wk[x][1]) : "r"(at));
-          uint32_t two;                               // scales of this lane's dimensions
-          if constexpr (WORDS == 4) {
-            asm volatile("{.reg .b16 h; ld.shared.b16 h, [%1]; cvt.u32.u16 %0, h;}"
-                         : "=r"(two) : "r"(sKs + (g + 8 * x) * C4::SROW + t * 2));
-          } else {
-            asm volatile("{.reg .b16 h; ld.shared.u8 h, [%1]; cvt.u32.u16 %0, h;}"
-                         : "=r"(two) : "r"(sKs + (g + 8 * x) * C4::SROW + t));
+        for (int ks = 0; ks < KS; ++ks) {
+          const uint32_t sK = ring + ((ring_at + i + ks) % STAGES) * C4::STAGE;
+          const uint32_t sKs = sK + 2 * STEP * C4::ROW;
+          // K: keys g and g + 8, D/4 dimensions of each (D/8 bytes), one scale per two words
+          constexpr int WORDS = D / 32;
+          uint32_t wk[2][WORDS];
+          uint32_t sc[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t at = sK + (g + 8 * x) * C4::ROW + t * (D / 8);
+            uint32_t two;                               // scales of this lane's dimensions
+            if constexpr (WORDS == 4) {
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(wk[x][0]), "=r"(wk[x][1]), "=r"(wk[x][2]), "=r"(wk[x][3]) : "r"(at));
+              asm volatile("{.reg .b16 h; ld.shared.b16 h, [%1]; cvt.u32.u16 %0, h;}"
+                           : "=r"(two) : "r"(sKs + (g + 8 * x) * C4::SROW + t * 2));
+            } else {
+              asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(wk[x][0]), "=r"(wk[x][1]) : "r"(at));
+              asm volatile("{.reg .b16 h; ld.shared.u8 h, [%1]; cvt.u32.u16 %0, h;}"
+                           : "=r"(two) : "r"(sKs + (g + 8 * x) * C4::SROW + t));
+            }
+            sc[x] = e4m3x2_to_f16x2(two);
           }
-          sc[x] = e4m3x2_to_f16x2(two);
+#pragma unroll
+          for (int w = 0; w < WORDS; ++w) {
+            uint32_t f0[4], f1[4];
+            const uint32_t s0 = __byte_perm(sc[0], sc[0], w >= 2 ? 0x3232 : 0x1010);
+            const uint32_t s1 = __byte_perm(sc[1], sc[1], w >= 2 ? 0x3232 : 0x1010);
+            e2m1x8_to_f16(wk[0][w], f0);
+            e2m1x8_to_f16(wk[1][w], f1);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {               // exact: two significant bits times four
+              f0[x] = hmul2(f0[x], s0);
+              f1[x] = hmul2(f1[x], s1);
+            }
+            const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_16816<true>(s[ks][nt], a0, qb[nt][2 * w][0], qb[nt][2 * w][1]);
+              mma_16816<true>(s[ks][nt], a1, qb[nt][2 * w + 1][0], qb[nt][2 * w + 1][1]);
+            }
+          }
         }
-#pragma unroll
-        for (int w = 0; w < WORDS; ++w) {
-          uint32_t f0[4], f1[4];
-          const uint32_t s0 = __byte_perm(sc[0], sc[0], w >= 2 ? 0x3232 : 0x1010);
-          const uint32_t s1 = __byte_perm(sc[1], sc[1], w >= 2 ? 0x3232 : 0x1010);
-          e2m1x8_to_f16(wk[0][w], f0);
-          e2m1x8_to_f16(wk[1][w], f1);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {               // exact: two significant bits times four
-            f0[x] = hmul2(f0[x], s0);
-            f1[x] = hmul2(f1[x], s1);
-          }
-          const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_16816<true>(s[nt], a0, qb[nt][2 * w][0], qb[nt][2 * w][1]);
-            mma_16816<true>(s[nt], a1, qb[nt][2 * w + 1][0], qb[nt][2 * w + 1][1]);
-          }
-        }
-        softmax_step<true, NT, DT, CAP, HILO>(sp, rm, key0, lane, ragged, s, m_run, l_run, o, pb, pl);
+        softmax_step<true, KS, NT, DT, CAP, HILO>(sp, rm, key0, lane, ragged, s, m_run, l_run, o, pb, pl);
         // V: dimensions [D/8 g, D/8 (g + 1)) of keys 2t, 2t + 1, 2t + 8, 2t + 9.  The operand wants two keys side by side
         // in a register, so the codes of two keys are put into one byte first: lo holds the even dimensions, hi the odd
         // ones.  Row m of tile c <-> dimension D/8 m + 2c, row m + 8 <-> the next one.
-        constexpr int VW = D / 64;                    // words per key
-        uint32_t wv[4][VW], sb[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int key = 2 * t + (x & 1) + (x >> 1) * 8;
-          const uint32_t at = sV + key * C4::ROW + g * (D / 16);
-          if constexpr (VW == 2)
-            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(wv[x][0]), "=r"(wv[x][1]) : "r"(at));
-          else
-            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wv[x][0]) : "r"(at));
-          const uint32_t sat = sVs + key * C4::SROW + g * (D / 8) / 16;
-          asm volatile("{.reg .b16 h; ld.shared.u8 h, [%1]; cvt.u32.u16 %0, h;}" : "=r"(sb[x]) : "r"(sat));
-        }
-        // a masked key's scale may be a NaN pattern: the mask clears the product, not the factor
-        const uint32_t sv0 = e4m3x2_to_f16x2(sb[0] | (sb[1] << 8)), sv1 = e4m3x2_to_f16x2(sb[2] | (sb[3] << 8));
+        for (int ks = 0; ks < KS; ++ks) {
+          const uint32_t sV = ring + ((ring_at + i + ks) % STAGES) * C4::STAGE + STEP * C4::ROW;
+          const uint32_t sVs = sV + STEP * C4::ROW + STEP * C4::SROW;
+          uint32_t vm0 = ~0u, vm1 = ~0u;
+          if (clear) v_mask(ks, vm0, vm1);
+          constexpr int VW = D / 64;                    // words per key
+          uint32_t wv[4][VW], sb[4];
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          constexpr uint32_t M = 0x0F0F0F0Fu;
-          uint32_t f[4][4];                           // lo and hi of keys 2t, 2t + 1; of keys 2t + 8, 2t + 9
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint32_t ka = wv[2 * x][w], kb = wv[2 * x + 1][w], sc2 = x ? sv1 : sv0;
-            e2m1x8_to_f16((ka & M) | ((kb << 4) & ~M), f[2 * x]);
-            e2m1x8_to_f16(((ka >> 4) & M) | (kb & ~M), f[2 * x + 1]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              f[2 * x][i] = hmul2(f[2 * x][i], sc2);
-              f[2 * x + 1][i] = hmul2(f[2 * x + 1][i], sc2);
-            }
+          for (int x = 0; x < 4; ++x) {
+            const int key = 2 * t + (x & 1) + (x >> 1) * 8;
+            const uint32_t at = sV + key * C4::ROW + g * (D / 16);
+            if constexpr (VW == 2)
+              asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(wv[x][0]), "=r"(wv[x][1]) : "r"(at));
+            else
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(wv[x][0]) : "r"(at));
+            asm volatile("{.reg .b16 h; ld.shared.u8 h, [%1]; cvt.u32.u16 %0, h;}"
+                         : "=r"(sb[x]) : "r"(sVs + key * C4::SROW + g * (D / 8) / 16));
           }
-          if (clear) {
+          // a masked key's scale may be a NaN pattern: the mask clears the product, not the factor
+          const uint32_t sv0 = e4m3x2_to_f16x2(sb[0] | (sb[1] << 8)), sv1 = e4m3x2_to_f16x2(sb[2] | (sb[3] << 8));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              f[0][i] &= vm0;
-              f[1][i] &= vm0;
-              f[2][i] &= vm1;
-              f[3][i] &= vm1;
+          for (int w = 0; w < VW; ++w) {
+            constexpr uint32_t M = 0x0F0F0F0Fu;
+            uint32_t f[4][4];                           // lo and hi of keys 2t, 2t + 1; of keys 2t + 8, 2t + 9
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t ka = wv[2 * x][w], kb = wv[2 * x + 1][w], sc2 = x ? sv1 : sv0;
+              e2m1x8_to_f16((ka & M) | ((kb << 4) & ~M), f[2 * x]);
+              e2m1x8_to_f16(((ka >> 4) & M) | (kb & ~M), f[2 * x + 1]);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                f[2 * x][k] = hmul2(f[2 * x][k], sc2);
+                f[2 * x + 1][k] = hmul2(f[2 * x + 1][k], sc2);
+              }
             }
-          }
+            if (clear) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t a[4] = {f[0][i], f[1][i], f[2][i], f[3][i]};
+              for (int k = 0; k < 4; ++k) {
+                f[0][k] &= vm0;
+                f[1][k] &= vm0;
+                f[2][k] &= vm1;
+                f[3][k] &= vm1;
+              }
+            }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_16816<true>(o[w * 4 + i][nt], a, pb[nt][0], pb[nt][1]);
-              if (HILO) mma_16816<true>(o[w * 4 + i][nt], a, pl[nt][0], pl[nt][1]);
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t a[4] = {f[0][k], f[1][k], f[2][k], f[3][k]};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_16816<true>(o[w * 4 + k][nt], a, pb[ks][nt][0], pb[ks][nt][1]);
+                if (HILO) mma_16816<true>(o[w * 4 + k][nt], a, pl[ks][nt][0], pl[ks][nt][1]);
+              }
             }
           }
         }
