@@ -34,6 +34,7 @@ struct AppendParams {
   long long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, qo_ts, qo_hs;
   int q_heads, rot;        // rot: dimensions that are rotated
   int shares;              // warps per token
+  float k_six, k_inv_six, v_six, v_inv_six;   // FP4: 6 * global and its reciprocal
 };
 struct GatherParams {
   PagedBatch batch;
@@ -83,15 +84,44 @@ __device__ __noinline__ void angle_64(int pos, float inv_freq, double* s, double
   sincos((double)pos * (double)inv_freq, s, c);
 }
 
-// 8 values -> 8 codes of 4 bits, first value lowest
-__device__ __forceinline__ uint32_t e2m1_codes(const float (&y)[8], float s) {
+// The quotient a / b rounded to nearest from inv = 1 / b rounded to nearest: q = a inv, then one correction by its exact
+// remainder (P. Markstein's theorem).  16-bit values meet the rounding borders of e2m1 and e4m3 exactly, where a plain
+// product with the reciprocal would miss the tie.  For b and a / b well inside the range of f32.
+__device__ __forceinline__ float quotient(float a, float b, float inv) {
+  const float q = __fmul_rn(a, inv);
+  return __fmaf_rn(__fmaf_rn(-q, b, a), inv, q);
+}
+// A block's scale e4m3(amax / (6 g)) and 8 of its values -> codes of 4 bits, first value lowest.
+struct BlockScale {
+  uint32_t byte;
+  float s, inv;
+  bool plain;              // the quotients need the general division: s far out of range, or an infinity in the block
+};
+__device__ __forceinline__ BlockScale block_scale(float amax, float glob, float six_g, float inv_six_g) {
+  BlockScale x;
+  const bool tame = amax < 0x1p100f && (amax > 0x1p-100f || amax == 0.0f) && six_g > 0x1p-20f && six_g < 0x1p20f;
+  const float q = tame ? quotient(amax, six_g, inv_six_g) : __fdiv_rn(amax, six_g);
+  x.byte = __nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
+  x.s = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)x.byte, __NV_E4M3))) * glob;
+  x.inv = __frcp_rn(x.s);
+  x.plain = !tame;
+  return x;
+}
+__device__ __noinline__ uint32_t e2m1_codes_plain(float a, float b, float s) {
+  return (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(__fdiv_rn(a, s), __fdiv_rn(b, s)), __NV_E2M1, cudaRoundNearest);
+}
+__device__ __forceinline__ uint32_t e2m1_codes(const float (&y)[8], const BlockScale& b) {
+  if (!(b.s > 0.0f)) return 0u;
   uint32_t w = 0;
+  if (b.plain) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    // true divisions: 16-bit values meet the rounding borders of e2m1 exactly, where a reciprocal would miss the tie
-    const float2 d = s > 0.0f ? make_float2(__fdiv_rn(y[2 * i], s), __fdiv_rn(y[2 * i + 1], s)) : make_float2(0.0f, 0.0f);
-    w |= (uint32_t)__nv_cvt_float2_to_fp4x2(d, __NV_E2M1, cudaRoundNearest) << (8 * i);
+    for (int i = 0; i < 4; ++i) w |= e2m1_codes_plain(y[2 * i], y[2 * i + 1], b.s) << (8 * i);
+    return w;
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(quotient(y[2 * i], b.s, b.inv), quotient(y[2 * i + 1], b.s, b.inv)),
+                                            __NV_E2M1, cudaRoundNearest) << (8 * i);
   return w;
 }
 
@@ -103,10 +133,6 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
   const long long warp_id = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int t = (int)(warp_id / p.shares), share = (int)(warp_id - (long long)t * p.shares);
   if (t >= p.batch.tokens) return;
-  const int b = seq_of_token(p.batch, t, lane);
-  if (b < 0) return;
-  const TokenPlace at = place_of(p.batch, b, t, status);
-
   const int sub = lane % LPH;
   const int total = p.q_heads + 2 * p.c.kv_heads;
   const int stride = HPW * p.shares;
@@ -138,6 +164,10 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
     lo[j] = hi[j] = make_uint4(0, 0, 0, 0);
     load(first + j * stride, lo[j], hi[j]);
   }
+  // the rows are on their way (they do not depend on the sequence) while the token's place is looked up
+  const int b = seq_of_token(p.batch, t, lane);
+  if (b < 0) return;
+  const TokenPlace at = place_of(p.batch, b, t, status);
 
   // cos and sin of this lane's 8 pairs: every lane evaluates LPH / 4 of them, the others come by shuffle
   float cs[8], sn[8];
@@ -214,7 +244,7 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
           }
         }
       }
-      if (FP4) {
+      if (FP4 && i - lane / LPH + HPW > p.q_heads) {           // warp-uniform: some head of this round is K's or V's
         // a block of 16 is this vector and its neighbour lane's (rotated pairs, V) or this lane's two (the rest)
         float ma = 0.0f, mc = 0.0f;
 #pragma unroll
@@ -225,29 +255,21 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
         const float na = __shfl_xor_sync(0xffffffffu, ma, 1), nc = __shfl_xor_sync(0xffffffffu, mc, 1);
         if (!is_q && i < total && at.page >= 0) {
           const bool halves = is_v || rotates;
-          ma = fmaxf(ma, halves ? na : mc);
-          mc = halves ? fmaxf(mc, nc) : ma;
-          const float gl = is_v ? p.c.v_global : p.c.k_global;
-          const __nv_fp8_storage_t sa = __nv_cvt_float_to_fp8(__fdiv_rn(ma, 6.0f * gl), __NV_SATFINITE, __NV_E4M3);
-          const __nv_fp8_storage_t sc = __nv_cvt_float_to_fp8(__fdiv_rn(mc, 6.0f * gl), __NV_SATFINITE, __NV_E4M3);
-          const float fa = __half2float(__half(__nv_cvt_fp8_to_halfraw(sa, __NV_E4M3))) * gl;
-          const float fc = __half2float(__half(__nv_cvt_fp8_to_halfraw(sc, __NV_E4M3))) * gl;
+          const float both = fmaxf(ma, mc);
+          const float gl = is_v ? p.c.v_global : p.c.k_global, six = is_v ? p.v_six : p.k_six,
+                      inv = is_v ? p.v_inv_six : p.k_inv_six;
+          const BlockScale sa = block_scale(halves ? fmaxf(ma, na) : both, gl, six, inv);
+          const BlockScale sc = block_scale(halves ? fmaxf(mc, nc) : both, gl, six, inv);
           const long long h = is_v ? i - p.q_heads - p.c.kv_heads : i - p.q_heads;
           const long long* st = is_v ? p.c.v_st : p.c.k_st;
           const long long* sst = is_v ? p.c.vs_st : p.c.ks_st;
           uint8_t* row = (is_v ? p.c.v : p.c.k) + at.page * st[0] + h * st[1] + at.slot * st[2];
           uint8_t* srow = (is_v ? p.c.vs : p.c.ks) + at.page * sst[0] + h * sst[1] + at.slot * sst[2];
           const int da = is_v ? v_lo : lo_at, dc = is_v ? v_hi : hi_at;
-          *reinterpret_cast<uint32_t*>(row + da / 2) = e2m1_codes(a, fa);
-          *reinterpret_cast<uint32_t*>(row + dc / 2) = e2m1_codes(c, fc);
-          if (halves) {
-            if ((sub & 1) == 0) {
-              srow[da / 16] = sa;
-              srow[dc / 16] = sc;
-            }
-          } else {
-            srow[da / 16] = sa;
-          }
+          *reinterpret_cast<uint32_t*>(row + da / 2) = e2m1_codes(a, sa);
+          *reinterpret_cast<uint32_t*>(row + dc / 2) = e2m1_codes(c, sc);
+          if (!halves || (sub & 1) == 0) srow[da / 16] = (uint8_t)sa.byte;
+          if (halves && (sub & 1) == 0) srow[dc / 16] = (uint8_t)sc.byte;
         }
       }
     }
@@ -265,37 +287,53 @@ __global__ void __launch_bounds__(128) paged_gather_kernel(const __grid_constant
   const int b = seq_of_token(p.batch, t, lane);
   if (b < 0) return;
   const TokenPlace at = place_of(p.batch, b, t, status);
-  const int sub = lane % LPH, total = 2 * p.c.kv_heads;
-  for (int i = share * HPW + lane / LPH; i < total; i += HPW * p.shares) {
-    const bool is_v = i >= p.c.kv_heads;
-    const long long h = is_v ? i - p.c.kv_heads : i;
-    uint4 y0 = make_uint4(0, 0, 0, 0), y1 = y0;
-    if (at.page >= 0) {
+  const int sub = lane % LPH, total = 2 * p.c.kv_heads, stride = HPW * p.shares;
+  constexpr int U = 4;                        // rounds whose loads are in flight together
+  for (int i0 = share * HPW + lane / LPH; i0 - lane / LPH < total; i0 += U * stride) {
+    uint4 y0[U], y1[U];                       // FP4: y0.x, y0.y the codes, y0.z the scale
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = i0 + j * stride;
+      y0[j] = y1[j] = make_uint4(0, 0, 0, 0);
+      if (i >= total || at.page < 0) continue;
+      const bool is_v = i >= p.c.kv_heads;
+      const long long h = is_v ? i - p.c.kv_heads : i;
       const long long* st = is_v ? p.c.v_st : p.c.k_st;
       const uint8_t* row = (is_v ? p.c.v : p.c.k) + at.page * st[0] + h * st[1] + at.slot * st[2];
       if constexpr (!FP4) {
-        y0 = __ldg(reinterpret_cast<const uint4*>(row) + sub * 2);
-        y1 = __ldg(reinterpret_cast<const uint4*>(row) + sub * 2 + 1);
+        y0[j] = __ldg(reinterpret_cast<const uint4*>(row) + sub * 2);
+        y1[j] = __ldg(reinterpret_cast<const uint4*>(row) + sub * 2 + 1);
       } else {
         const long long* sst = is_v ? p.c.vs_st : p.c.ks_st;
         const uint8_t* srow = (is_v ? p.c.vs : p.c.ks) + at.page * sst[0] + h * sst[1] + at.slot * sst[2];
         const uint2 w = __ldg(reinterpret_cast<const uint2*>(row) + sub);
-        const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw(__ldg(srow + sub), __NV_E4M3))) *
-                        (is_v ? p.c.v_global : p.c.k_global);
-        uint32_t o[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t byte = ((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu;
-          const float2 f = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)byte, __NV_E2M1)));
-          o[j] = paged_pack16<F16>(f.x * s, f.y * s);
-        }
-        y0 = make_uint4(o[0], o[1], o[2], o[3]);
-        y1 = make_uint4(o[4], o[5], o[6], o[7]);
+        y0[j] = make_uint4(w.x, w.y, __ldg(srow + sub), 0);
       }
     }
-    uint16_t* dst = is_v ? p.v_out + (long long)t * p.v_ts + h * p.v_hs : p.k_out + (long long)t * p.k_ts + h * p.k_hs;
-    reinterpret_cast<uint4*>(dst)[sub * 2] = y0;
-    reinterpret_cast<uint4*>(dst)[sub * 2 + 1] = y1;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int i = i0 + j * stride;
+      if (i >= total) continue;
+      const bool is_v = i >= p.c.kv_heads;
+      const long long h = is_v ? i - p.c.kv_heads : i;
+      if constexpr (FP4) {
+        const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)y0[j].z, __NV_E4M3))) *
+                        (is_v ? p.c.v_global : p.c.k_global);
+        const uint32_t w[2] = {y0[j].x, y0[j].y};
+        uint32_t o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const __half2_raw c = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(w[k >> 2] >> (8 * (k & 3))), __NV_E2M1);
+          const float2 f = __half22float2(__half2(c));
+          o[k] = paged_pack16<F16>(f.x * s, f.y * s);
+        }
+        y0[j] = make_uint4(o[0], o[1], o[2], o[3]);
+        y1[j] = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+      uint16_t* dst = is_v ? p.v_out + (long long)t * p.v_ts + h * p.v_hs : p.k_out + (long long)t * p.k_ts + h * p.k_hs;
+      reinterpret_cast<uint4*>(dst)[sub * 2] = y0[j];
+      reinterpret_cast<uint4*>(dst)[sub * 2 + 1] = y1[j];
+    }
   }
 }
 
@@ -348,6 +386,8 @@ int b200_paged_append_dispatch(int dtype, const b200tile_paged_cache& c, const b
   p.qo_ts = qos ? qos[0] : 0; p.qo_hs = qos ? qos[1] : 0;
   p.q_heads = q ? q_heads : 0;
   p.rot = rot;
+  p.k_six = 6.0f * c.k_global; p.k_inv_six = 1.0f / p.k_six;
+  p.v_six = 6.0f * c.v_global; p.v_inv_six = 1.0f / p.v_six;
   const int hpw = 32 / (c.head_dim / 16);
   p.shares = shares_for(batch.tokens, (p.q_heads + 2 * c.kv_heads + hpw - 1) / hpw, di->sm_count);
   const long long warps = (long long)batch.tokens * p.shares;
