@@ -824,42 +824,63 @@ def linear_nvfp4_prepared(z: Tensor, x: Tensor, y: Tensor, x_scales: Tensor, y_s
     return z
 
 
-# The paged calls sit in decode loops, where a kernel takes a few microseconds: one comparison per tensor decides whether
-# it is what the call needs, and only a mismatch looks for the reason.
+# The paged calls sit in decode loops, where a kernel takes a few microseconds: what a call has to know of a Tensor is
+# worked out once and kept with it, one comparison decides whether it fits, and only a mismatch looks for the reason.
+_PAGED_DTYPES = {"bf16": b"bf16", "f16": b"f16"}
+
+
+def _paged_describe(t: Tensor):
+    pair = _i64x2(t.strides[0], t.strides[1]) if len(t.shape) == 3 else None
+    t._row_strides, t._row_strides_at = pair, ctypes.addressof(pair) if pair is not None else 0
+    fits = len(t.shape) == 3 and t.strides[2] == 1
+    t._paged_key = (*t.shape, t.dtype, t.storage.device) if fits else ()
+    return t._paged_key
+
+
 def _paged_rows(who: str, name: str, t: Tensor, tokens: int, heads: int, cache: PagedKvCache, dt: str) -> int:
     """Checks that ``t`` is [tokens, heads, D] of type ``dt`` beside the cache; the address of its {token, head} strides."""
+    key = t.__dict__.get("_paged_key") or _paged_describe(t)
+    if key == (tokens, heads, cache.head_dim, dt, cache.device):
+        return t._row_strides_at
     if t.shape != [tokens, heads, cache.head_dim]:
         raise KernelLaunchError(f"{who}: {name} is {t.shape}, expected [{tokens}, {heads}, {cache.head_dim}]")
     if t.strides[2] != 1:
         raise KernelLaunchError(f"{who}: the head vectors of {name} must be contiguous")
     if t.dtype != dt:
         raise KernelLaunchError(f"{who}: the tensors have different element types, {name} is {t.dtype} beside {dt}")
-    if t.storage.device != cache.device:
-        raise KernelLaunchError(f"{who}: {name} is on {t.storage.device}, the cache on {cache.device}")
-    pair = t.__dict__.get("_row_strides")
-    if pair is None:
-        pair = t._row_strides = _i64x2(t.strides[0], t.strides[1])
-        t._row_strides_at = ctypes.addressof(pair)
-    return t._row_strides_at
+    raise KernelLaunchError(f"{who}: {name} is on {t.storage.device}, the cache on {cache.device}")
 
 
 def _paged_dtype(who: str, cache: PagedKvCache, dt: str) -> bytes:
     if cache.dtype is not None and cache.dtype != dt:
         raise KernelLaunchError(f"{who}: the cache holds {cache.dtype}, the tensors {dt}")
-    return dt.encode()
+    name = _PAGED_DTYPES.get(dt)
+    if name is None:
+        raise KernelLaunchError(f"{who}: unsupported element type {dt}")
+    return name
 
 
 def _paged_stream(who: str, cache: PagedKvCache, batch: PagedBatch, stream: Optional[torch.cuda.Stream]) -> int:
     dev = cache.device
     if batch.device != dev:
         raise KernelLaunchError(f"{who}: the batch is on {batch.device}, the cache on {dev}")
-    if dev.type != "cuda" or torch.cuda.current_device() != dev.index:
+    if dev.type != "cuda" or torch._C._cuda_getDevice() != dev.index:
         raise KernelLaunchError(f"{who}: the cache is on {dev}, which is not the current device")
     if stream is None:
         return torch._C._cuda_getCurrentRawStream(dev.index)
     if stream.device != dev:
         raise KernelLaunchError(f"{who}: the stream is on {stream.device}, the cache on {dev}")
     return stream.cuda_stream
+
+
+def _paged_inv_freq(who: str, t: Tensor, cache: PagedKvCache) -> int:
+    key = t.__dict__.get("_inv_freq_key")
+    if key is None:
+        ok = t.dtype == "f32" and len(t.shape) == 1 and (t.strides[0] == 1 or t.shape[0] < 2)
+        key = t._inv_freq_key = (t.storage.device, 2 * t.shape[0]) if ok else (None, 0)
+    if key[0] != cache.device:
+        raise KernelLaunchError(f"{who}: inv_freq must be a contiguous f32 vector on {cache.device}")
+    return key[1]
 
 
 def paged_kv_append(cache: PagedKvCache, batch: PagedBatch, k: Tensor, v: Tensor, q: Optional[Tensor] = None,
@@ -882,10 +903,7 @@ def paged_kv_append(cache: PagedKvCache, batch: PagedBatch, k: Tensor, v: Tensor
                                                                                    cache, dt)
         qp, qop = q.storage.data_ptr(), q_out.storage.data_ptr()
     if inv_freq is not None:
-        if inv_freq.dtype != "f32" or len(inv_freq.shape) != 1 or inv_freq.strides[0] != 1 or \
-                inv_freq.storage.device != cache.device:
-            raise KernelLaunchError(f"{who}: inv_freq must be a contiguous f32 vector on {cache.device}")
-        rot = 2 * inv_freq.shape[0]
+        rot = _paged_inv_freq(who, inv_freq, cache)
         f = inv_freq.storage.data_ptr()
     dt = _paged_dtype(who, cache, dt)
     rc = lib.b200tile_paged_kv_append(dt, cache.c, batch.c, qp, k.storage.data_ptr(), v.storage.data_ptr(), qop, f, tokens,
