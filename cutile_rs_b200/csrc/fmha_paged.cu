@@ -101,6 +101,7 @@ struct SplitParams {
   int4* desc;
   long long part_floats;
   int workers, by_item, rb_max;
+  int coop;                          // CTAs per item (a cluster), whose warps share its steps: no parts, no merge kernel; or 0
   int min_steps;
   // FP4 operands, strides in bytes: those that are multiplied in every step fit in 32 bits
   const uint8_t *k, *v, *ks, *vs;
@@ -263,6 +264,31 @@ struct Core4 {
   static constexpr int SMEM = RING;
 };
 
+// One 16 x 8 tile of O^T (numerators and their sums) to the output rows of block nt.
+template <int D, bool F16, bool FP4, int NT>
+__device__ __forceinline__ void write_tile(const SplitParams& p, const SeqView& sv, int rb, int h, int nt, int c, int lane,
+                                           const float (&o)[4], const float (&l)[2]) {
+  const int g = lane >> 2, t = lane & 3;
+  // a row that saw nothing is 0; NaN stays NaN
+  const float i0 = l[0] == 0.0f ? 0.0f : (FP4 ? p.out_scale : 1.0f) / l[0];
+  const float i1 = l[1] == 0.0f ? 0.0f : (FP4 ? p.out_scale : 1.0f) / l[1];
+  // (dimension, rows 2t, 2t + 1) -> (row g, dimensions 2t, 2t + 1 of the tile's eight)
+  const uint32_t a = mat_trans(paged_pack16<F16>(o[0] * i0, o[1] * i1));
+  const uint32_t d2 = mat_trans(paged_pack16<F16>(o[2] * i0, o[3] * i1));
+  const int row = rb * 8 * NT + nt * 8 + g;
+  const int tok = row / p.group;
+  if (tok >= sv.n) return;
+  uint16_t* orow = p.out + (long long)(sv.q0 + tok) * p.o_ts + (long long)(h * p.group + row - tok * p.group) * p.o_hs;
+  if constexpr (!FP4) {
+    *reinterpret_cast<uint32_t*>(orow + c * 16 + 2 * t) = a;
+    *reinterpret_cast<uint32_t*>(orow + c * 16 + 8 + 2 * t) = d2;
+  } else {
+    // tile row m stands for dimension D/8 m + 2c, row m + 8 for the next one
+    *reinterpret_cast<uint32_t*>(orow + (D / 8) * (2 * t) + 2 * c) = __byte_perm(a, d2, 0x5410);
+    *reinterpret_cast<uint32_t*>(orow + (D / 8) * (2 * t + 1) + 2 * c) = __byte_perm(a, d2, 0x7632);
+  }
+}
+
 // Finds the first piece of work of every worker of the CTA.  s_sum[i] = steps of the sequences before chunk i.
 template <int RB, int THREADS>
 __device__ __forceinline__ long long block_line(const SplitParams& p, long long* s_sum) {
@@ -330,31 +356,43 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
   } else {
     ring = base + warp * (STAGES * C4::STAGE);
   }
-  const long long total = block_line<RB, THREADS>(p, s_sum);
-
-  const int wid = warp * gridDim.x + blockIdx.x;     // neighbouring runs on different SMs
-  long long per = (total + p.workers - 1) / p.workers;
-  if (per < p.min_steps) per = p.min_steps;
-  long long u = (long long)wid * per;
-  const long long u_end = min(total, u + per);
-  if (!p.by_item && lane == 0) p.desc[wid] = make_int4(0, 0, 0, 0);
-  if (u >= u_end) return;
-
-  // the sequence that holds step u: binary search over the chunks, then along the chunk
-  int c_lo = 0, c_hi = THREADS - 1;
-  while (c_lo < c_hi) {
-    const int mid = (c_lo + c_hi + 1) >> 1;
-    if (s_sum[mid] <= u) c_lo = mid;
-    else c_hi = mid - 1;
-  }
-  const int chunk = (p.batch.batch + THREADS - 1) / THREADS;
-  int b = c_lo * chunk;
-  long long line = s_sum[c_lo];                       // first step of sequence b
-  SeqWork sw = seq_work<RB>(p, b);
-  while (line + (long long)sw.rbs * p.kv_heads * sw.steps <= u) {
-    line += (long long)sw.rbs * p.kv_heads * sw.steps;
-    if (++b >= p.batch.batch) return;
+  long long per = 0, u = 0, u_end = 0, line = 0;
+  int b, wid = 0, coop_rb = 0, coop_h = 0;
+  SeqWork sw;
+  if (p.coop) {
+    const int item = blockIdx.x / p.coop;               // (sequence * rb_max + row block) * kv_heads + head
+    b = item / (p.rb_max * p.kv_heads);
+    coop_rb = item / p.kv_heads % p.rb_max;
+    coop_h = item % p.kv_heads;
     sw = seq_work<RB>(p, b);
+    if (coop_rb >= sw.rbs) return;                      // the whole cluster
+    __syncthreads();
+    u_end = 1;
+  } else {
+    const long long total = block_line<RB, THREADS>(p, s_sum);
+    wid = warp * gridDim.x + blockIdx.x;                // neighbouring runs on different SMs
+    per = (total + p.workers - 1) / p.workers;
+    if (per < p.min_steps) per = p.min_steps;
+    u = (long long)wid * per;
+    u_end = min(total, u + per);
+    if (!p.by_item && lane == 0) p.desc[wid] = make_int4(0, 0, 0, 0);
+    if (u >= u_end) return;
+
+    // the sequence that holds step u: binary search over the chunks, then along the chunk
+    int c_lo = 0, c_hi = THREADS - 1;
+    while (c_lo < c_hi) {
+      const int mid = (c_lo + c_hi + 1) >> 1;
+      if (s_sum[mid] <= u) c_lo = mid;
+      else c_hi = mid - 1;
+    }
+    b = c_lo * ((p.batch.batch + THREADS - 1) / THREADS);
+    line = s_sum[c_lo];                                 // first step of sequence b
+    sw = seq_work<RB>(p, b);
+    while (line + (long long)sw.rbs * p.kv_heads * sw.steps <= u) {
+      line += (long long)sw.rbs * p.kv_heads * sw.steps;
+      if (++b >= p.batch.batch) return;
+      sw = seq_work<RB>(p, b);
+    }
   }
 
   uint32_t ring_at = 0;        // steps taken through the ring since the kernel began (stage and phase of the next)
@@ -362,13 +400,22 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
   const int ck = lane >> 4, cv = (lane >> 3) & 1;
 
   while (u < u_end) {
-    const long long rel = u - line;
-    const int item = (int)(rel / sw.steps);
-    const int st0 = (int)(rel - (long long)item * sw.steps);
-    const int st1 = (int)min((long long)sw.steps, st0 + (u_end - u));
-    const int rb = item / p.kv_heads, h = item - rb * p.kv_heads;
+    int item = 0, st0, st1, rb, h;
+    if (p.coop) {
+      const int share = (sw.steps + p.coop * WARPS - 1) / (p.coop * WARPS);
+      st0 = min(sw.steps, ((int)blockIdx.x % p.coop * WARPS + warp) * share);
+      st1 = min(sw.steps, st0 + share);
+      rb = coop_rb;
+      h = coop_h;
+    } else {
+      const long long rel = u - line;
+      item = (int)(rel / sw.steps);
+      st0 = (int)(rel - (long long)item * sw.steps);
+      st1 = (int)min((long long)sw.steps, st0 + (u_end - u));
+      rb = item / p.kv_heads;
+      h = item - rb * p.kv_heads;
+    }
     const SeqView& sv = sw.s;
-    const int rows = min(RB, sv.n * p.group - rb * RB);
     RowMask<NT> rm = row_mask<NT>(p, sv, rb, lane);
     // the part's key steps, cut to what the block's rows can see
     const int k0 = max(sw.base + st0, rm.lo_min / STEP);
@@ -697,36 +744,107 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
         l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], 8);
         l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], 16);
       }
-    const bool whole = st0 == 0 && st1 == sw.steps;
-    if (whole) {
-      float inv[NT][2];
+    if (p.coop) {
+      // the warps' parts through shared memory, each in its own ring (done with), and added tile by tile
+      float* mine = reinterpret_cast<float*>(smem_raw + (ring - smem_u32(smem_raw)));
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int c = 0; c < DT; ++c)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)   // a row that saw nothing is 0; NaN stays NaN
-          inv[nt][j] = l_run[nt][j] == 0.0f ? 0.0f : (FP4 ? p.out_scale : 1.0f) / l_run[nt][j];
+        for (int nt = 0; nt < NT; ++nt)
+          reinterpret_cast<float4*>(mine)[(c * NT + nt) * 32 + lane] =
+              make_float4(o[c][nt][0], o[c][nt][1], o[c][nt][2], o[c][nt][3]);
+      if (g == 0) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int row = rb * RB + nt * 8 + g;
-        const int tok = row / p.group;
-        uint16_t* orow = p.out + (long long)(sv.q0 + tok) * p.o_ts + (long long)(h * p.group + row - tok * p.group) * p.o_hs;
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 0; c < DT; ++c) {
-          // (dimension, rows 2t, 2t + 1) -> (row g, lanes' dimensions 2t, 2t + 1 of the tile's eight)
-          const uint32_t a = mat_trans(paged_pack16<F16>(o[c][nt][0] * inv[nt][0], o[c][nt][1] * inv[nt][1]));
-          const uint32_t d2 = mat_trans(paged_pack16<F16>(o[c][nt][2] * inv[nt][0], o[c][nt][3] * inv[nt][1]));
-          if (nt * 8 + g < rows) {
-            if constexpr (!FP4) {
-              *reinterpret_cast<uint32_t*>(orow + c * 16 + 2 * t) = a;
-              *reinterpret_cast<uint32_t*>(orow + c * 16 + 8 + 2 * t) = d2;
-            } else {
-              // tile row m stands for dimension D/8 m + 2c, row m + 8 for the next one
-              *reinterpret_cast<uint32_t*>(orow + (D / 8) * (2 * t) + 2 * c) = __byte_perm(a, d2, 0x5410);
-              *reinterpret_cast<uint32_t*>(orow + (D / 8) * (2 * t + 1) + 2 * c) = __byte_perm(a, d2, 0x7632);
-            }
+          for (int j = 0; j < 2; ++j) {
+            mine[DT * NT * 128 + nt * 8 + 2 * t + j] = m_run[nt][j];
+            mine[DT * NT * 128 + RB + nt * 8 + 2 * t + j] = l_run[nt][j];
+          }
+      }
+      __syncthreads();
+      constexpr int RING_BYTES = STAGES * (FP4 ? C4::STAGE : C16::STAGE);
+      constexpr int TILE_BYTES = 32 * 16 + 2 * 8 * 4;  // a tile of the CTA's sum: O, and m and l of its eight rows
+      static_assert(RING_BYTES >= RB * (D + 2) * 4 && WARPS >= DT, "a part fits a ring, a warp takes a tile");
+      auto add = [&](float (&m)[2], float (&l)[2], float (&x)[4], const float2& pm, const float2& pl2, const float4& v) {
+        const float a[2] = {pm.x, pm.y}, q[2] = {pl2.x, pl2.y}, vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float mn = fmaxf(m[j], a[j]), mu = mn == -CUDART_INF_F ? 0.0f : mn;
+          const float wa = paged_ex2(m[j] - mu), wb = paged_ex2(a[j] - mu);
+          m[j] = mn;
+          l[j] = l[j] * wa + q[j] * wb;
+          x[j] = x[j] * wa + vv[j] * wb;
+          x[2 + j] = x[2 + j] * wa + vv[2 + j] * wb;
+        }
+      };
+      // warp c: tile c of every warp's part
+      const int c = warp;
+      float m[NT][2], l[NT][2], x[NT][4];
+      if (c < DT) {
+        const float* all = reinterpret_cast<const float*>(smem_raw + (base - smem_u32(smem_raw)));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          m[nt][0] = m[nt][1] = -CUDART_INF_F;
+          l[nt][0] = l[nt][1] = x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.0f;
+#pragma unroll 4
+          for (int w = 0; w < WARPS; ++w) {
+            const float* src = all + w * (RING_BYTES / 4);
+            const float* ml = src + DT * NT * 128 + nt * 8 + 2 * t;
+            add(m[nt], l[nt], x[nt], *reinterpret_cast<const float2*>(ml), *reinterpret_cast<const float2*>(ml + RB),
+                reinterpret_cast<const float4*>(src)[(c * NT + nt) * 32 + lane]);
           }
         }
       }
+      if (p.coop == 1) {
+        if (c < DT)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) write_tile<D, F16, FP4, NT>(p, sv, rb, h, nt, c, lane, x[nt], l[nt]);
+        return;
+      }
+      // the cluster's CTAs: every one leaves its sums in its shared memory, and tile c goes to CTA c mod coop
+      __syncthreads();                                 // the warps' parts have been read
+      if (c < DT) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float* dst = reinterpret_cast<float*>(smem_raw + (base - smem_u32(smem_raw)) + (c * NT + nt) * TILE_BYTES);
+          reinterpret_cast<float4*>(dst)[lane] = make_float4(x[nt][0], x[nt][1], x[nt][2], x[nt][3]);
+          if (g == 0) {
+            *reinterpret_cast<float2*>(dst + 128 + 2 * t) = make_float2(m[nt][0], m[nt][1]);
+            *reinterpret_cast<float2*>(dst + 136 + 2 * t) = make_float2(l[nt][0], l[nt][1]);
+          }
+        }
+      }
+      cluster_sync_all();
+      if (c < DT && c % p.coop == (int)blockIdx.x % p.coop) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          m[nt][0] = m[nt][1] = -CUDART_INF_F;
+          l[nt][0] = l[nt][1] = x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.0f;
+          const uint32_t at = base + (c * NT + nt) * TILE_BYTES;
+#pragma unroll 8
+          for (int r = 0; r < p.coop; ++r) {
+            const uint32_t src = mapa_u32(at, r);
+            float4 v;
+            float2 pm, pl2;
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(src + lane * 16));
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(pm.x), "=f"(pm.y) : "r"(src + 512 + t * 8));
+            asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(pl2.x), "=f"(pl2.y) : "r"(src + 544 + t * 8));
+            add(m[nt], l[nt], x[nt], pm, pl2, v);
+          }
+          write_tile<D, F16, FP4, NT>(p, sv, rb, h, nt, c, lane, x[nt], l[nt]);
+        }
+      }
+      cluster_sync_all();                              // no CTA leaves while another reads its shared memory
+      return;
+    }
+    const bool whole = st0 == 0 && st1 == sw.steps;
+    if (whole) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < DT; ++c) write_tile<D, F16, FP4, NT>(p, sv, rb, h, nt, c, lane, o[c][nt], l_run[nt]);
     } else {
       const int slot = st0 == 0 ? 1 : 0;              // an item's first part, or the continuation of an earlier worker's
       float* dst = p.part + ((long long)wid * 2 + slot) * p.part_floats;
@@ -782,8 +900,12 @@ __global__ void __launch_bounds__(256) fmha_paged_merge_kernel(const __grid_cons
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!exists) return;
-  const int4 d = p.desc[blockIdx.x];
-  if (d.x == 0) return;
+  int4 d = p.desc[blockIdx.x];
+  // whatever a workspace holds that other work has written to meanwhile, nothing outside of it is touched
+  if (d.x <= 0 || (unsigned)d.y >= (unsigned)p.workers || (unsigned)d.z >= (unsigned)p.batch.batch || d.w < 0 ||
+      d.w >= p.rb_max * p.kv_heads)
+    return;
+  d.x = min(d.x, p.workers - d.y);
   const int pw = warp % PW, c = blockIdx.y * CT + warp / PW;
   const int b = d.z, rb = d.w / p.kv_heads, h = d.w % p.kv_heads;
   float m[NT][2], l[NT][2], o[NT][4];
@@ -857,23 +979,7 @@ __global__ void __launch_bounds__(256) fmha_paged_merge_kernel(const __grid_cons
   if (c >= DT) return;
   const SeqView sv = seq_view(p.batch, b);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const float i0 = l[nt][0] == 0.0f ? 0.0f : (FP4 ? p.out_scale : 1.0f) / l[nt][0];
-    const float i1 = l[nt][1] == 0.0f ? 0.0f : (FP4 ? p.out_scale : 1.0f) / l[nt][1];
-    const uint32_t a = mat_trans(paged_pack16<F16>(o[nt][0] * i0, o[nt][1] * i1));
-    const uint32_t d2 = mat_trans(paged_pack16<F16>(o[nt][2] * i0, o[nt][3] * i1));
-    const int row = rb * RB + nt * 8 + g;
-    const int tok = row / p.group;
-    if (tok >= sv.n) continue;
-    uint16_t* orow = p.out + (long long)(sv.q0 + tok) * p.o_ts + (long long)(h * p.group + row - tok * p.group) * p.o_hs;
-    if constexpr (!FP4) {
-      *reinterpret_cast<uint32_t*>(orow + c * 16 + 2 * t) = a;
-      *reinterpret_cast<uint32_t*>(orow + c * 16 + 8 + 2 * t) = d2;
-    } else {
-      *reinterpret_cast<uint32_t*>(orow + (D / 8) * (2 * t) + 2 * c) = __byte_perm(a, d2, 0x5410);
-      *reinterpret_cast<uint32_t*>(orow + (D / 8) * (2 * t + 1) + 2 * c) = __byte_perm(a, d2, 0x7632);
-    }
-  }
+  for (int nt = 0; nt < NT; ++nt) write_tile<D, F16, FP4, NT>(p, sv, rb, h, nt, c, lane, o[nt], l[nt]);
 }
 
 template <int D, bool F16, int NT, bool CAP, bool FP4>
@@ -901,6 +1007,7 @@ int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
   p.desc = reinterpret_cast<int4*>(static_cast<char*>(a.workspace) + plan.desc_off);
   p.workers = plan.workers;
   p.by_item = plan.by_item;
+  p.coop = plan.coop;
   p.rb_max = (int)((std::min<long long>((long long)a.batch.max_q * p.group, a.row_limit) + 8 * NT - 1) / (8 * NT));
   p.min_steps = 2;
   CUtensorMap tmK = {}, tmV = {};
@@ -929,19 +1036,29 @@ int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
     B200_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     attr_done.set(di->ordinal);
   }
-  kern<<<plan.ctas, THREADS, SMEM, a.stream>>>(tmK, tmV, p, di->status);
-  B200_CUDA_CHECK(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(plan.ctas);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = a.stream;
+  cfg.attrs = attr;
+  if (plan.coop > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = plan.coop;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tmK, tmV, p, di->status));
+  if (plan.coop) return B200_OK;
   // few items with many parts: all eight warps of a CTA share the parts of one tile; else a warp per tile
   const unsigned x = (unsigned)(plan.by_item ? plan.items : plan.workers);
   const bool wide = x * (D / 16) <= 8u * di->sm_count;
-  cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(x, wide ? D / 16 : 1);
   cfg.blockDim = dim3(256);
-  cfg.stream = a.stream;
-  cudaLaunchAttribute attr[1];
+  cfg.dynamicSmemBytes = 0;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (wide) B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fmha_paged_merge_kernel<D, F16, NT, FP4, 8>, p));
   else B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fmha_paged_merge_kernel<D, F16, NT, FP4, 1>, p));
@@ -952,6 +1069,8 @@ int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
 }  // namespace b200
 
 // The plan depends on sizes the host knows; SM count 148 is the part's (fewer SMs run the same CTAs in turn).
+static constexpr int COOP_STEPS = 16;
+
 PagedSplitPlan b200_paged_split_plan(int format, int head_dim, int kv_heads, int batch, long long rows,
                                      long long max_keys) {
   PagedSplitPlan pl;
@@ -960,6 +1079,21 @@ PagedSplitPlan b200_paged_split_plan(int format, int head_dim, int kv_heads, int
   const long long rb_max = (rows + pl.rows_per_block - 1) / pl.rows_per_block;
   pl.items = (long long)batch * rb_max * kv_heads;
   const long long steps = pl.items * ((max_keys + 15) / 16);
+  // As many CTAs per item as the machine has for it, if that leaves a warp a few steps only: 700 keys of 8 heads 6.8
+  // against 8.9 us, 18 x 8 items of 700 keys 9.9 against 21, of 2048 keys 29 against 39.  With more steps the two come
+  // together for equal lengths (1.03 at 18 x 32768 keys), and runs win where lengths differ, which the host does not
+  // know.  Clusters of eight stop fitting side by side at 16 of them (11.5 against 6.4 us for 8).
+  int per_item = 1;
+  while (per_item < 8 && pl.items * per_item * 2 <= (per_item == 4 ? 96 : 148)) per_item *= 2;
+  pl.coop = pl.items <= 148 && (max_keys + 15) / 16 <= (long long)per_item * warps * COOP_STEPS ? per_item : 0;
+  if (pl.coop) {
+    pl.ctas = (int)pl.items * pl.coop;
+    pl.workers = 0;
+    pl.by_item = false;
+    pl.part_floats = pl.desc_off = 0;
+    pl.bytes = 16;
+    return pl;
+  }
   pl.ctas = (int)std::max<long long>(1, std::min<long long>(148, (steps + 1) / 2));
   pl.workers = pl.ctas * warps;
   pl.by_item = pl.items <= pl.workers;

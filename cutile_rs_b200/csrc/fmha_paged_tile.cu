@@ -937,13 +937,15 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 template <int D, bool F16>
 __global__ void __launch_bounds__(128) fmha_paged_tile_merge_kernel(const __grid_constant__ TileParams p) {
   grid_dep_wait();
-  const int4 d = p.desc[blockIdx.x];
-  if (d.x == 0) return;
+  int4 d = p.desc[blockIdx.x];
+  // whatever a workspace holds that other work has written to meanwhile, nothing outside of it is touched
+  if (d.x <= 0 || (unsigned)d.y >= (unsigned)p.batch.batch || d.z < 0 || (unsigned)d.w >= (unsigned)p.kv_heads) return;
+  d.x = min(d.x, (int)(gridDim.x - blockIdx.x));
   const int t = blockIdx.y & 1, c0 = (blockIdx.y >> 1) * (D / 32);       // float4 columns c0 .. c0 + D / 32
   const int row = threadIdx.x, tok = row / p.group;
   const SeqView sv = seq_view(p.batch, d.y);
-  const int tok0 = (d.z * 2 + t) * p.tpt;
-  if (tok >= min(max(sv.n - tok0, 0), p.tpt)) return;
+  const long long tok0 = (d.z * 2ll + t) * p.tpt;
+  if (tok >= min(max(sv.n - tok0, 0ll), (long long)p.tpt)) return;
   float m = -CUDART_INF_F, l = 0.0f;
   float4 o[D / 32];
 #pragma unroll

@@ -117,6 +117,7 @@ struct PagedSplitPlan {
   int rows_per_block;     // 8 or 16 query rows of one K/V head
   int ctas, workers;      // one worker = one warp
   long long items;        // (sequence, row block, K/V head) at most
+  int coop;               // CTAs per item (no workspace needed), or 0: runs of the whole line
   bool by_item;           // descriptors indexed by item (few items) or by worker
   size_t part_floats;     // floats per partial-result slot
   size_t desc_off, bytes;
