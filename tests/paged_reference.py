@@ -103,11 +103,14 @@ def attention(p, scale, causal=True, window=0, softcap=0.0):
     error (a 32-bit dot product of d terms, the score's scale and the exponential's argument: (d + 8) 2^-24 of
     sum |q k| scale, with a cap 2^-19 of it more) and which are handed over in two 16-bit pieces (2^-15 of p; one f16 piece, 2^-11,
     for bf16 over NVFP4; one piece of the type, half a step, for sequences of many rows), all against sum p |v|; sums of n
-    terms in 32 bits."""
+    terms in 32 bits.  Pieces in f16 (f16 rows, and all rows over NVFP4) have no relative step below 2^-14: they are off by
+    up to half of f16's smallest step, 2^-25, each, while the largest p is at least 1 and so is the sum they are divided by:
+    2^-25 sum |v| over the keys seen."""
     out = torch.zeros(p.tokens, p.heads, p.d, dtype=torch.float64, device="cuda")
     tol = torch.zeros_like(out)
     group = p.heads // p.kvh
     eps = torch.finfo(p.dtype).eps
+    small_pieces = p.dtype == torch.float16 or p.fmt != "16bit"
     few = 2.0 ** -11 if p.fmt != "16bit" and p.dtype == torch.bfloat16 else 2.0 ** -15
     for b, (n, kv) in enumerate(zip(p.q_lens, p.kv_lens)):
         if n == 0 or kv <= 0:
@@ -135,7 +138,7 @@ def attention(p, scale, causal=True, window=0, softcap=0.0):
             o = w @ vh
             out[p.cu[b]:p.cu[b + 1], h] = o
             tol[p.cu[b]:p.cu[b + 1], h] = eps / 2 * o.abs() + (3 * ds + piece + (kv + 16) * 2.0 ** -24 + 2.0 ** -20) * \
-                (w @ vh.abs()) + 1e-7
+                (w @ vh.abs()) + (2.0 ** -25 * (seen.double() @ vh.abs()) if small_pieces else 0.0) + 1e-7
     return out, tol
 
 

@@ -173,6 +173,155 @@ def test_strided_rows(b200):
         assert (ow[:, :, 128:] == SENTINEL).all()
 
 
+@pytest.mark.parametrize("fmt,d,dtype", [("16bit", 128, BF16), ("16bit", 64, F16), ("nvfp4", 128, BF16), ("nvfp4", 64, F16)])
+def test_caps_near_and_far_from_the_scores(b200, fmt, d, dtype):
+    """Scores that are a small part of the cap, about its size, and far beyond it, in one call: the capped score has one
+    form for small arguments and one for all."""
+    for cap in (1.0, 4.0, 300.0):
+        p = ref.Problem([200, 3, 90], [260, 40, 90], 6, 2, d, 16, dtype, fmt, seed=40)
+        p.q[:70].mul_(6)
+        _check(p, d ** -0.5, softcap=cap)
+        _check(p, d ** -0.5, softcap=cap, window=50)
+
+
+@pytest.mark.parametrize("unit", [2.0 ** -30, 2.0 ** 13])
+def test_prompts_of_small_and_large_queries_over_fp4(b200, unit):
+    for softcap in (0.0, 20.0):
+        p = ref.Problem([150, 20], [300, 33], 4, 2, 128, 16, BF16, "nvfp4", seed=41)
+        p.q[::3].mul_(2.0 ** -9)                        # rows of very different size in one tile
+        p.q.mul_(unit)
+        _check(p, 128 ** -0.5 / unit, softcap=softcap)
+
+
+def test_many_heads_per_kv_head(b200):
+    """More heads per K/V head than a tile has rows: row blocks take the prompt."""
+    p = ref.Problem([3, 2], [40, 90], 260, 2, 64, 16, BF16, seed=42)
+    _check(p, 0.125)
+    p = ref.Problem([9, 1], [40, 90], 128, 1, 64, 16, F16, "nvfp4", seed=42)
+    _check(p, 0.125)
+
+
+def test_decode_runs_and_clusters_agree(b200):
+    """The same sequences behind a short block table (a cluster per item) and a long one (runs of the whole line)."""
+    for fmt in ("16bit", "nvfp4"):
+        for q_len in (1, 3):
+            p = ref.Problem([q_len] * 3, [700, 300, 45], 8, 2, 128, 16, F16, fmt, seed=43)
+            a = _check(p, 0.1)
+            wide = torch.full((3, 6000), -1, dtype=torch.int32, device="cuda")
+            wide[:, :p.table.shape[1]] = p.table
+            p.table = wide
+            p.batch = paged.PagedBatch(wide, p.cu_q, p.kv, q_len)
+            b = _check(p, 0.1)
+            assert (a.double() - b.double()).abs().max() <= 2.0 ** -9
+
+
+def test_workspace_contents_do_not_matter(b200):
+    for q_lens, kv_lens in (([1, 1], [30000, 17000]), ([100, 1], [5000, 600])):
+        for fmt in ("16bit", "nvfp4"):
+            p = ref.Problem(q_lens, kv_lens, 4, 2, 64, 64, BF16, fmt, seed=44)
+            ws = launch.paged_attention_workspace(p.cache, p.batch, 4)
+            a = _attend(p, 0.1, workspace=ws)
+            ws.fill_(255)                               # NaN everywhere, -1 in every descriptor
+            assert torch.equal(a, _attend(p, 0.1, workspace=ws))
+            ws.random_(0, 256)
+            assert torch.equal(a, _attend(p, 0.1, workspace=ws))
+
+
+def test_output_may_be_the_query_tensor(b200):
+    for q_lens in ([1, 1, 2], [130, 1, 70]):
+        p = ref.Problem(q_lens, [700, 40, 300], 4, 2, 128, 16, BF16, seed=45)
+        want = _attend(p, 0.1)
+        t = api.from_torch(p.q.clone())
+        launch.paged_attention(t, t, p.cache, p.batch, 0.1)
+        assert torch.equal(want, t.storage)
+
+
+def test_sequences_that_share_pages(b200):
+    """A common prefix in common pages, read by all."""
+    for fmt in ("16bit", "nvfp4"):
+        p = ref.Problem([1, 1, 80], [200, 220, 240], 4, 2, 64, 16, F16, fmt, seed=46)
+        p.table[1:, :9] = p.table[0, :9]
+        got = _attend(p, 0.2)
+        want, tol = ref.attention(p, 0.2)
+        assert ((got.double() - want).abs() <= tol).all()
+
+
+def test_lengths_and_ranges_that_do_not_fit(b200):
+    """Lengths beyond the block table, negative ones, token ranges beyond the tensors: what fits is computed, nothing else
+    is touched."""
+    for fmt in ("16bit", "nvfp4"):
+        for q_lens in ([1, 1, 1], [100, 1, 90]):
+            p = ref.Problem(q_lens, [150, 60, 120], 4, 2, 64, 16, BF16, fmt, seed=47)
+            cap = p.table.shape[1] * 16
+            p.table.clamp_(min=0)                       # every entry a page: positions up to the table's end exist
+            p.kv[0] = cap + 37                          # keys behind the table are left out, positions keep counting
+            got = _attend(p, 0.2)
+            n = q_lens[0]
+            k, v = p.rows(0, cap)
+            pos = torch.arange(cap + 37 - n, cap + 37, device="cuda")[:, None]
+            seen = torch.arange(cap, device="cuda")[None] <= pos
+            s = (p.q[:n, 0].double() @ k[:, 0].T * 0.2).masked_fill(~seen, float("-inf"))
+            want = torch.softmax(s, -1) @ v[:, 0]
+            assert ((got[:n, 0].double() - want).abs() <= 2.0 ** -6).all()
+            before = [x.clone() for x in p.pools]
+            p.kv[1] = -5
+            p.cu_q[3] = p.tokens + 1000                 # the last sequence's range reaches behind the tensors
+            got = _attend(p, 0.2)
+            assert (got[p.cu[1]:p.cu[2]] == 0).all() and not torch.isnan(got).any()
+            p.kv[0] = cap + n                           # positions cap .. cap + n - 1: all behind the table
+            p.cu_q[3] = p.tokens
+            p.kv[2] = 0
+            launch.paged_kv_append(p.cache, p.batch, api.from_torch(p.k), api.from_torch(p.v))
+            assert all(torch.equal(a, b) for a, b in zip(before, p.pools))
+    assert _status(b200)[0] == 0
+
+
+def test_no_more_than_max_q_len_tokens(b200):
+    p = ref.Problem([5, 2], [50, 60], 4, 2, 64, 16, BF16, seed=48, max_q=3)
+    got = _attend(p, 0.2)
+    want, tol = ref.attention(p, 0.2)
+    rows = [0, 1, 2, 5, 6]
+    assert ((got[rows].double() - want[rows]).abs() <= tol[rows]).all()
+    assert (got[3:5] == SENTINEL).all()
+
+
+def test_pools_beyond_four_gigabytes(b200):
+    """Pages whose offsets pass 2^32 bytes and 2^31 elements, in both formats and both kernels, and append and gather on
+    them."""
+    g = torch.Generator(device="cuda").manual_seed(49)
+    for fmt in ("16bit", "nvfp4"):
+        d, kvh, page = 128, 8, 64
+        row = d if fmt == "16bit" else d // 2
+        per = kvh * page * row
+        pages = (1 << 31) // per + 40 if fmt == "16bit" else (1 << 32) // per + 40
+        dt = BF16 if fmt == "16bit" else torch.uint8
+        pools = [torch.empty(pages, kvh, page, row, dtype=dt, device="cuda") for _ in range(2)]
+        scales = [torch.empty(pages, kvh, page, d // 16, dtype=torch.uint8, device="cuda") for _ in range(2)] if fmt != "16bit" \
+            else [None, None]
+        p = ref.Problem([1, 100], [300, 200], 16, kvh, d, page, BF16, fmt, seed=50)
+        used = torch.arange(pages - 9, pages, device="cuda")
+        for big, small, bs, ss in zip(pools, p.pools, scales, p.scales):
+            big[used] = small[:9]
+            if ss is not None:
+                bs[used] = ss[:9]
+        p.table[0, :5], p.table[1, :4] = used[:5].int(), used[5:].int()
+        p.pools, p.scales, p.pages = pools, scales, pages
+        p.cache = paged.PagedKvCache(*pools, *scales)
+        launch.paged_kv_append(p.cache, p.batch, api.from_torch(p.k), api.from_torch(p.v))
+        out = [torch.empty_like(p.k) for _ in range(2)]
+        launch.paged_kv_gather(api.from_torch(out[0]), api.from_torch(out[1]), p.cache, p.batch)
+        for b, n in enumerate(p.q_lens):
+            for got, want in zip(out, p.rows(b, p.kv_lens[b])):
+                assert torch.equal(got[p.cu[b]:p.cu[b + 1]].double(), want[-n:])
+        if fmt == "16bit":
+            assert torch.equal(out[0], p.k)
+        got = _attend(p, 0.1)
+        want, tol = ref.attention(p, 0.1)
+        assert ((got.double() - want).abs() <= tol).all()
+        del pools, scales, p, out
+        torch.cuda.empty_cache()
+
+
 # ---- append ------------------------------------------------------------------------------------------------------
 def _inv_freq(r, base=500000.0):
     i = torch.arange(0, r, 2, dtype=torch.float64, device="cuda")
