@@ -1044,8 +1044,9 @@ int launch_tile(const PagedAttnArgs& a, const PagedTilePlan& plan) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = a.row_limit > 0 ? 1 : 0;          // beside the row-block kernel, or alone behind whatever came before
   B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tmQ, tmK, tmV, p, di->status));
+  cfg.numAttrs = 1;
   cfg.gridDim = dim3(plan.ctas, 16);
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 0;

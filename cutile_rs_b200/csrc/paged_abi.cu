@@ -234,8 +234,13 @@ int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cach
   const bool tiles = may_tile(batch->max_q_len, group) && !misaligned(q, 16) && !misaligned(out, 16) && !(a.q_ts % 8) &&
                      !(a.q_hs % 8) && !(a.o_ts % 8) && !(a.o_hs % 8) && a.q_ts > 0 && a.q_hs > 0;
   a.tile_off = tiles ? split_bytes(cache, batch, kTileRows) : 0;
-  a.row_limit = tiles ? kTileRows : 0x7fffffff;
-  if (int rc = b200_paged_split_dispatch(a)) return rc;
+  // Mostly prompts: one launch of the tile kernel takes every sequence.  Mostly decode steps with some prompts among
+  // them: each kernel takes its own.  A decode step costs the tile kernel a whole tile per 128 keys (it reads the cache at
+  // 70 % of the rate the row blocks reach); the second kernel costs its launches, @@ us.
+  const bool only_tiles = tiles && (long long)tokens * group >= (long long)batch->batch * kTileRows;
+  a.row_limit = only_tiles ? 0 : tiles ? kTileRows : 0x7fffffff;
+  if (!only_tiles)
+    if (int rc = b200_paged_split_dispatch(a)) return rc;
   return tiles ? b200_paged_tile_dispatch(a) : B200TILE_OK;
 }
 

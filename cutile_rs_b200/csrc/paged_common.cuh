@@ -130,5 +130,6 @@ struct PagedTilePlan {
   size_t desc_off, bytes;
 };
 PagedTilePlan b200_paged_tile_plan(int head_dim);
-// Launched right behind the row-block kernel, whose rows it leaves alone, and runs beside it.
+// Takes the sequences with more than row_limit rows; with row_limit > 0 launched right behind the row-block kernel, whose
+// rows it leaves alone, and beside it.
 int b200_paged_tile_dispatch(const PagedAttnArgs& a);
