@@ -375,7 +375,13 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
     if (per < p.min_steps) per = p.min_steps;
     u = (long long)wid * per;
     u_end = min(total, u + per);
-    if (!p.by_item && lane == 0) p.desc[wid] = make_int4(0, 0, 0, 0);
+    if (!p.by_item) {
+      if (lane == 0) p.desc[wid] = make_int4(0, 0, 0, 0);
+    } else {
+      // items that do not exist in this launch: nobody else writes their descriptors
+      for (int i = blockIdx.x * THREADS + threadIdx.x; i < p.batch.batch * p.rb_max * p.kv_heads; i += gridDim.x * THREADS)
+        if (i / p.kv_heads % p.rb_max >= seq_work<RB>(p, i / (p.rb_max * p.kv_heads)).rbs) p.desc[i] = make_int4(0, 0, 0, 0);
+    }
     if (u >= u_end) return;
 
     // the sequence that holds step u: binary search over the chunks, then along the chunk
@@ -886,20 +892,13 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
 // are stored the way the worker held them (one float4 per lane and 16 x 8 tile), so a warp adds one tile with
 // full-width loads; PW warps share the parts of a tile and are added through shared memory in a fixed order.
 template <int D, bool F16, int NT, bool FP4, int PW>
-__global__ void __launch_bounds__(256) fmha_paged_merge_kernel(const __grid_constant__ SplitParams p) {
+__global__ void __launch_bounds__(256, NT == 1 ? 4 : 2) fmha_paged_merge_kernel(const __grid_constant__ SplitParams p) {
   constexpr int DT = D / 16, RB = 8 * NT, CT = 8 / PW;
   __shared__ float4 s_o[8][NT][32];
   __shared__ float s_ml[8][NT][2][4][2];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the tile kernel of the same call, if there is one
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  bool exists = true;
-  if (p.by_item) {
-    // items that do not exist in this launch have no descriptor (lengths are the call's inputs: known before the wait)
-    const int b = blockIdx.x / (p.rb_max * p.kv_heads), rb = (blockIdx.x / p.kv_heads) % p.rb_max;
-    exists = rb < seq_work<RB>(p, b).rbs;
-  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!exists) return;
   int4 d = p.desc[blockIdx.x];
   // whatever a workspace holds that other work has written to meanwhile, nothing outside of it is touched
   if (d.x <= 0 || (unsigned)d.y >= (unsigned)p.workers || (unsigned)d.z >= (unsigned)p.batch.batch || d.w < 0 ||
@@ -929,7 +928,7 @@ __global__ void __launch_bounds__(256) fmha_paged_merge_kernel(const __grid_cons
     }
   };
   if (c < DT) {
-    constexpr int U = NT == 1 ? 8 : 4;               // parts whose loads are in flight together
+    constexpr int U = 4;                             // parts whose loads are in flight together
     for (int i0 = pw; i0 < d.x; i0 += U * PW) {
       float4 v[U][NT];
       float2 pm[U][NT], pl[U][NT];
@@ -1051,16 +1050,18 @@ int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
   }
   B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, tmK, tmV, p, di->status));
   if (plan.coop) return B200_OK;
-  // few items with many parts: all eight warps of a CTA share the parts of one tile; else a warp per tile
+  // PW warps of a CTA share the parts of one tile, as many as an item has parts on average to keep them all in flight
   const unsigned x = (unsigned)(plan.by_item ? plan.items : plan.workers);
-  const bool wide = x * (D / 16) <= 8u * di->sm_count;
-  cfg.gridDim = dim3(x, wide ? D / 16 : 1);
+  const unsigned parts = plan.workers / x;
+  const int pw = x * (D / 16) <= 8u * di->sm_count ? 8 : parts > 4 ? 2 : 1;
+  cfg.gridDim = dim3(x, (D / 16 * pw + 7) / 8);
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 1;
-  if (wide) B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fmha_paged_merge_kernel<D, F16, NT, FP4, 8>, p));
+  if (pw == 8) B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fmha_paged_merge_kernel<D, F16, NT, FP4, 8>, p));
+  else if (pw == 2) B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fmha_paged_merge_kernel<D, F16, NT, FP4, 2>, p));
   else B200_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fmha_paged_merge_kernel<D, F16, NT, FP4, 1>, p));
   return B200_OK;
 }
