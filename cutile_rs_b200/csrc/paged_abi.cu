@@ -17,8 +17,22 @@ int b200_paged_gather_dispatch(int dtype, const b200tile_paged_cache& c, const b
 
 namespace {
 
-// Sequences with more query rows (tokens * group) per K/V head than this go to the tile kernel.
-constexpr int kTileRows = 64;
+// Which kernel takes a sequence of `rows` query rows (tokens * group) per K/V head.  The row-block kernel reads the cache
+// once per 16 rows, the tile kernel once per 256 but with more to start and end; it pays once the call is large enough.
+// Measured (us, row blocks against tiles, 8 K/V heads of 128):
+//   16-bit, 20 rows:  8 x 1024 keys 17 / 27, 8 x 2048 keys 38 / 32, 32 x 8192 keys 354 / 211
+//   16-bit, 64 rows:  1 x 2048 keys 16 / 25, 8 x 1024 keys 30 / 28, 32 x 2048 keys 191 / 71
+//   NVFP4,  36 rows:  8 x 1024 keys 34 / 38, 32 x 8192 keys 312 / 304;  20 rows: 32 x 8192 keys 217 / 303
+//   NVFP4,  64 rows:  8 x 512 keys 32 / 36, 8 x 2048 keys 49 / 42, 32 x 8192 keys 410 / 305
+int tile_rows(const b200tile_paged_cache* c) { return c->format ? 48 : 16; }
+bool may_tile(const b200tile_paged_cache* c, const b200tile_paged_batch* b, int group) {
+  const long long rows = (long long)b->max_q_len * group;
+  if (group > 128 || rows <= tile_rows(c)) return false;
+  // steps of 16 keys that the row blocks of the largest such call would take
+  const long long keys = (long long)b->max_pages * c->page_size;
+  const double steps = (double)b->batch * c->kv_heads * (double)((rows + 15) / 16) * (double)((keys + 15) / 16);
+  return steps >= (c->format ? 16384.0 : 12288.0);
+}
 
 bool misaligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
 
@@ -88,8 +102,6 @@ int check_batch(const char* who, const b200tile_paged_cache* c, const b200tile_p
     return set_error(B200TILE_ERR_UNSUPPORTED, "%s: %d pages of %d exceed 2^31 positions", who, b->max_pages, c->page_size);
   return B200TILE_OK;
 }
-
-bool may_tile(long long max_q, int group) { return max_q * group > kTileRows && group <= 128; }
 
 // Workspace of the row-block kernel for sequences of up to `rows` query rows, a multiple of 256 bytes.
 size_t split_bytes(const b200tile_paged_cache* c, const b200tile_paged_batch* b, long long rows) {
@@ -178,9 +190,9 @@ uint64_t b200tile_paged_attention_workspace_bytes(const b200tile_paged_cache* ca
     return 0;
   const int group = q_heads / cache->kv_heads;
   const size_t all = split_bytes(cache, batch, (long long)batch->max_q_len * group);
-  if (!may_tile(batch->max_q_len, group)) return all;
+  if (!may_tile(cache, batch, group)) return all;
   // the tile kernel's part lies behind the row-block kernel's; without it (rows it cannot move) the latter takes all rows
-  return std::max(all, split_bytes(cache, batch, kTileRows) + b200_paged_tile_plan(cache->head_dim).bytes);
+  return std::max(all, split_bytes(cache, batch, tile_rows(cache)) + b200_paged_tile_plan(cache->head_dim).bytes);
 }
 
 int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cache, const b200tile_paged_batch* batch,
@@ -231,14 +243,18 @@ int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cach
   a.workspace = workspace;
   a.stream = static_cast<cudaStream_t>(cu_stream);
   // the tile kernel moves rows by TMA and in 16-byte pieces; rows that do not lie so take row blocks, whatever their number
-  const bool tiles = may_tile(batch->max_q_len, group) && !misaligned(q, 16) && !misaligned(out, 16) && !(a.q_ts % 8) &&
+  const bool tiles = may_tile(cache, batch, group) && !misaligned(q, 16) && !misaligned(out, 16) && !(a.q_ts % 8) &&
                      !(a.q_hs % 8) && !(a.o_ts % 8) && !(a.o_hs % 8) && a.q_ts > 0 && a.q_hs > 0;
-  a.tile_off = tiles ? split_bytes(cache, batch, kTileRows) : 0;
-  // Mostly prompts: one launch of the tile kernel takes every sequence.  Mostly decode steps with some prompts among
-  // them: each kernel takes its own.  A decode step costs the tile kernel a whole tile per 128 keys (it reads the cache at
-  // 70 % of the rate the row blocks reach); the second kernel costs its launches, @@ us.
-  const bool only_tiles = tiles && (long long)tokens * group >= (long long)batch->batch * kTileRows;
-  a.row_limit = only_tiles ? 0 : tiles ? kTileRows : 0x7fffffff;
+  a.tile_off = tiles ? split_bytes(cache, batch, tile_rows(cache)) : 0;
+  // Prompts alone take one launch of the tile kernel; decode steps with prompts among them take both kernels, each its
+  // own sequences.  The second kernel costs 5 to 20 us (launches, merge, its CTAs in front of the tiles'); a decode step in
+  // the tile kernel costs a whole tile per 128 keys.  Beside a prompt of 512 tokens, one kernel against two: 31 steps of 256
+  // keys 39 / 44 us, 255 of them 159 / 101, over NVFP4 56 / 62 and 219 / 110; 100 steps of 4096 keys over NVFP4 491 / 217.  How
+  // many decode steps there may be follows from the sizes: as many sequences as are left when the others have max_q_len
+  // tokens each.
+  const long long full = (tokens + (long long)batch->max_q_len - 1) / batch->max_q_len;
+  const bool only_tiles = tiles && (batch->batch - full) * cache->kv_heads <= (cache->format ? 64 : 256);
+  a.row_limit = only_tiles ? 0 : tiles ? tile_rows(cache) : 0x7fffffff;
   if (!only_tiles)
     if (int rc = b200_paged_split_dispatch(a)) return rc;
   return tiles ? b200_paged_tile_dispatch(a) : B200TILE_OK;

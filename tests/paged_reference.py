@@ -3,6 +3,7 @@ import math
 
 import torch
 
+MANY_KEYS = 1 << 17
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
@@ -21,17 +22,19 @@ def dequant(codes, scales, glob=1.0):
 
 
 class Problem:
-    """Pools filled with random rows, a shuffled block table with junk behind every sequence's pages, ragged lengths."""
+    """Pools filled with random rows, a shuffled block table with junk behind every sequence's pages, ragged lengths.
+    `table_keys` makes the block table that long at least: the choice of kernels goes by what a table could hold, so that
+    MANY_KEYS has small problems of more than a few rows take the kernel of the large ones."""
 
     def __init__(self, q_lens, kv_lens, heads, kv_heads, d, page=16, dtype=torch.bfloat16, fmt="16bit", layout="hnd",
-                 seed=0, extra_pages=3, k_global=1.0, v_global=1.0, pad_tokens=0, junk=-7, max_q=None):
+                 seed=0, extra_pages=3, k_global=1.0, v_global=1.0, pad_tokens=0, junk=-7, max_q=None, table_keys=0):
         g = torch.Generator(device="cuda").manual_seed(seed)
         self.q_lens, self.kv_lens, self.heads, self.kvh, self.d, self.page = q_lens, kv_lens, heads, kv_heads, d, page
         self.dtype, self.fmt, self.kg, self.vg = dtype, fmt, k_global, v_global
         need = [-(-max(n, 0) // page) for n in kv_lens]
         self.pages = sum(need) + extra_pages
         order = torch.randperm(self.pages, generator=g, device="cuda").int()
-        self.table = torch.full((len(q_lens), max(max(need), 1) + 2), junk, dtype=torch.int32, device="cuda")
+        self.table = torch.full((len(q_lens), max(max(need) + 2, 3, table_keys // page)), junk, dtype=torch.int32, device="cuda")
         at = 0
         for b, n in enumerate(need):
             self.table[b, :n] = order[at:at + n]
@@ -102,7 +105,7 @@ def attention(p, scale, causal=True, window=0, softcap=0.0):
     Per row: the output's own rounding, half a step of its type; probabilities whose exponents are off by the scores'
     error (a 32-bit dot product of d terms, the score's scale and the exponential's argument: (d + 8) 2^-24 of
     sum |q k| scale, with a cap 2^-19 of it more) and which are handed over in two 16-bit pieces (2^-15 of p; one f16 piece, 2^-11,
-    for bf16 over NVFP4; one piece of the type, half a step, in calls with sequences of more than 64 rows), all against sum p |v|; sums of n
+    for bf16 over NVFP4; one piece of the type, half a step, in calls with sequences of more than 16 rows, 48 over NVFP4), all against sum p |v|; sums of n
     terms in 32 bits.  Pieces in f16 (f16 rows, and all rows over NVFP4) have no relative step below 2^-14: they are off by
     up to half of f16's smallest step, 2^-25, each, while the largest p is at least 1 and so is the sum they are divided by:
     2^-25 sum |v| over the keys seen."""
@@ -115,7 +118,7 @@ def attention(p, scale, causal=True, window=0, softcap=0.0):
     for b, (n, kv) in enumerate(zip(p.q_lens, p.kv_lens)):
         if n == 0 or kv <= 0:
             continue
-        piece = few if max(p.q_lens) * group <= 64 else eps / 2
+        piece = few if max(p.q_lens) * group <= (16 if p.fmt == "16bit" else 48) else eps / 2
         k, v = p.rows(b, kv)
         pos = torch.arange(kv - n, kv, device="cuda")[:, None]
         key = torch.arange(kv, device="cuda")[None, :]

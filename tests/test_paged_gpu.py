@@ -59,38 +59,41 @@ def test_decode_lengths(b200, fmt, layout, d, heads, kvh, page, dtype):
     assert _status(b200)[0] == 0
 
 
+@pytest.mark.parametrize("keys", [0, ref.MANY_KEYS])
 @pytest.mark.parametrize("fmt", ["16bit", "nvfp4"])
 @pytest.mark.parametrize("causal,window,softcap", [(True, 0, 30.0), (True, 1, 0.0), (True, 33, 0.0), (True, 100, 5.0),
                                                    (False, 0, 0.0), (False, 0, 20.0)])
-def test_masks_and_cap(b200, fmt, causal, window, softcap):
+def test_masks_and_cap(b200, fmt, causal, window, softcap, keys):
     """Several tokens per sequence: causal edges inside a block of rows, windows, caps; a sequence shorter than its
     tokens, whose first rows see nothing."""
-    p = ref.Problem([3, 5, 1, 4, 2], [3, 260, 77, 2, 130], 6, 2, 64, 16, F16, fmt, seed=window + 1)
+    p = ref.Problem([3, 5, 1, 4, 2], [3, 260, 77, 2, 130], 6, 2, 64, 16, F16, fmt, seed=window + 1, table_keys=keys)
     got = _check(p, 0.3, causal=causal, window=window, softcap=softcap)
     if causal:
         assert (got[p.cu[3]:p.cu[3] + 2] == 0).all()   # positions -2 and -1
 
 
+@pytest.mark.parametrize("keys", [0, ref.MANY_KEYS])
 @pytest.mark.parametrize("fmt,d,dtype", [("16bit", 128, BF16), ("16bit", 64, F16), ("nvfp4", 128, F16), ("nvfp4", 64, BF16)])
 @pytest.mark.parametrize("heads,kvh,page,window,softcap", [(8, 2, 16, 0, 0.0), (6, 2, 128, 150, 25.0), (7, 1, 32, 0, 50.0),
                                                            (2, 2, 64, 40, 0.0)])
-def test_prompt_chunks(b200, fmt, d, dtype, heads, kvh, page, window, softcap):
+def test_prompt_chunks(b200, fmt, d, dtype, heads, kvh, page, window, softcap, keys):
     """Prompts and chunks behind cached prefixes in one call with decode steps."""
     p = ref.Problem([150, 1, 300, 64, 0, 17], [150, 200, 555, 70, 40, 400], heads, kvh, d, page, dtype, fmt,
-                    seed=heads + page, pad_tokens=5)
+                    seed=heads + page, pad_tokens=5, table_keys=keys)
     _check(p, d ** -0.5, window=window, softcap=softcap)
     assert _status(b200)[0] == 0
 
 
+@pytest.mark.parametrize("keys", [0, ref.MANY_KEYS])
 @pytest.mark.parametrize("fmt,d,dtype", [("16bit", 128, F16), ("16bit", 64, BF16), ("nvfp4", 128, BF16), ("nvfp4", 64, F16)])
 @pytest.mark.parametrize("heads,kvh,page,causal,window,softcap", [(8, 1, 64, True, 0, 0.0), (4, 4, 256, True, 700, 0.0),
                                                                   (10, 2, 16, True, 130, 30.0), (4, 1, 32, False, 0, 0.0),
                                                                   (4, 2, 128, False, 0, 40.0)])
-def test_long_prompts(b200, fmt, d, dtype, heads, kvh, page, causal, window, softcap):
+def test_long_prompts(b200, fmt, d, dtype, heads, kvh, page, causal, window, softcap, keys):
     """Several tiles per sequence, ends inside tiles, pages and steps, whole steps before the window, a first step in
     which early rows see nothing yet; a sequence shorter than its tokens."""
     p = ref.Problem([1000, 129, 257, 90], [1500, 129, 2999, 33], heads, kvh, d, page, dtype, fmt, "nhd" if page == 64 else "hnd",
-                    seed=heads + page)
+                    seed=heads + page, table_keys=keys)
     got = _check(p, d ** -0.5, causal=causal, window=window, softcap=softcap)
     if causal:
         assert (got[p.cu[3]:p.cu[3] + 57] == 0).all()
@@ -101,7 +104,7 @@ def test_long_prompts_with_very_negative_scores(b200):
     """Windows whose first step is empty for late rows, with scores far below zero: the reference of the running
     exponent must come from keys that are seen."""
     for fmt in ("16bit", "nvfp4"):
-        p = ref.Problem([400], [900], 2, 1, 128, 16, BF16, fmt, seed=30)
+        p = ref.Problem([400], [900], 2, 1, 128, 16, BF16, fmt, seed=30, table_keys=ref.MANY_KEYS)
         p.q.copy_(p.q.abs())
         if fmt == "16bit":
             p.pools[0].copy_(-p.pools[0].abs())
@@ -126,6 +129,24 @@ def test_many_sequences(b200):
     _check(p, 0.125)
     p = ref.Problem([(i * 7) % 3 for i in range(700)], kv, 2, 1, 64, 16, F16, "nvfp4", seed=10)
     _check(p, 0.125)
+
+
+@pytest.mark.parametrize("fmt,d", [("16bit", 128), ("16bit", 64), ("nvfp4", 128), ("nvfp4", 64)])
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (70, 20.0)])
+def test_many_steps_and_a_prompt(b200, fmt, d, window, softcap):
+    """So many decode steps beside the prompts that each kernel takes its own sequences; call after call, which run into
+    one another, with one workspace."""
+    q_lens = [1] * 150 + [130, 0, 40, 3]
+    kv_lens = [1 + (53 * i) % 400 for i in range(150)] + [300, 20, 40, 500]
+    p = ref.Problem(q_lens, kv_lens, 8, 2, d, 16, BF16, fmt, seed=d, table_keys=ref.MANY_KEYS, pad_tokens=3)
+    got = _check(p, d ** -0.5, window=window, softcap=softcap)
+    ws = launch.paged_attention_workspace(p.cache, p.batch, 8)
+    outs = [torch.full_like(p.q, SENTINEL) for _ in range(10)]
+    for o in outs:
+        launch.paged_attention(api.from_torch(o), api.from_torch(p.q), p.cache, p.batch, d ** -0.5, window=window,
+                               softcap=softcap, workspace=ws)
+    assert all(torch.equal(got, o) for o in outs)
+    assert _status(b200)[0] == 0
 
 
 def test_large_scores_and_infinities(b200):
@@ -160,7 +181,7 @@ def test_global_factors_and_wide_scales(b200):
 def test_strided_rows(b200):
     """q inside a fused projection's rows, out inside a wider buffer, heads in reverse memory order of tokens."""
     for q_lens, kv_lens in (([1, 1, 2], [30, 200, 64]), ([130, 1, 40], [130, 50, 90])):
-        p = ref.Problem(q_lens, kv_lens, 4, 2, 128, 16, BF16, seed=8)
+        p = ref.Problem(q_lens, kv_lens, 4, 2, 128, 16, BF16, seed=8, table_keys=ref.MANY_KEYS)
         p.poison()
         wide = torch.zeros(p.tokens, 8, 130, dtype=BF16, device="cuda")
         qv = wide[:, 2:6, :128]
@@ -173,12 +194,13 @@ def test_strided_rows(b200):
         assert (ow[:, :, 128:] == SENTINEL).all()
 
 
+@pytest.mark.parametrize("keys", [0, ref.MANY_KEYS])
 @pytest.mark.parametrize("fmt,d,dtype", [("16bit", 128, BF16), ("16bit", 64, F16), ("nvfp4", 128, BF16), ("nvfp4", 64, F16)])
-def test_caps_near_and_far_from_the_scores(b200, fmt, d, dtype):
+def test_caps_near_and_far_from_the_scores(b200, fmt, d, dtype, keys):
     """Scores that are a small part of the cap, about its size, and far beyond it, in one call: the capped score has one
     form for small arguments and one for all."""
     for cap in (1.0, 4.0, 300.0):
-        p = ref.Problem([200, 3, 90], [260, 40, 90], 6, 2, d, 16, dtype, fmt, seed=40)
+        p = ref.Problem([200, 3, 90], [260, 40, 90], 6, 2, d, 16, dtype, fmt, seed=40, table_keys=keys)
         p.q[:70].mul_(6)
         _check(p, d ** -0.5, softcap=cap)
         _check(p, d ** -0.5, softcap=cap, window=50)
@@ -187,7 +209,7 @@ def test_caps_near_and_far_from_the_scores(b200, fmt, d, dtype):
 @pytest.mark.parametrize("unit", [2.0 ** -30, 2.0 ** 13])
 def test_prompts_of_small_and_large_queries_over_fp4(b200, unit):
     for softcap in (0.0, 20.0):
-        p = ref.Problem([150, 20], [300, 33], 4, 2, 128, 16, BF16, "nvfp4", seed=41)
+        p = ref.Problem([150, 20], [300, 33], 4, 2, 128, 16, BF16, "nvfp4", seed=41, table_keys=ref.MANY_KEYS)
         p.q[::3].mul_(2.0 ** -9)                        # rows of very different size in one tile
         p.q.mul_(unit)
         _check(p, 128 ** -0.5 / unit, softcap=softcap)
@@ -197,7 +219,7 @@ def test_many_heads_per_kv_head(b200):
     """More heads per K/V head than a tile has rows: row blocks take the prompt."""
     p = ref.Problem([3, 2], [40, 90], 260, 2, 64, 16, BF16, seed=42)
     _check(p, 0.125)
-    p = ref.Problem([9, 1], [40, 90], 128, 1, 64, 16, F16, "nvfp4", seed=42)
+    p = ref.Problem([9, 1], [40, 90], 128, 1, 64, 16, F16, "nvfp4", seed=42, table_keys=ref.MANY_KEYS)
     _check(p, 0.125)
 
 
@@ -218,7 +240,7 @@ def test_decode_runs_and_clusters_agree(b200):
 def test_workspace_contents_do_not_matter(b200):
     for q_lens, kv_lens in (([1, 1], [30000, 17000]), ([100, 1], [5000, 600])):
         for fmt in ("16bit", "nvfp4"):
-            p = ref.Problem(q_lens, kv_lens, 4, 2, 64, 64, BF16, fmt, seed=44)
+            p = ref.Problem(q_lens, kv_lens, 4, 2, 64, 64, BF16, fmt, seed=44, table_keys=ref.MANY_KEYS)
             ws = launch.paged_attention_workspace(p.cache, p.batch, 4)
             a = _attend(p, 0.1, workspace=ws)
             ws.fill_(255)                               # NaN everywhere, -1 in every descriptor
@@ -229,7 +251,7 @@ def test_workspace_contents_do_not_matter(b200):
 
 def test_output_may_be_the_query_tensor(b200):
     for q_lens in ([1, 1, 2], [130, 1, 70]):
-        p = ref.Problem(q_lens, [700, 40, 300], 4, 2, 128, 16, BF16, seed=45)
+        p = ref.Problem(q_lens, [700, 40, 300], 4, 2, 128, 16, BF16, seed=45, table_keys=ref.MANY_KEYS)
         want = _attend(p, 0.1)
         t = api.from_torch(p.q.clone())
         launch.paged_attention(t, t, p.cache, p.batch, 0.1)
@@ -239,7 +261,7 @@ def test_output_may_be_the_query_tensor(b200):
 def test_sequences_that_share_pages(b200):
     """A common prefix in common pages, read by all."""
     for fmt in ("16bit", "nvfp4"):
-        p = ref.Problem([1, 1, 80], [200, 220, 240], 4, 2, 64, 16, F16, fmt, seed=46)
+        p = ref.Problem([1, 1, 80], [200, 220, 240], 4, 2, 64, 16, F16, fmt, seed=46, table_keys=ref.MANY_KEYS)
         p.table[1:, :9] = p.table[0, :9]
         got = _attend(p, 0.2)
         want, tol = ref.attention(p, 0.2)
@@ -251,7 +273,8 @@ def test_lengths_and_ranges_that_do_not_fit(b200):
     is touched."""
     for fmt in ("16bit", "nvfp4"):
         for q_lens in ([1, 1, 1], [100, 1, 90]):
-            p = ref.Problem(q_lens, [150, 60, 120], 4, 2, 64, 16, BF16, fmt, seed=47)
+            p = ref.Problem(q_lens, [150, 60, 120], 4, 2, 64, 16, BF16, fmt, seed=47,
+                            table_keys=4096 if q_lens[0] > 1 else 0)   # the tile kernel / row blocks
             cap = p.table.shape[1] * 16
             p.table.clamp_(min=0)                       # every entry a page: positions up to the table's end exist
             p.kv[0] = cap + 37                          # keys behind the table are left out, positions keep counting
@@ -298,7 +321,7 @@ def test_pools_beyond_four_gigabytes(b200):
         pools = [torch.empty(pages, kvh, page, row, dtype=dt, device="cuda") for _ in range(2)]
         scales = [torch.empty(pages, kvh, page, d // 16, dtype=torch.uint8, device="cuda") for _ in range(2)] if fmt != "16bit" \
             else [None, None]
-        p = ref.Problem([1, 100], [300, 200], 16, kvh, d, page, BF16, fmt, seed=50)
+        p = ref.Problem([1, 100], [300, 200], 16, kvh, d, page, BF16, fmt, seed=50, table_keys=ref.MANY_KEYS)
         used = torch.arange(pages - 9, pages, device="cuda")
         for big, small, bs, ss in zip(pools, p.pools, scales, p.scales):
             big[used] = small[:9]
@@ -315,9 +338,10 @@ def test_pools_beyond_four_gigabytes(b200):
                 assert torch.equal(got[p.cu[b]:p.cu[b + 1]].double(), want[-n:])
         if fmt == "16bit":
             assert torch.equal(out[0], p.k)
-        got = _attend(p, 0.1)
         want, tol = ref.attention(p, 0.1)
-        assert ((got.double() - want).abs() <= tol).all()
+        for width in (p.table.shape[1], 6):              # tiles, row blocks
+            p.batch = paged.PagedBatch(p.table[:, :width], p.cu_q, p.kv, 100)
+            assert ((_attend(p, 0.1).double() - want).abs() <= tol).all()
         del pools, scales, p, out
         torch.cuda.empty_cache()
 
