@@ -124,7 +124,7 @@ __device__ __forceinline__ SeqWork seq_work(const SplitParams& p, int b) {
   int lo = 0, hi = w.s.len;
   if (p.causal) {
     hi = min(hi, w.s.pos0 + w.s.n);
-    if (p.window > 0) lo = max(0, w.s.pos0 - p.window + 1);
+    if (p.window > 0) lo = window_start(w.s.pos0, p.window);
   }
   w.base = hi > lo ? lo / STEP : 0;
   w.steps = hi > lo ? (hi + STEP - 1) / STEP - w.base : 1;
@@ -148,7 +148,7 @@ __device__ __forceinline__ RowMask<NT> row_mask(const SplitParams& p, const SeqV
     if (p.causal) {
       const int pos = s.pos0 + row / p.group;
       hi = min(hi, pos + 1);
-      if (p.window > 0) lo = max(0, pos - p.window + 1);
+      if (p.window > 0) lo = window_start(pos, p.window);
     }
   };
   int l0, h0, l1, h1;
@@ -1011,9 +1011,9 @@ int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
   p.min_steps = 2;
   CUtensorMap tmK = {}, tmV = {};
   if constexpr (FP4) {
-    p.score.scale_log2 *= c.k_global ;
-    p.score.cap_arg *= c.k_global ;
-    p.out_scale = c.v_global ;
+    p.score.scale_log2 *= c.k_global;
+    p.score.cap_arg *= c.k_global;
+    p.out_scale = c.v_global;
     p.k = static_cast<const uint8_t*>(c.k);
     p.v = static_cast<const uint8_t*>(c.v);
     p.ks = static_cast<const uint8_t*>(c.k_scales);

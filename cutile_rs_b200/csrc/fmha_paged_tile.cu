@@ -116,7 +116,7 @@ __device__ __forceinline__ PairSpan pair_span(const TileParams& p, const SeqView
   PairSpan x;
   const int t0 = pair * 2 * p.tpt, n = min(s.n - t0, 2 * p.tpt);
   x.hi = p.causal ? min(s.len, s.pos0 + t0 + n) : s.len;
-  x.lo = p.causal && p.window > 0 ? max(0, s.pos0 + t0 - p.window + 1) : 0;
+  x.lo = p.causal && p.window > 0 ? window_start(s.pos0 + t0, p.window) : 0;
   x.j0 = x.hi > x.lo ? x.lo / FA_BN : 0;
   x.steps = x.hi > x.lo ? (x.hi + FA_BN - 1) / FA_BN - x.j0 : 1;
   return x;
@@ -136,7 +136,7 @@ __device__ __forceinline__ SeqLine seq_line(const TileParams& p, const SeqView& 
   x.pairs = seq_pairs(p, s);
   const int tokens = 2 * p.tpt;
   x.slope = p.causal ? tokens : 0;
-  x.base = p.causal ? max(0, s.pos0) + tokens : s.len;
+  x.base = p.causal ? (long long)max(0, s.pos0) + tokens : s.len;
   x.top = p.causal && p.window > 0 ? (long long)p.window + tokens : (1ll << 40);
   x.bend = x.top <= x.base ? 0 : x.slope == 0 ? x.pairs : (int)min((long long)x.pairs, (x.top - x.base) / x.slope + 1);
   return x;
@@ -289,7 +289,6 @@ __device__ __forceinline__ void expand8(uint32_t w, uint32_t scale, uint32_t (&o
 #pragma unroll
   for (int i = 0; i < 4; ++i) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(o[i]) : "r"(o[i]), "r"(scale));
 }
-
 
 template <int D, bool F16, bool CAP, bool FP4>
 __global__ void __launch_bounds__(FP4 ? 512 : 384, 1)
@@ -619,7 +618,7 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       if (tok < w.tokens[t]) {
         const int pos = w.pos0 + t * p.tpt + tok;
         row_hi = p.causal ? min(w.len, pos + 1) : w.len;
-        if (p.causal && p.window > 0) row_lo = max(0, pos - p.window + 1);
+        if (p.causal && p.window > 0) row_lo = window_start(pos, p.window);
       }
       const bool blind = row_hi <= row_lo;
       float poly_max = 0.0f;

@@ -134,6 +134,15 @@ int check_rows(const char* who, const char* name, const void* p, const int64_t* 
   return B200TILE_OK;
 }
 
+// the same for rows that are written: each must have a place of its own
+int check_out_rows(const char* who, const char* name, const void* p, const int64_t* st, int tokens, int heads, int unit,
+                   uintptr_t align) {
+  if (int rc = check_rows(who, name, p, st, tokens, unit, align)) return rc;
+  if ((tokens > 1 && st[0] == 0) || (heads > 1 && st[1] == 0))
+    return set_error(B200TILE_ERR_INVALID, "%s: the rows of %s must not share memory (a stride is 0)", who, name);
+  return B200TILE_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -158,7 +167,7 @@ int b200tile_paged_kv_append(const char* dtype, const b200tile_paged_cache* cach
   if (q) {
     if (q_heads <= 0) return set_error(B200TILE_ERR_INVALID, "%s: q_heads must be positive", who);
     if (int rc = check_rows(who, "q", q, q_strides, tokens, 8, 16)) return rc;
-    if (int rc = check_rows(who, "q_out", q_out, q_out_strides, tokens, 8, 16)) return rc;
+    if (int rc = check_out_rows(who, "q_out", q_out, q_out_strides, tokens, q_heads, 8, 16)) return rc;
   }
   if (int rc = check_rows(who, "k", k, k_strides, tokens, 8, 16)) return rc;
   if (int rc = check_rows(who, "v", v, v_strides, tokens, 8, 16)) return rc;
@@ -176,8 +185,8 @@ int b200tile_paged_kv_gather(const char* dtype, const b200tile_paged_cache* cach
   if (int rc = check_dtype(dtype, who, &dt)) return rc;
   if (int rc = check_cache(who, cache)) return rc;
   if (int rc = check_batch(who, cache, batch, tokens)) return rc;
-  if (int rc = check_rows(who, "k_out", k_out, k_out_strides, tokens, 8, 16)) return rc;
-  if (int rc = check_rows(who, "v_out", v_out, v_out_strides, tokens, 8, 16)) return rc;
+  if (int rc = check_out_rows(who, "k_out", k_out, k_out_strides, tokens, cache->kv_heads, 8, 16)) return rc;
+  if (int rc = check_out_rows(who, "v_out", v_out, v_out_strides, tokens, cache->kv_heads, 8, 16)) return rc;
   if (tokens == 0 || batch->batch == 0) return B200TILE_OK;
   return b200_paged_gather_dispatch(dt, *cache, device_batch(cache, batch, tokens), k_out, v_out, k_out_strides,
                                     v_out_strides, static_cast<cudaStream_t>(cu_stream));
@@ -205,7 +214,7 @@ int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cach
   if (int rc = check_cache(who, cache)) return rc;
   if (int rc = check_batch(who, cache, batch, tokens)) return rc;
   if (int rc = check_rows(who, "q", q, q_strides, tokens, 2, 4)) return rc;
-  if (int rc = check_rows(who, "out", out, out_strides, tokens, 2, 4)) return rc;
+  if (int rc = check_out_rows(who, "out", out, out_strides, tokens, q_heads, 2, 4)) return rc;
   if (q_heads <= 0 || q_heads % cache->kv_heads)
     return set_error(B200TILE_ERR_INVALID, "%s: q_heads %d must be a positive multiple of kv_heads %d", who, q_heads,
                      cache->kv_heads);
@@ -243,7 +252,7 @@ int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cach
   a.workspace = workspace;
   a.stream = static_cast<cudaStream_t>(cu_stream);
   // the tile kernel moves rows by TMA and in 16-byte pieces; rows that do not lie so take row blocks, whatever their number
-  const bool tiles = may_tile(cache, batch, group) && !misaligned(q, 16) && !misaligned(out, 16) && !(a.q_ts % 8) &&
+  const bool tiles = may_tile(cache, batch, group) && (long long)a.batch.max_q * group > tile_rows(cache) && !misaligned(q, 16) && !misaligned(out, 16) && !(a.q_ts % 8) &&
                      !(a.q_hs % 8) && !(a.o_ts % 8) && !(a.o_hs % 8) && a.q_ts > 0 && a.q_hs > 0;
   a.tile_off = tiles ? split_bytes(cache, batch, tile_rows(cache)) : 0;
   // Prompts alone take one launch of the tile kernel; decode steps with prompts among them take both kernels, each its

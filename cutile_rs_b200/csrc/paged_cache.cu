@@ -99,7 +99,7 @@ struct BlockScale {
 };
 __device__ __forceinline__ BlockScale block_scale(float amax, float glob, float six_g, float inv_six_g) {
   BlockScale x;
-  const bool tame = amax < 0x1p100f && (amax > 0x1p-100f || amax == 0.0f) && six_g > 0x1p-20f && six_g < 0x1p20f;
+  const bool tame = amax < 0x1p90f && (amax > 0x1p-90f || amax == 0.0f) && six_g > 0x1p-20f && six_g < 0x1p20f;
   const float q = tame ? quotient(amax, six_g, inv_six_g) : __fdiv_rn(amax, six_g);
   x.byte = __nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
   x.s = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)x.byte, __NV_E4M3))) * glob;

@@ -40,6 +40,9 @@ __device__ __forceinline__ SeqView seq_view(const PagedBatch& p, int b) {
   return s;
 }
 
+// First key of the window of the token at position pos (which may be negative, and the window longer than anything).
+__device__ __forceinline__ int window_start(int pos, int window) { return pos >= window ? pos - window + 1 : 0; }
+
 // Page of key position `key` of sequence b, or num_pages (just outside the pool, where TMA reads zeros) with the
 // status record set.  Called for positions inside [0, len) only.
 __device__ __forceinline__ int page_of(const PagedBatch& p, int b, int key, uint32_t* status) {

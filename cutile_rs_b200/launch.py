@@ -957,7 +957,7 @@ def paged_attention(out: Tensor, q: Tensor, cache: PagedKvCache, batch: PagedBat
     elif workspace.device != cache.device or not workspace.is_contiguous():
         raise KernelLaunchError(f"{who}: the workspace must be contiguous on {cache.device}")
     rc = lib.b200tile_paged_attention(dt, cache.c, batch.c, q.storage.data_ptr(), out.storage.data_ptr(), tokens, q_heads,
-                                      qs, os, qk_scale, int(causal), window, softcap, workspace.data_ptr(),
+                                      qs, os, qk_scale, int(causal), min(window, 0x7fffffff), softcap, workspace.data_ptr(),
                                       workspace.nbytes, s)
     if rc:
         raise KernelLaunchError(lib.b200tile_last_error().decode())

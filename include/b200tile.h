@@ -402,6 +402,7 @@ typedef struct b200tile_paged_batch {
  * a 32-bit product is off by 2^-24 of it.  Format 1 writes, per 16 values, the scale e4m3(amax / (6 * global))
  * and the codes e2m1(y / (scale * global)), ties to even, saturating; y is not rounded to 16 bits before.  A block
  * cannot hold infinities or NaN: they become its largest code.
+ * Every new position needs a slot of its own; pages that sequences share are read only.
  *   q [tokens, q_heads, D] or NULL (then q_out is NULL too), k / v [tokens, kv_heads, D]; strides {token, head} in
  *   elements, multiples of 8; all tensors 16-byte aligned.  `q_out` may be `q`.
  *   rotary_dim  0 (inv_freq NULL: no rotation) or a multiple of 16 (format 1: 32) up to D; inv_freq f32
@@ -431,8 +432,8 @@ B200TILE_API int b200tile_paged_kv_gather(const char* dtype, const b200tile_page
  *   workspace  DEVICE scratch of b200tile_paged_attention_workspace_bytes(...) bytes for the same cache and batch
  *              (sizes only, not contents), 16-byte aligned; nothing in it outlives the call.  Calls that may overlap
  *              on the device must not share one, nor graphs that may be replayed at the same time
- * Cached rows at or behind kv_lens[b] and rows before every window of a block of queries are never looked at: they may hold anything, NaN
- * included.  A NaN or infinity in V at a key that some token of the sequence sees may also reach other tokens of the
+ * `out` may be `q` (the same rows); it must not overlap anything else that the call reads.  Cached rows at or behind
+ * kv_lens[b] are never looked at: they may hold anything, NaN included.  A NaN or infinity in V at a key that some token of the sequence sees may also reach other tokens of the
  * same sequence in the call (it is multiplied by a probability of 0). */
 B200TILE_API uint64_t b200tile_paged_attention_workspace_bytes(const b200tile_paged_cache* cache,
                                                                const b200tile_paged_batch* batch, int q_heads);

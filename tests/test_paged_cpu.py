@@ -105,6 +105,18 @@ def test_append_arguments():
     assert _append(c, b, tokens=0)[0] == _lib.OK
 
 
+def test_rows_that_are_written_share_no_memory():
+    lib = _lib.load()
+    for st in (I2(0, 128), I2(1024, 0)):
+        assert _attend(_cache(), _batch(), os=st)[0] == _lib.ERR_INVALID
+        rc = lib.b200tile_paged_kv_append(b"bf16", _cache(), _batch(), P, P, P, P, None, 4, 8, 0, I2(1024, 128), I2(512, 128),
+                                          I2(512, 128), st, None)
+        assert rc == _lib.ERR_INVALID and b"q_out" in lib.b200tile_last_error()
+        for ks, vs, name in ((st, I2(512, 128), b"k_out"), (I2(512, 128), st, b"v_out")):
+            assert lib.b200tile_paged_kv_gather(b"bf16", _cache(), _batch(), P, P, 4, ks, vs, None) == _lib.ERR_INVALID
+            assert name in lib.b200tile_last_error()
+
+
 def test_workspace_grows_with_what_it_holds():
     lib = _lib.load()
     size = lambda **kw: lib.b200tile_paged_attention_workspace_bytes(_cache(), _batch(**kw), 8)  # noqa: E731

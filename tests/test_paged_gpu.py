@@ -299,6 +299,46 @@ def test_lengths_and_ranges_that_do_not_fit(b200):
     assert _status(b200)[0] == 0
 
 
+@pytest.mark.parametrize("keys", [0, ref.MANY_KEYS])
+def test_windows_longer_than_anything(b200, keys):
+    """No window at all, whatever its size, also for a sequence shorter than its tokens."""
+    for fmt in ("16bit", "nvfp4"):
+        p = ref.Problem([60, 2, 40], [50, 1, 700], 4, 2, 64, 16, BF16, fmt, seed=51, table_keys=keys)
+        want = _check(p, 0.2)
+        for window in (701, 0x7ffffffe, 0x7fffffff, 1 << 40):
+            assert torch.equal(want, _attend(p, 0.2, window=window))
+
+
+@pytest.mark.parametrize("keys", [0, ref.MANY_KEYS])
+def test_pages_outside_the_pool_in_prompts(b200, keys):
+    """As for single tokens: zeros in their place, the sequence named in the status record."""
+    for fmt in ("16bit", "nvfp4"):
+        for bad in (-1, 1 << 20, -(1 << 31)):
+            p = ref.Problem([40, 120], [40, 700], 4, 2, 64, 16, BF16, fmt, seed=52, table_keys=keys)
+            p.table[1, 20] = bad
+            got = _attend(p, 0.2)
+            assert _status(b200)[:2] == (4, 1)
+            _lib.check(b200.b200tile_status_reset(torch.cuda.current_stream().cuda_stream))
+            for x in p.pools:
+                x[p.free[0]] = 0
+            p.table[1, 20] = int(p.free[0])
+            assert torch.equal(got, _attend(p, 0.2))
+
+
+@pytest.mark.parametrize("keys", [0, 8192])
+def test_lengths_up_to_the_largest_integer(b200, keys):
+    """Lengths and token ranges that no cache has: nothing outside the tensors is touched, nothing hangs."""
+    for fmt in ("16bit", "nvfp4"):
+        p = ref.Problem([40, 120], [40, 700], 4, 2, 64, 16, BF16, fmt, seed=53, table_keys=keys)
+        p.table.clamp_(min=0)
+        want = _attend(p, 0.2)
+        for kv, cu, window in ((0x7fffffff, 40, 0), (-(1 << 31), 40, 100), (700, -(1 << 31), 0), (700, 0x7fffffff, 33)):
+            p.kv[0], p.cu_q[0], p.cu_q[1] = kv, min(cu, 0), cu
+            _attend(p, 0.2, window=window)
+        p.kv[0], p.cu_q[0], p.cu_q[1] = 40, 0, 40
+        assert torch.equal(want, _attend(p, 0.2))
+
+
 def test_no_more_than_max_q_len_tokens(b200):
     p = ref.Problem([5, 2], [50, 60], 4, 2, 64, 16, BF16, seed=48, max_q=3)
     got = _attend(p, 0.2)
@@ -429,6 +469,18 @@ def test_append_large_and_special_values_fp4(b200):
     assert (v[0] == 0).all() and (v[1] == 2688).all() and (v[2] == 0).all()
     assert torch.equal(v[3], p.v[3].double())           # scale 0.5 exactly
     assert v[4, 0, 3] == 2688 and torch.isfinite(v).all()
+
+
+def test_append_of_extreme_values_with_extreme_factors_fp4(b200):
+    """Quotients beyond 32 bits keep their sign and saturate; those below the smallest scale are zeros."""
+    for glob in (2.0 ** -21, 2.0 ** 17):
+        p = ref.Problem([5], [5], 2, 1, 64, 16, BF16, "nvfp4", seed=3, k_global=glob, v_global=glob)
+        for i, unit in enumerate((2.0 ** 127, 2.0 ** 99, 2.0 ** 90, 2.0 ** 89, 2.0 ** -110)):
+            p.v[i] = unit
+            p.v[i, :, ::2] = -unit
+        launch.paged_kv_append(p.cache, p.batch, api.from_torch(p.k), api.from_torch(p.v))
+        k, v = p.rows(0, 5)
+        assert torch.equal(v[:4], torch.sign(p.v[:4].double()) * 2688 * glob) and (v[4] == 0).all()
 
 
 def test_gather_returns_what_append_wrote(b200):
