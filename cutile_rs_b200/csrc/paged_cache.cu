@@ -5,7 +5,9 @@
 // for every head of Q (to q_out) and K (to its slot); V and the dimensions from r on are copied.  An NVFP4 cache takes
 // blocks of 16: scale = e4m3(max |y| / (6 g)), code = e2m1(y / (scale g)) with g the pool's factor.
 //
-// HBM-bound: each value is read once and written once.  A warp takes a token (or a share of its heads): lane l always
+// HBM-bound in 16 bits (8192 tokens, 32 + 8 heads of 128: 45 us, 5.6 TB/s), by instructions with FP4 blocks (6700 tokens: 34
+// us against 22 us of traffic; two values at a time where the machine can).
+// Each value is read once and written once.  A warp takes a token (or a share of its heads): lane l always
 // holds the same D/16-th of a head, so its 8 cosines and sines stay in registers for all heads, and nothing but loads,
 // eight FMAs per vector and stores is left in the loop.  Angles: p * f_i reaches 1e5 and more, where a product rounded
 // to 32 bits is off by 1e-2 radians; angle, sine and cosine are taken in 64 bits and rounded to 32 once (64 of them per
@@ -13,6 +15,8 @@
 // on how far the position is.
 #include <cuda_fp4.h>
 #include <cuda_fp8.h>
+
+#include <algorithm>
 
 #include "paged_common.cuh"
 
@@ -35,6 +39,7 @@ struct AppendParams {
   int q_heads, rot;        // rot: dimensions that are rotated
   int shares;              // warps per token
   float k_six, k_inv_six, v_six, v_inv_six;   // FP4: 6 * global and its reciprocal
+  bool k_tame, v_tame;                        // and whether that is far from the ends of f32
 };
 struct GatherParams {
   PagedBatch batch;
@@ -79,50 +84,78 @@ __device__ __forceinline__ TokenPlace place_of(const PagedBatch& p, int b, int t
   return x;
 }
 
+template <bool F16>
+__device__ __forceinline__ uint32_t pack_pair(uint64_t x) {
+  float lo, hi;
+  unpack2(x, lo, hi);
+  return paged_pack16<F16>(lo, hi);
+}
+
 // Out of line: the argument reduction's registers stay out of the streaming loop.
 __device__ __noinline__ void angle_64(int pos, float inv_freq, double* s, double* c) {
   sincos((double)pos * (double)inv_freq, s, c);
 }
 
-// The quotient a / b rounded to nearest from inv = 1 / b rounded to nearest: q = a inv, then one correction by its exact
-// remainder (P. Markstein's theorem).  16-bit values meet the rounding borders of e2m1 and e4m3 exactly, where a plain
-// product with the reciprocal would miss the tie.  For b and a / b well inside the range of f32.
+// Quotients a / b from inv close to 1 / b: q = a inv, then one correction by its exact remainder, which leaves half a step
+// and a few millionths of one.  16-bit values meet the rounding borders of e2m1 and e4m3 exactly, where a plain product
+// with the reciprocal would miss the tie; the correction hits a quotient that 32 bits hold.  For b and a / b well inside
+// the range of f32.
 __device__ __forceinline__ float quotient(float a, float b, float inv) {
   const float q = __fmul_rn(a, inv);
   return __fmaf_rn(__fmaf_rn(-q, b, a), inv, q);
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t quotient2(uint64_t a, uint64_t neg_b, uint64_t inv) {
+  const uint64_t q = mul2(a, inv);
+  return fma2(fma2(q, neg_b, a), inv, q);
+}
 // A block's scale e4m3(amax / (6 g)) and 8 of its values -> codes of 4 bits, first value lowest.
 struct BlockScale {
   uint32_t byte;
-  float s, inv;
+  float s;
   bool plain;              // the quotients need the general division: s far out of range, or an infinity in the block
 };
-__device__ __forceinline__ BlockScale block_scale(float amax, float glob, float six_g, float inv_six_g) {
+__device__ __forceinline__ BlockScale block_scale(float amax, float glob, float six_g, float inv_six_g, bool tame_g) {
   BlockScale x;
-  const bool tame = amax < 0x1p90f && (amax > 0x1p-90f || amax == 0.0f) && six_g > 0x1p-20f && six_g < 0x1p20f;
-  const float q = tame ? quotient(amax, six_g, inv_six_g) : __fdiv_rn(amax, six_g);
-  x.byte = __nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
-  x.s = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)x.byte, __NV_E4M3))) * glob;
-  x.inv = __frcp_rn(x.s);
-  x.plain = !tame;
+  x.plain = !(tame_g && amax < 0x1p90f && (amax > 0x1p-90f || amax == 0.0f));
+  float q = quotient(amax, six_g, inv_six_g);
+  if (x.plain) q = __fdiv_rn(amax, six_g);
+  uint32_t f16x2;
+  asm("{.reg .b16 h; cvt.rn.satfinite.e4m3x2.f32 h, 0f00000000, %2; cvt.u32.u16 %0, h; cvt.rn.f16x2.e4m3x2 %1, h;}"
+      : "=r"(x.byte), "=r"(f16x2) : "f"(q));
+  x.s = __low2float(*reinterpret_cast<__half2*>(&f16x2)) * glob;
   return x;
 }
-__device__ __noinline__ uint32_t e2m1_codes_plain(float a, float b, float s) {
-  return (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(__fdiv_rn(a, s), __fdiv_rn(b, s)), __NV_E2M1, cudaRoundNearest);
-}
-__device__ __forceinline__ uint32_t e2m1_codes(const float (&y)[8], const BlockScale& b) {
-  if (!(b.s > 0.0f)) return 0u;
-  uint32_t w = 0;
-  if (b.plain) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w |= e2m1_codes_plain(y[2 * i], y[2 * i + 1], b.s) << (8 * i);
-    return w;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(quotient(y[2 * i], b.s, b.inv), quotient(y[2 * i + 1], b.s, b.inv)),
-                                            __NV_E2M1, cudaRoundNearest) << (8 * i);
+__device__ __forceinline__ uint32_t e2m1x8(const float (&y)[8]) {
+  uint32_t w;
+  asm("{.reg .b8 a, b, c, d;"
+      " cvt.rn.satfinite.e2m1x2.f32 a, %2, %1; cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;"
+      " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5; cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;"
+      " mov.b32 %0, {a, b, c, d};}"
+      : "=r"(w) : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
   return w;
+}
+__device__ __noinline__ uint32_t e2m1_codes_plain(uint64_t a, uint64_t b, uint64_t c, uint64_t d, float s) {
+  float y[8];
+  unpack2(a, y[0], y[1]);
+  unpack2(b, y[2], y[3]);
+  unpack2(c, y[4], y[5]);
+  unpack2(d, y[6], y[7]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(y[i], s);
+  return s > 0.0f ? e2m1x8(y) : 0u;
+}
+__device__ __forceinline__ uint32_t e2m1_codes(const uint64_t (&y)[4], float s) {
+  const float r = paged_rcp(s);
+  const uint64_t neg_b = pack2(-s, -s), inv = pack2(r, r);
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) unpack2(quotient2(y[i], neg_b, inv), f[2 * i], f[2 * i + 1]);
+  return s > 0.0f ? e2m1x8(f) : 0u;
 }
 
 template <int D, bool F16, bool FP4>
@@ -170,7 +203,7 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
   const TokenPlace at = place_of(p.batch, b, t, status);
 
   // cos and sin of this lane's 8 pairs: every lane evaluates LPH / 4 of them, the others come by shuffle
-  float cs[8], sn[8];
+  uint64_t cs[4], sn[4], neg_sn[4];                           // pairs of neighbours
   {
     constexpr int PER = D / 2 / 32 > 0 ? D / 2 / 32 : 1;      // angles per lane (1 or 2)
     float c[PER], s[PER];
@@ -187,10 +220,13 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
       }
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = (rotates ? sub * 8 : 0) + j;              // angle index
-      cs[j] = __shfl_sync(0xffffffffu, c[j % PER], i / PER);
-      sn[j] = __shfl_sync(0xffffffffu, s[j % PER], i / PER);
+    for (int j = 0; j < 4; ++j) {
+      const int i = (rotates ? sub * 8 : 0) + 2 * j;          // angle index
+      const float c0 = __shfl_sync(0xffffffffu, c[0], i / PER), s0 = __shfl_sync(0xffffffffu, s[0], i / PER);
+      const float c1 = __shfl_sync(0xffffffffu, c[PER - 1], (i + 1) / PER), s1 = __shfl_sync(0xffffffffu, s[PER - 1], (i + 1) / PER);
+      cs[j] = pack2(c0, c1);
+      sn[j] = pack2(s0, s1);
+      neg_sn[j] = pack2(-s0, -s1);
     }
   }
 
@@ -204,21 +240,19 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
       const bool is_v = i >= p.q_heads + p.c.kv_heads, is_q = i < p.q_heads;
       const bool turn = rotates && !is_v;
       const uint32_t wl[4] = {xl.x, xl.y, xl.z, xl.w}, wh[4] = {xh.x, xh.y, xh.z, xh.w};
-      float a[8], c[8];
+      uint64_t a[4], c[4];                                    // pairs of neighbours
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float2 f = paged_unpack16<F16>(wl[e]), h = paged_unpack16<F16>(wh[e]);
-        a[2 * e] = f.x;
-        a[2 * e + 1] = f.y;
-        c[2 * e] = h.x;
-        c[2 * e + 1] = h.y;
+        a[e] = pack2(f.x, f.y);
+        c[e] = pack2(h.x, h.y);
       }
       if (turn) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = a[e], y = c[e];
-          a[e] = __fsub_rn(__fmul_rn(x, cs[e]), __fmul_rn(y, sn[e]));   // the roundings of b200tile_rope_seq
-          c[e] = __fadd_rn(__fmul_rn(y, cs[e]), __fmul_rn(x, sn[e]));
+        for (int e = 0; e < 4; ++e) {                         // the roundings of b200tile_rope_seq
+          const uint64_t x = a[e], y = c[e];
+          a[e] = add2(mul2(x, cs[e]), mul2(y, neg_sn[e]));
+          c[e] = add2(mul2(y, cs[e]), mul2(x, sn[e]));
         }
       }
       if (!FP4 || is_q) {
@@ -234,10 +268,8 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
             const int da = is_v ? v_lo : lo_at, dc = is_v ? v_hi : hi_at;
             uint4 yl = xl, yh = xh;                           // copies stay the bits they were
             if (turn) {
-              yl = make_uint4(paged_pack16<F16>(a[0], a[1]), paged_pack16<F16>(a[2], a[3]), paged_pack16<F16>(a[4], a[5]),
-                              paged_pack16<F16>(a[6], a[7]));
-              yh = make_uint4(paged_pack16<F16>(c[0], c[1]), paged_pack16<F16>(c[2], c[3]), paged_pack16<F16>(c[4], c[5]),
-                              paged_pack16<F16>(c[6], c[7]));
+              yl = make_uint4(pack_pair<F16>(a[0]), pack_pair<F16>(a[1]), pack_pair<F16>(a[2]), pack_pair<F16>(a[3]));
+              yh = make_uint4(pack_pair<F16>(c[0]), pack_pair<F16>(c[1]), pack_pair<F16>(c[2]), pack_pair<F16>(c[3]));
             }
             *reinterpret_cast<uint4*>(dst + da) = yl;
             *reinterpret_cast<uint4*>(dst + dc) = yh;
@@ -248,9 +280,12 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
         // a block of 16 is this vector and its neighbour lane's (rotated pairs, V) or this lane's two (the rest)
         float ma = 0.0f, mc = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          ma = fmaxf(ma, fabsf(a[e]));
-          mc = fmaxf(mc, fabsf(c[e]));
+        for (int e = 0; e < 4; ++e) {
+          float x, y;
+          unpack2(a[e], x, y);
+          ma = fmaxf(ma, fmaxf(fabsf(x), fabsf(y)));
+          unpack2(c[e], x, y);
+          mc = fmaxf(mc, fmaxf(fabsf(x), fabsf(y)));
         }
         const float na = __shfl_xor_sync(0xffffffffu, ma, 1), nc = __shfl_xor_sync(0xffffffffu, mc, 1);
         if (!is_q && i < total && at.page >= 0) {
@@ -258,16 +293,22 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
           const float both = fmaxf(ma, mc);
           const float gl = is_v ? p.c.v_global : p.c.k_global, six = is_v ? p.v_six : p.k_six,
                       inv = is_v ? p.v_inv_six : p.k_inv_six;
-          const BlockScale sa = block_scale(halves ? fmaxf(ma, na) : both, gl, six, inv);
-          const BlockScale sc = block_scale(halves ? fmaxf(mc, nc) : both, gl, six, inv);
+          const bool tame = is_v ? p.v_tame : p.k_tame;
+          const BlockScale sa = block_scale(halves ? fmaxf(ma, na) : both, gl, six, inv, tame);
+          const BlockScale sc = block_scale(halves ? fmaxf(mc, nc) : both, gl, six, inv, tame);
+          uint32_t wa = e2m1_codes(a, sa.s), wc = e2m1_codes(c, sc.s);
+          if (sa.plain || sc.plain) {
+            wa = e2m1_codes_plain(a[0], a[1], a[2], a[3], sa.s);
+            wc = e2m1_codes_plain(c[0], c[1], c[2], c[3], sc.s);
+          }
           const long long h = is_v ? i - p.q_heads - p.c.kv_heads : i - p.q_heads;
           const long long* st = is_v ? p.c.v_st : p.c.k_st;
           const long long* sst = is_v ? p.c.vs_st : p.c.ks_st;
           uint8_t* row = (is_v ? p.c.v : p.c.k) + at.page * st[0] + h * st[1] + at.slot * st[2];
           uint8_t* srow = (is_v ? p.c.vs : p.c.ks) + at.page * sst[0] + h * sst[1] + at.slot * sst[2];
           const int da = is_v ? v_lo : lo_at, dc = is_v ? v_hi : hi_at;
-          *reinterpret_cast<uint32_t*>(row + da / 2) = e2m1_codes(a, sa);
-          *reinterpret_cast<uint32_t*>(row + dc / 2) = e2m1_codes(c, sc);
+          *reinterpret_cast<uint32_t*>(row + da / 2) = wa;
+          *reinterpret_cast<uint32_t*>(row + dc / 2) = wc;
           if (!halves || (sub & 1) == 0) srow[da / 16] = (uint8_t)sa.byte;
           if (halves && (sub & 1) == 0) srow[dc / 16] = (uint8_t)sc.byte;
         }
@@ -356,10 +397,11 @@ CacheView cache_view(const b200tile_paged_cache& c) {
   return v;
 }
 
-// Warps per token: one when the tokens alone fill the machine, else as many as there are rounds to share out.
-int shares_for(int tokens, int rounds, int sms) {
-  int s = (sms * 16 + tokens - 1) / tokens;
-  return s < 1 ? 1 : (s > rounds ? rounds : s);
+// Warps per token: one when the tokens alone fill the machine with `warps`, else as many as there are rounds to share out.
+// Every warp looks its token up, and append's takes the angles: at 6700 tokens two warps instead of one cost append 4 us of
+// 37 (FP4) and save gather 1 of 11.
+int shares_for(int tokens, int rounds, int warps) {
+  return std::max(1, std::min(rounds, (warps + tokens - 1) / tokens));
 }
 
 }  // namespace
@@ -388,8 +430,10 @@ int b200_paged_append_dispatch(int dtype, const b200tile_paged_cache& c, const b
   p.rot = rot;
   p.k_six = 6.0f * c.k_global; p.k_inv_six = 1.0f / p.k_six;
   p.v_six = 6.0f * c.v_global; p.v_inv_six = 1.0f / p.v_six;
+  p.k_tame = p.k_six > 0x1p-20f && p.k_six < 0x1p20f;
+  p.v_tame = p.v_six > 0x1p-20f && p.v_six < 0x1p20f;
   const int hpw = 32 / (c.head_dim / 16);
-  p.shares = shares_for(batch.tokens, (p.q_heads + 2 * c.kv_heads + hpw - 1) / hpw, di->sm_count);
+  p.shares = shares_for(batch.tokens, (p.q_heads + 2 * c.kv_heads + hpw - 1) / hpw, di->sm_count * 16);
   const long long warps = (long long)batch.tokens * p.shares;
   const unsigned grid = (unsigned)((warps + 3) / 4);
 #define B200_PA(D_, F_, Q_) paged_append_kernel<D_, F_, Q_><<<grid, 128, 0, stream>>>(p, di->status)
@@ -415,7 +459,7 @@ int b200_paged_gather_dispatch(int dtype, const b200tile_paged_cache& c, const b
   p.k_ts = ks[0]; p.k_hs = ks[1];
   p.v_ts = vs[0]; p.v_hs = vs[1];
   const int hpw = 32 / (c.head_dim / 16);
-  p.shares = shares_for(batch.tokens, (2 * c.kv_heads + hpw - 1) / hpw, di->sm_count);
+  p.shares = shares_for(batch.tokens, (2 * c.kv_heads + hpw - 1) / hpw, di->sm_count * 64);
   const unsigned grid = (unsigned)(((long long)batch.tokens * p.shares + 3) / 4);
 #define B200_PG(D_, F_, Q_) paged_gather_kernel<D_, F_, Q_><<<grid, 128, 0, stream>>>(p, di->status)
 #define B200_PG_F(D_, Q_) do { if (dtype) B200_PG(D_, true, Q_); else B200_PG(D_, false, Q_); } while (0)
