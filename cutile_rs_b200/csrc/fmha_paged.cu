@@ -12,7 +12,8 @@
 // nothing about the lengths has to be known on the host (a captured graph may be replayed with other lengths).  A run
 // that holds whole items writes their output; a run that holds part of an item writes (m, l, O) in 32 bits, at most
 // two such parts per worker, and the merge kernel adds the parts of an item in the order of the workers.  No atomics
-// and no state between launches: the same call gives the same bits.
+// and no state between launches: the same call gives the same bits.  (A run is taken by a few workers, one per head of
+// `heads_abreast`: the line counts groups of heads.)
 //
 // Inside a worker the products are transposed, S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16): the 16 rows of the
 // instruction are keys (or head dimensions) and its 8 columns the query rows, so 8 rows fill it; the usual orientation
@@ -101,6 +102,7 @@ struct SplitParams {
   int4* desc;
   long long part_floats;
   int workers, by_item, rb_max;
+  int heads_abreast, head_groups;    // neighbouring workers take these many heads of the same keys; kv_heads / that
   int coop;                          // CTAs per item (a cluster), whose warps share its steps: no parts, no merge kernel; or 0
   int min_steps;
   // FP4 operands, strides in bytes: those that are multiplied in every step fit in 32 bits
@@ -296,7 +298,7 @@ __device__ __forceinline__ long long block_line(const SplitParams& p, long long*
   long long mine = 0;
   for (int b = threadIdx.x * per; b < min(p.batch.batch, (int)(threadIdx.x + 1) * per); ++b) {
     const SeqWork w = seq_work<RB>(p, b);
-    mine += (long long)w.rbs * p.kv_heads * w.steps;
+    mine += (long long)w.rbs * p.head_groups * w.steps;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long inc = mine;
@@ -371,9 +373,10 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
   } else {
     const long long total = block_line<RB, THREADS>(p, s_sum);
     wid = warp * gridDim.x + blockIdx.x;                // neighbouring runs on different SMs
-    per = (total + p.workers - 1) / p.workers;
+    const int runs = p.workers / p.heads_abreast;
+    per = (total + runs - 1) / runs;
     if (per < p.min_steps) per = p.min_steps;
-    u = (long long)wid * per;
+    u = (long long)(wid / p.heads_abreast) * per;
     u_end = min(total, u + per);
     if (!p.by_item) {
       if (lane == 0) p.desc[wid] = make_int4(0, 0, 0, 0);
@@ -394,8 +397,8 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
     b = c_lo * ((p.batch.batch + THREADS - 1) / THREADS);
     line = s_sum[c_lo];                                 // first step of sequence b
     sw = seq_work<RB>(p, b);
-    while (line + (long long)sw.rbs * p.kv_heads * sw.steps <= u) {
-      line += (long long)sw.rbs * p.kv_heads * sw.steps;
+    while (line + (long long)sw.rbs * p.head_groups * sw.steps <= u) {
+      line += (long long)sw.rbs * p.head_groups * sw.steps;
       if (++b >= p.batch.batch) return;
       sw = seq_work<RB>(p, b);
     }
@@ -418,8 +421,8 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
       item = (int)(rel / sw.steps);
       st0 = (int)(rel - (long long)item * sw.steps);
       st1 = (int)min((long long)sw.steps, st0 + (u_end - u));
-      rb = item / p.kv_heads;
-      h = item - rb * p.kv_heads;
+      rb = item / p.head_groups;
+      h = (item - rb * p.head_groups) * p.heads_abreast + wid % p.heads_abreast;
     }
     const SeqView& sv = sw.s;
     RowMask<NT> rm = row_mask<NT>(p, sv, rb, lane);
@@ -878,8 +881,8 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
       if (p.by_item || parts) p.desc[at] = make_int4(parts, wid, b, rb * p.kv_heads + h);
     }
     u += st1 - st0;
-    if (u >= line + (long long)sw.rbs * p.kv_heads * sw.steps) {
-      line += (long long)sw.rbs * p.kv_heads * sw.steps;
+    if (u >= line + (long long)sw.rbs * p.head_groups * sw.steps) {
+      line += (long long)sw.rbs * p.head_groups * sw.steps;
       do {
         if (++b >= p.batch.batch) return;
         sw = seq_work<RB>(p, b);
@@ -904,7 +907,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 4 : 2) fmha_paged_merge_kernel(
   if (d.x <= 0 || (unsigned)d.y >= (unsigned)p.workers || (unsigned)d.z >= (unsigned)p.batch.batch || d.w < 0 ||
       d.w >= p.rb_max * p.kv_heads)
     return;
-  d.x = min(d.x, p.workers - d.y);
+  d.x = min(d.x, (p.workers - 1 - d.y) / p.heads_abreast + 1);
   const int pw = warp % PW, c = blockIdx.y * CT + warp / PW;
   const int b = d.z, rb = d.w / p.kv_heads, h = d.w % p.kv_heads;
   float m[NT][2], l[NT][2], o[NT][4];
@@ -935,7 +938,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 4 : 2) fmha_paged_merge_kernel(
 #pragma unroll
       for (int x = 0; x < U; ++x) {
         const int i = i0 + x * PW;
-        const float* src = p.part + ((long long)(d.y + i) * 2 + (i == 0 ? 1 : 0)) * p.part_floats;
+        const float* src = p.part + ((long long)(d.y + i * p.heads_abreast) * 2 + (i == 0 ? 1 : 0)) * p.part_floats;
         const float* ml = src + DT * NT * 128;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -1007,6 +1010,8 @@ int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
   p.workers = plan.workers;
   p.by_item = plan.by_item;
   p.coop = plan.coop;
+  p.heads_abreast = plan.heads_abreast;
+  p.head_groups = c.kv_heads / plan.heads_abreast;
   p.rb_max = (int)((std::min<long long>((long long)a.batch.max_q * p.group, a.row_limit) + 8 * NT - 1) / (8 * NT));
   p.min_steps = 2;
   CUtensorMap tmK = {}, tmV = {};
@@ -1092,12 +1097,19 @@ PagedSplitPlan b200_paged_split_plan(int format, int head_dim, int kv_heads, int
     pl.workers = 0;
     pl.by_item = false;
     pl.part_floats = pl.desc_off = 0;
+    pl.heads_abreast = 1;
     pl.bytes = 16;
     return pl;
   }
   pl.ctas = (int)std::max<long long>(1, std::min<long long>(148, (steps + 1) / 2));
   pl.workers = pl.ctas * warps;
   pl.by_item = pl.items <= pl.workers;
+  // Heads of a token lie side by side in one of the two usual orders, 64 to 256 bytes each: workers that take four of them
+  // at the same keys use what DRAM has open (NVFP4 32 x 16384 keys 99 -> 73 us, 24 x 16 heads of 64 70 -> 63; more than four,
+  // and the other order, change 2 % either way).  The smallest divisor from four on.
+  pl.heads_abreast = std::min(kv_heads, 4);
+  while (kv_heads % pl.heads_abreast) ++pl.heads_abreast;
+  if (pl.heads_abreast > 32 || pl.heads_abreast > pl.workers) pl.heads_abreast = 1;
   pl.part_floats = (size_t)pl.rows_per_block * (head_dim + 2);
   pl.desc_off = (size_t)pl.workers * 2 * pl.part_floats * sizeof(float);
   pl.bytes = pl.desc_off + sizeof(int4) * (size_t)(pl.by_item ? pl.items : pl.workers);

@@ -121,6 +121,7 @@ struct PagedSplitPlan {
   int ctas, workers;      // one worker = one warp
   long long items;        // (sequence, row block, K/V head) at most
   int coop;               // CTAs per item (no workspace needed), or 0: runs of the whole line
+  int heads_abreast;      // heads that neighbouring workers take side by side, a divisor of kv_heads
   bool by_item;           // descriptors indexed by item (few items) or by worker
   size_t part_floats;     // floats per partial-result slot
   size_t desc_off, bytes;
