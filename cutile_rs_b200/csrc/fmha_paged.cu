@@ -86,8 +86,9 @@ __device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&r)[4]) {
 
 constexpr int STEP = 16;             // keys per step
 // Warps per CTA, one CTA per SM.  16-bit, D = 128: 8 rings of 3 x 8 KB fill the shared memory; D = 64 halves the step and
-// takes half again as many warps.  NVFP4: what the registers allow.
-constexpr int split_warps(bool fp4, int d) { return fp4 ? 12 : d == 64 ? 12 : 8; }
+// takes half again as many warps.  NVFP4: what the registers allow (16 rows of 128: 8 warps 97, 12 that spill 108 us for 32 x
+// 16384 keys and four tokens).
+constexpr int split_warps(bool fp4, int d, int nt) { return fp4 ? (d == 128 && nt == 2 ? 8 : 12) : d == 64 ? 12 : 8; }
 constexpr float LAZY = 8.0f;         // the running reference of the exponents may lag behind the maximum by this
 
 struct SplitParams {
@@ -247,18 +248,18 @@ __device__ __forceinline__ void softmax_step(const ScoreParams (&sp)[NT][2], con
 }
 
 // One 16-bit K/V step: TMA boxes of 16 keys x 64 elements with the 128-byte swizzle, in a ring of the warp's own.
-template <int D>
+template <int D, int NT>
 struct Core16 {
-  static constexpr int WARPS = split_warps(false, D), STAGES = D == 64 ? 4 : 3;
+  static constexpr int WARPS = split_warps(false, D, NT), STAGES = D == 64 ? 4 : 3;
   static constexpr int KS = D == 64 ? 2 : 1;           // steps per iteration
   static constexpr int HALVES = D / 64, BOX = STEP * 128, TILE = HALVES * BOX, STAGE = 2 * TILE;
   static constexpr int RING = WARPS * STAGES * STAGE;
   static constexpr int SMEM = 1024 + RING + WARPS * STAGES * 8 + 16;
 };
 // One FP4 step: 16 keys of packed values and scales copied with cp.async into a ring of the warp's own.
-template <int D>
+template <int D, int NT>
 struct Core4 {
-  static constexpr int WARPS = split_warps(true, D), STAGES = 6;
+  static constexpr int WARPS = split_warps(true, D, NT), STAGES = 6;
   static constexpr int KS = 2;
   static constexpr int ROW = D / 2, SROW = D / 16;
   static constexpr int STAGE = 2 * STEP * (ROW + SROW);
@@ -321,11 +322,11 @@ __device__ __forceinline__ long long block_line(const SplitParams& p, long long*
 }
 
 template <int D, bool F16, int NT, bool CAP, bool FP4>
-__global__ void __launch_bounds__((FP4 ? Core4<D>::WARPS : Core16<D>::WARPS) * 32, 1)
+__global__ void __launch_bounds__((FP4 ? Core4<D, NT>::WARPS : Core16<D, NT>::WARPS) * 32, 1)
 fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                         const __grid_constant__ SplitParams p, uint32_t* status) {
-  using C16 = Core16<D>;
-  using C4 = Core4<D>;
+  using C16 = Core16<D, NT>;
+  using C4 = Core4<D, NT>;
   constexpr int WARPS = FP4 ? C4::WARPS : C16::WARPS, THREADS = WARPS * 32;
   constexpr int STAGES = FP4 ? C4::STAGES : C16::STAGES;
   constexpr int KS = FP4 ? C4::KS : C16::KS;
@@ -441,12 +442,16 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
         for (int j = 0; j < 2; ++j) rm.hi[nt][j] = min(rm.hi[nt][j], k1 * STEP);
     }
 
-    // page numbers of 32 steps at a time, one per lane
-    int pages = 0, pages_at = 0;
-    auto fetch_pages = [&](int i) {
-      pages_at = i;
-      const int key = (k0 + i + lane) * STEP;
-      pages = i + lane < nk ? page_of(p.batch, b, key, status) : 0;
+    // page numbers of 32 steps at a time, one per lane; with FP4's shorter steps the next 32 are on their way
+    int pages = 0, pages_ahead = 0, pages_at = 0;
+    auto fetch_pages = [&](int i) { return i + lane < nk ? page_of(p.batch, b, (k0 + i + lane) * STEP, status) : 0; };
+    auto page_at = [&](int i) {                       // of step i, for steps in rising order
+      while (i - pages_at >= 32) {
+        pages_at += 32;
+        pages = FP4 ? pages_ahead : fetch_pages(pages_at);
+        if (FP4) pages_ahead = fetch_pages(pages_at + 32);
+      }
+      return __shfl_sync(0xffffffffu, pages, i - pages_at);
     };
     const int slot_mask = (1 << p.batch.page_shift) - 1;
     // FP4: where this lane's pieces of a step lie in the pools, for page 0 and slot 0 of this head
@@ -461,13 +466,14 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
       s_slot = is_v ? p.vs_slot : p.ks_slot;
       s_lane = (is_v ? p.vs : p.ks) + (long long)h * (is_v ? p.vs_head : p.ks_head) + (long long)(lane & 15) * s_slot;
     }
-    auto issue = [&](int i) {
+    // FP4: this lane's pieces of the step issued last; the next step of the same page is one addition away
+    const uint8_t *k_from = nullptr, *v_from = nullptr, *s_from = nullptr;
+    bool page_ok = false;
+    auto issue = [&](int i, uint32_t dst) {
       if (i >= nk) return;                            // warp-uniform
-      if (i - pages_at >= 32) fetch_pages(i);
-      const int pg = __shfl_sync(0xffffffffu, pages, i - pages_at);
       const int slot = ((k0 + i) * STEP) & slot_mask;
-      const uint32_t dst = ring + ((ring_at + i) % STAGES) * (FP4 ? C4::STAGE : C16::STAGE);
       if constexpr (!FP4) {
+        const int pg = page_at(i);
         const uint32_t bar = bars + ((ring_at + i) % STAGES) * 8;
         if (lane == 0) {
           mbar_expect_tx(bar, C16::STAGE);
@@ -478,25 +484,36 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
           }
         }
       } else {
-        const bool ok = pg < p.batch.num_pages;
-        const uint32_t pgc = ok ? pg : 0;             // a valid address for the copies that read nothing
-        const uint8_t* kp = k_lane + (uint64_t)pgc * p.k_page + (uint64_t)(uint32_t)slot * p.k_slot;
-        const uint8_t* vp = v_lane + (uint64_t)pgc * p.v_page + (uint64_t)(uint32_t)slot * p.v_slot;
-        const uint8_t* sp_ = s_lane + (uint64_t)pgc * s_page + (uint64_t)(uint32_t)slot * s_slot;
+        if (i == 0 || slot == 0) {
+          const int pg = page_at(i);
+          page_ok = pg < p.batch.num_pages;
+          const uint32_t pgc = page_ok ? pg : 0;      // a valid address for the copies that read nothing
+          k_from = k_lane + (uint64_t)pgc * p.k_page + (uint64_t)(uint32_t)slot * p.k_slot;
+          v_from = v_lane + (uint64_t)pgc * p.v_page + (uint64_t)(uint32_t)slot * p.v_slot;
+          s_from = s_lane + (uint64_t)pgc * s_page + (uint64_t)(uint32_t)slot * s_slot;
+        } else {
+          k_from += (uint64_t)STEP * p.k_slot;
+          v_from += (uint64_t)STEP * p.v_slot;
+          s_from += (uint64_t)STEP * s_slot;
+        }
         constexpr int CH = C4::ROW / 16, ROWS = 32 / CH;   // 16-byte chunks per row; rows a pass of the warp covers
 #pragma unroll
         for (int c = 0; c < STEP / ROWS; ++c) {
-          cp_async_16(dst + c * 512 + lane * 16, kp + (uint64_t)(c * ROWS) * p.k_slot, ok);
-          cp_async_16(dst + STEP * C4::ROW + c * 512 + lane * 16, vp + (uint64_t)(c * ROWS) * p.v_slot, ok);
+          cp_async_16(dst + c * 512 + lane * 16, k_from + (uint64_t)(c * ROWS) * p.k_slot, page_ok);
+          cp_async_16(dst + STEP * C4::ROW + c * 512 + lane * 16, v_from + (uint64_t)(c * ROWS) * p.v_slot, page_ok);
         }
-        cp_async_small<C4::SROW>(dst + 2 * STEP * C4::ROW + lane * C4::SROW, sp_, ok);
+        cp_async_small<C4::SROW>(dst + 2 * STEP * C4::ROW + lane * C4::SROW, s_from, page_ok);
       }
     };
+    constexpr uint32_t STAGE_BYTES = FP4 ? C4::STAGE : C16::STAGE;
+    // FP4: an iteration's KS slots lie side by side; those being worked on, and those the next copies go to
+    uint32_t group_at = ring, group_to = ring + (STAGES - KS) * STAGE_BYTES;
     if (nk > 0) {
-      fetch_pages(0);
+      pages = fetch_pages(0);
+      if (FP4) pages_ahead = fetch_pages(32);
 #pragma unroll
       for (int s = 0; s < STAGES - (FP4 ? KS : 0); ++s) {
-        issue(s);
+        issue(s, ring + (FP4 ? s : (ring_at + s) % STAGES) * STAGE_BYTES);
         if (FP4 && s % KS == KS - 1) asm volatile("cp.async.commit_group;" ::: "memory");
       }
     }
@@ -624,17 +641,17 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
         }
         __syncwarp();                                 // every lane is done with the slots before they are filled again
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) issue(i + STAGES + ks);
+        for (int ks = 0; ks < KS; ++ks) issue(i + STAGES + ks, at[ks]);
       } else {
         // one group per iteration: KS steps
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES / KS - 2) : "memory");
         __syncwarp();
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) issue(i + STAGES - KS + ks);   // into the slots that the last iteration was done with
+        for (int ks = 0; ks < KS; ++ks) issue(i + STAGES - KS + ks, group_to + ks * STAGE_BYTES);   // the last iteration is done with those
         asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          const uint32_t sK = ring + ((ring_at + i + ks) % STAGES) * C4::STAGE;
+          const uint32_t sK = group_at + ks * C4::STAGE;
           const uint32_t sKs = sK + 2 * STEP * C4::ROW;
           // K: keys g and g + 8, D/4 dimensions of each (D/8 bytes), one scale per two words
           constexpr int WORDS = D / 32;
@@ -682,7 +699,7 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
         // ones.  Row m of tile c <-> dimension D/8 m + 2c, row m + 8 <-> the next one.
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-          const uint32_t sV = ring + ((ring_at + i + ks) % STAGES) * C4::STAGE + STEP * C4::ROW;
+          const uint32_t sV = group_at + ks * C4::STAGE + STEP * C4::ROW;
           const uint32_t sVs = sV + STEP * C4::ROW + STEP * C4::SROW;
           uint32_t vm0 = ~0u, vm1 = ~0u;
           if (clear) v_mask(ks, vm0, vm1);
@@ -736,13 +753,15 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
             }
           }
         }
+        group_to = group_at;
+        group_at = group_at == ring + (STAGES - KS) * STAGE_BYTES ? ring : group_at + KS * STAGE_BYTES;
       }
     }
     if (FP4 && nk > 0) {
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
     }
-    if (nk > 0) ring_at += nk;
+    if (!FP4 && nk > 0) ring_at += nk;
 
     // ---- the part's result ----
 #pragma unroll
@@ -986,8 +1005,8 @@ __global__ void __launch_bounds__(256, NT == 1 ? 4 : 2) fmha_paged_merge_kernel(
 
 template <int D, bool F16, int NT, bool CAP, bool FP4>
 int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
-  using C16 = Core16<D>;
-  using C4 = Core4<D>;
+  using C16 = Core16<D, NT>;
+  using C4 = Core4<D, NT>;
   constexpr int SMEM = FP4 ? C4::SMEM : C16::SMEM;
   constexpr int THREADS = (FP4 ? C4::WARPS : C16::WARPS) * 32;
   const b200h::DeviceInfo* di = b200h::device_info();
@@ -1080,7 +1099,7 @@ static constexpr int COOP_STEPS = 16;
 PagedSplitPlan b200_paged_split_plan(int format, int head_dim, int kv_heads, int batch, long long rows,
                                      long long max_keys) {
   PagedSplitPlan pl;
-  const int warps = b200::split_warps(format != 0, head_dim);
+  const int warps = b200::split_warps(format != 0, head_dim, rows <= 8 ? 1 : 2);
   pl.rows_per_block = rows <= 8 ? 8 : 16;
   const long long rb_max = (rows + pl.rows_per_block - 1) / pl.rows_per_block;
   pl.items = (long long)batch * rb_max * kv_heads;
