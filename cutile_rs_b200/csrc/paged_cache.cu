@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
   const TokenPlace at = place_of(p.batch, b, t, status);
 
   // cos and sin of this lane's 8 pairs: every lane evaluates LPH / 4 of them, the others come by shuffle
-  uint64_t cs[4], sn[4], neg_sn[4];                           // pairs of neighbours
+  float cs[8], sn[8];
   {
     constexpr int PER = D / 2 / 32 > 0 ? D / 2 / 32 : 1;      // angles per lane (1 or 2)
     float c[PER], s[PER];
@@ -220,13 +220,10 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = (rotates ? sub * 8 : 0) + 2 * j;          // angle index
-      const float c0 = __shfl_sync(0xffffffffu, c[0], i / PER), s0 = __shfl_sync(0xffffffffu, s[0], i / PER);
-      const float c1 = __shfl_sync(0xffffffffu, c[PER - 1], (i + 1) / PER), s1 = __shfl_sync(0xffffffffu, s[PER - 1], (i + 1) / PER);
-      cs[j] = pack2(c0, c1);
-      sn[j] = pack2(s0, s1);
-      neg_sn[j] = pack2(-s0, -s1);
+    for (int j = 0; j < 8; ++j) {
+      const int i = (rotates ? sub * 8 : 0) + j;              // angle index
+      cs[j] = __shfl_sync(0xffffffffu, c[j % PER], i / PER);
+      sn[j] = __shfl_sync(0xffffffffu, s[j % PER], i / PER);
     }
   }
 
@@ -243,17 +240,17 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
       uint64_t a[4], c[4];                                    // pairs of neighbours
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float2 f = paged_unpack16<F16>(wl[e]), h = paged_unpack16<F16>(wh[e]);
+        float2 f = paged_unpack16<F16>(wl[e]), h = paged_unpack16<F16>(wh[e]);
+        if (turn) {
+          // the roundings of b200tile_rope_seq; in scalars, since the paired products and sums get fused
+          const float2 x = f, y = h;
+          f.x = __fsub_rn(__fmul_rn(x.x, cs[2 * e]), __fmul_rn(y.x, sn[2 * e]));
+          f.y = __fsub_rn(__fmul_rn(x.y, cs[2 * e + 1]), __fmul_rn(y.y, sn[2 * e + 1]));
+          h.x = __fadd_rn(__fmul_rn(y.x, cs[2 * e]), __fmul_rn(x.x, sn[2 * e]));
+          h.y = __fadd_rn(__fmul_rn(y.y, cs[2 * e + 1]), __fmul_rn(x.y, sn[2 * e + 1]));
+        }
         a[e] = pack2(f.x, f.y);
         c[e] = pack2(h.x, h.y);
-      }
-      if (turn) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {                         // the roundings of b200tile_rope_seq
-          const uint64_t x = a[e], y = c[e];
-          a[e] = add2(mul2(x, cs[e]), mul2(y, neg_sn[e]));
-          c[e] = add2(mul2(y, cs[e]), mul2(x, sn[e]));
-        }
       }
       if (!FP4 || is_q) {
         if (i < total) {

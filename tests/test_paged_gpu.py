@@ -445,6 +445,32 @@ def test_append(b200, fmt, layout, d, rot, dtype, heads, kvh, page):
     assert _status(b200)[0] == 0
 
 
+@pytest.mark.parametrize("fmt", ["16bit", "nvfp4"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_append_rounds_as_the_formula_in_32_bits(b200, fmt, dtype):
+    """Angles in 64 bits, cosine and sine rounded to 32, then two products and a sum, each rounded: the same bits."""
+    p = ref.Problem([700, 1, 300], [700, 90000, 20300], 8, 2, 128, 64, dtype, fmt, seed=54)
+    f, q, k, v, _, q_out = _append_case(p, 128)
+    pos = torch.cat([torch.arange(kv - n, kv, device="cuda") for n, kv in zip(p.q_lens, p.kv_lens)])
+    angle = pos.double()[:, None] * f.double()[None]
+    c, s = angle.cos().float()[:, None], angle.sin().float()[:, None]
+
+    def turned(x):
+        lo, hi = x[..., :64].float(), x[..., 64:].float()
+        return torch.cat((lo * c - hi * s, hi * c + lo * s), -1)
+
+    assert torch.equal(q_out, turned(q).to(dtype))
+    at = 0
+    for b, n in enumerate(p.q_lens):
+        want = turned(k)[at:at + n]
+        got = p.rows(b, p.kv_lens[b])[0][-n:]
+        if fmt == "16bit":
+            assert torch.equal(got, want.to(dtype).double())
+        else:
+            assert torch.equal(got, ref.quantise(want.double())[0])
+        at += n
+
+
 def test_append_without_q_and_in_place(b200):
     p = ref.Problem([5, 1], [40, 9], 4, 2, 128, 16, BF16, seed=1)
     f, q, k, v, _, q_out = _append_case(p, 128, in_place=True)
