@@ -17,7 +17,7 @@
 //   - an NVFP4 cache takes four more warps: thread r expands key r of the step (64 bytes and 8 scales for D = 128) to f16
 //     straight into the swizzled operand tile, K and V in turn, with the next row's bytes already in registers.  The
 //     products are then f16 x f16, which holds every code * scale exactly; bf16 queries are brought to a power of two near
-//     1 row by row and converted in shared memory by two otherwise idle warps.
+//     1 row by row and converted in shared memory by the softmax threads before their first scores.
 //
 // What bounds it: as fmha_fwd.cu, the softmax threads and the tensor pipe together.
 #include <math_constants.h>
@@ -93,6 +93,11 @@ __device__ __forceinline__ void tma_load_4d_tile(uint32_t dst, const void* desc,
 __device__ __forceinline__ float absmax3(float a, float b, float c) {
   float d;
   asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {   // of a number and a NaN, the number
+  uint32_t d;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -304,7 +309,6 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   __shared__ Part s_part[PART_RING];
   __shared__ long long s_row_off[FA_BM];          // element offset of a tile's row in the output, from its first token
   __shared__ int s_row_tok[FA_BM];                // its token
-  __shared__ float s_unit[CONVERT ? 2 : 1][CONVERT ? 2 : 1][CONVERT ? 128 : 1];   // [item parity][tile][row]
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen_base = smem_raw + (base - smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -335,7 +339,7 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar_q_full + i * 8, 1);
       mbar_init(bar_q_free + i * 8, 1);
-      mbar_init(bar_q_ready + i * 8, 1);
+      mbar_init(bar_q_ready + i * 8, 4);               // the tile's softmax warps
       mbar_init(bar_s_full + i * 8, 1);
       mbar_init(bar_p_full + i * 8, 4);
       mbar_init(bar_o_done + i * 8, 1);
@@ -539,7 +543,7 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       }
     }
   } else if (warp < 4) {
-    // ------- Q of tile `warp - 2`; bf16 queries for f16 products: converted, a power of two per row taken out -------
+    // ----------------------------- Q of tile `warp - 2` -----------------------------
     const int t = warp - 2;
     uint32_t items = 0;
     for (int i = 0; have_part(i); ++i) {
@@ -555,46 +559,6 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         for (int h = 0; h < HALVES; ++h)
           tma_load_3d(sQ + t * TILE + h * HALF, &tmQ, bar_q_full + t * 8, h * 64, q_head, q_row);
       }
-      if (!CONVERT) {
-        ++items;
-        continue;
-      }
-      if (!wait_all(bar_q_full + t * 8, items & 1, 25)) break;
-#pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        const int r = i * 32 + lane;
-        const uint32_t row = sQ + t * TILE + r * 128;
-        float mx = 0.0f;
-#pragma unroll 4
-        for (int c = 0; c < HALVES * 8; ++c) {
-          uint32_t x[4];
-          ld_shared_v4(row + (c >> 3) * HALF + (((c & 7) ^ (r & 7)) << 4), x);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = paged_unpack16<false>(x[e]);
-            mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-        }
-        const uint32_t e = __float_as_uint(mx) & 0x7f800000u;
-        const bool scaled = e > (27u << 23) && e < (227u << 23);   // not for rows of zeros, infinities or NaN
-        const float inv = scaled ? __uint_as_float((254u << 23) - e) : 1.0f;
-        s_unit[items & 1][t][r] = scaled ? __uint_as_float(e) : 1.0f;
-#pragma unroll 4
-        for (int c = 0; c < HALVES * 8; ++c) {
-          const uint32_t at = row + (c >> 3) * HALF + (((c & 7) ^ (r & 7)) << 4);
-          uint32_t x[4];
-          ld_shared_v4(at, x);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = paged_unpack16<false>(x[k]);
-            x[k] = pack_f16x2(f.x * inv, f.y * inv);
-          }
-          st_shared_v4(at, x[0], x[1], x[2], x[3]);
-        }
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_q_ready + t * 8);
       ++items;
     }
     if (items > 0) mbar_wait(wctx, bar_q_full + t * 8, (items - 1) & 1, 15);   // nothing in flight when this warp leaves
@@ -625,14 +589,41 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       uint64_t k2[CAP_POLY_N];             // the polynomial in s itself
       float scale = p.score.scale_log2, cap_arg = p.score.cap_arg;
       float m_run = -CUDART_INF_F, l_run = 0.0f;
+      if (CONVERT && n_mine > 0) {
+        // bf16 queries for f16 products: this thread's row, a power of two taken out of it and put into the scale.  (By a
+        // warp per tile beside the softmax of the item before, a first item waited 10 us for it.)
+        if (!wait_all(bar_q_full + t * 8, items & 1, 25)) { ok = false; break; }
+        const uint32_t at = sQ + t * TILE + row * 128;
+        uint32_t x[HALVES * 8][4], most = 0;
+#pragma unroll
+        for (int c = 0; c < HALVES * 8; ++c) ld_shared_v4(at + (c >> 3) * HALF + (((c & 7) ^ (row & 7)) << 4), x[c]);
+#pragma unroll
+        for (int c = 0; c < HALVES * 8; ++c)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) most = max_bf16x2(most, x[c][k] & 0x7fff7fffu);
+        const float2 m2 = paged_unpack16<false>(most);
+        const uint32_t e = __float_as_uint(fmaxf(m2.x, m2.y)) & 0x7f800000u;
+        const bool scaled = e > (27u << 23) && e < (227u << 23);   // not for rows of zeros, infinities or NaN
+        const float inv = scaled ? __uint_as_float((254u << 23) - e) : 1.0f;
+        const float unit = scaled ? __uint_as_float(e) : 1.0f;
+#pragma unroll
+        for (int c = 0; c < HALVES * 8; ++c) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = paged_unpack16<false>(x[c][k]);
+            x[c][k] = pack_f16x2(f.x * inv, f.y * inv);
+          }
+          st_shared_v4(at + (c >> 3) * HALF + (((c & 7) ^ (row & 7)) << 4), x[c][0], x[c][1], x[c][2], x[c][3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_q_ready + t * 8);
+        scale *= unit;
+        cap_arg *= unit;
+      }
       for (int j = 0; j < n_mine; ++j, ++steps) {
         if (!wait_all(bar_s_full + t * 8, steps & 1, 30)) { ok = false; break; }
         tc_fence_after_sync();
-        if (CONVERT && j == 0) {
-          const float unit = s_unit[items & 1][t][row];
-          scale *= unit;
-          cap_arg *= unit;
-        }
         if (CAP && j == 0) {
           const float a = cap_arg * (0.5f / 1.4426950408889634f), aa = a * a;      // scale / c and its powers, if f32 holds them
           poly_max = a > 0x1p-14f && a < 0x1p14f ? CAP_POLY_MAX / a : -1.0f;
