@@ -19,7 +19,9 @@
 //     products are then f16 x f16, which holds every code * scale exactly; bf16 queries are brought to a power of two near
 //     1 row by row and converted in shared memory by the softmax threads before their first scores.
 //
-// What bounds it: as fmha_fwd.cu, the softmax threads and the tensor pipe together.
+// What bounds it: as fmha_fwd.cu, the softmax threads and the tensor pipe together, 2.1 us a step of 256 x 128 (2.45 with the
+// cap, 2.6 over NVFP4), and 4 to 5 us to begin and end an item.  A prompt of 4096 tokens, 32 / 8 heads of 128: 144 us, 950
+// TFLOP/s; four chunks to 256 tokens over 5000 NVFP4 keys 51 us.
 #include <math_constants.h>
 
 #include <algorithm>
