@@ -6,7 +6,7 @@
 // Query rows are packed per K/V head (row = token * group + head of the group) in blocks of 8 or 16, so that a K/V row
 // is read once for all heads that share it.  What bounds it is HBM: each cached byte is used for `group` rows only.
 // 8 x 65536 keys of 8 x 128: 330 us, 6.5 TB/s; 64 sequences to 8192 keys 157 us, 6.0 TB/s; launch, first copies and merge take
-// about 9 us of any call.  NVFP4 is bound by instructions, 300 a step of 16 keys, half of them conversions and scale
+// about 9 us of any call.  NVFP4 is bound by instructions, 325 a step of 16 keys, 128 of them conversions and scale
 // products: 32 sequences to 16384 keys 69 us, 3.9 TB/s.
 //
 // Work split.  One worker is ONE WARP.  Sequence b has steps(b) steps of 16 keys, an item is (sequence, row block, K/V
