@@ -105,7 +105,7 @@ def attention(p, scale, causal=True, window=0, softcap=0.0):
     Per row: the output's own rounding, half a step of its type; probabilities whose exponents are off by the scores'
     error (a 32-bit dot product of d terms, the score's scale and the exponential's argument: (d + 8) 2^-24 of
     sum |q k| scale, with a cap 2^-19 of it more) and which are handed over in two 16-bit pieces (2^-15 of p; one f16 piece, 2^-11,
-    for bf16 over NVFP4; one piece of the type, half a step, in calls with sequences of more than 16 rows, 48 over NVFP4), all against sum p |v|; sums of n
+    for bf16 over NVFP4; one piece of the type, half a step, in calls whose max_q_len allows more than 16 rows, 48 over NVFP4), all against sum p |v|; sums of n
     terms in 32 bits.  Pieces in f16 (f16 rows, and all rows over NVFP4) have no relative step below 2^-14: they are off by
     up to half of f16's smallest step, 2^-25, each, while the largest p is at least 1 and so is the sum they are divided by:
     2^-25 sum |v| over the keys seen."""
@@ -118,7 +118,7 @@ def attention(p, scale, causal=True, window=0, softcap=0.0):
     for b, (n, kv) in enumerate(zip(p.q_lens, p.kv_lens)):
         if n == 0 or kv <= 0:
             continue
-        piece = few if max(p.q_lens) * group <= (16 if p.fmt == "16bit" else 48) else eps / 2
+        piece = few if p.batch.max_q_len * group <= (16 if p.fmt == "16bit" else 48) else eps / 2
         k, v = p.rows(b, kv)
         pos = torch.arange(kv - n, kv, device="cuda")[:, None]
         key = torch.arange(kv, device="cuda")[None, :]
