@@ -188,13 +188,25 @@ __device__ __forceinline__ void softmax_step(const ScoreParams (&sp)[NT][2], con
                                              uint32_t (&pl)[KS][NT][2]) {
   const int g = lane >> 2;
   bool over = false;
+  if (CAP) {
+    auto capped = [&](auto&& score) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[ks][nt][e] = score(sp[nt][e & 1], s[ks][nt][e]);
+    };
+    if (sp[0][0].cap_out <= CAP_SMALL_OUT) capped([](const ScoreParams& a, float x) { return paged_score_near(a, x); });
+    else capped([](const ScoreParams& a, float x) { return paged_score<true>(a, x); });
+  }
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float x = paged_score<CAP>(sp[nt][e & 1], s[ks][nt][e]);
+        float x = CAP ? s[ks][nt][e] : paged_score<false>(sp[nt][e & 1], s[ks][nt][e]);
         if (ragged) {
           const int key = key0 + ks * STEP + g + (e >> 1) * 8;
           if (key < rm.lo[nt][e & 1] || key >= rm.hi[nt][e & 1]) x = -CUDART_INF_F;
@@ -568,7 +580,7 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
         for (int j = 0; j < 2; ++j) {
           const float f = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * j);
           sp[nt][j].scale_log2 *= f;
-          sp[nt][j].cap_arg *= f;
+          sp[nt][j].cap_arg = cap_arg_in_range(sp[nt][j].cap_arg * f);
         }
       }
     }
@@ -1020,7 +1032,7 @@ int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
   p.q = static_cast<const uint16_t*>(a.q);
   p.out = static_cast<uint16_t*>(a.out);
   p.q_ts = a.q_ts; p.q_hs = a.q_hs; p.o_ts = a.o_ts; p.o_hs = a.o_hs;
-  p.score = a.score;
+  p.score = paged_score_params(a, FP4 ? c.k_global : 1.0f);
   p.kv_heads = c.kv_heads;
   p.group = a.q_heads / c.kv_heads;
   p.causal = a.causal;
@@ -1038,8 +1050,6 @@ int launch_split(const PagedAttnArgs& a, const PagedSplitPlan& plan) {
   p.min_steps = 2;
   CUtensorMap tmK = {}, tmV = {};
   if constexpr (FP4) {
-    p.score.scale_log2 *= c.k_global;
-    p.score.cap_arg *= c.k_global;
     p.out_scale = c.v_global;
     p.k = static_cast<const uint8_t*>(c.k);
     p.v = static_cast<const uint8_t*>(c.v);

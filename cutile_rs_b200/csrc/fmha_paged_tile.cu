@@ -32,15 +32,6 @@
 namespace b200 {
 namespace {
 
-// c log2e tanh(x), x = s scale / c, as an odd polynomial in x with c log2e folded into the coefficients: the Chebyshev
-// interpolant of tanh(sqrt u) / sqrt u on [0, 0.4^2], off by at most 4.5e-8 for |x| <= 0.4.  Scores are a small part of the
-// cap almost always; steps with a larger one take exp2 and a reciprocal instead, which triples the load of the
-// special-function unit that bounds the softmax (8.2 against 2.6 thousand cycles a step).
-constexpr float CAP_POLY_MAX = 0.4f;
-constexpr int CAP_POLY_N = 4;
-constexpr float CAP_POLY[CAP_POLY_N] = {0.9999998807907104f, -0.33331355452537537f, 0.13270874321460724f,
-                                        -0.04754934832453728f};
-
 struct TileParams {
   PagedBatch batch;
   ScoreParams score;
@@ -51,7 +42,6 @@ struct TileParams {
   long long o_ts, o_hs;
   int wide_out;                      // the output's rows lie on 32-byte boundaries
   float out_scale;
-  float cap_poly[CAP_POLY_N];        // CAP_POLY * c log2e
   float* part;                       // two slots per CTA
   int4* desc;                        // one per CTA
   // FP4 operands: byte strides
@@ -108,6 +98,12 @@ __device__ __forceinline__ void st_shared_v4(uint32_t dst, uint32_t a, uint32_t 
 }
 __device__ __forceinline__ void ld_shared_v4(uint32_t src, uint32_t (&w)[4]) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src) : "memory");
+}
+
+// Out of line: with a cap beyond CAP_SMALL_OUT and scores near it, which hardly ever meet, and the registers of both forms
+// stay out of the softmax loop (inlined, prompt chunks with a cap of 30 took 126 us instead of 122).
+__device__ __noinline__ float score_any_cap(float scale, float cap_arg, float cap_out, float s) {
+  return paged_score<true>(ScoreParams{scale, cap_arg, cap_out}, s);
 }
 
 // Pairs of tiles that sequence b has here: none when its rows are few enough for the row-block kernel.
@@ -621,18 +617,21 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_q_ready + t * 8);
         scale *= unit;
-        cap_arg *= unit;
+        cap_arg = cap_arg_in_range(cap_arg * unit);
       }
       for (int j = 0; j < n_mine; ++j, ++steps) {
         if (!wait_all(bar_s_full + t * 8, steps & 1, 30)) { ok = false; break; }
         tc_fence_after_sync();
         if (CAP && j == 0) {
-          const float a = cap_arg * (0.5f / 1.4426950408889634f), aa = a * a;      // scale / c and its powers, if f32 holds them
-          poly_max = a > 0x1p-14f && a < 0x1p14f ? CAP_POLY_MAX / a : -1.0f;
-          float f = a;
+          // The polynomial in s itself, for rows whose scores are all a small part of the cap: c tanh(s a) log2e = s (k0 + k1 s^2
+          // + ..), a = scale / c.  Up to 2^62 the powers of s are numbers; those of a may underflow, where the cap is so
+          // far away that they do not matter.  With a beyond 2^14 they might overflow.
+          const float a = cap_arg * CAP_HALF_ARG, aa = a * a;
+          poly_max = a < 0x1p14f ? fminf(CAP_POLY_MAX / a, 0x1p62f) : -1.0f;
+          float f = scale;
 #pragma unroll
           for (int i = 0; i < CAP_POLY_N; ++i) {
-            k2[i] = pack2(p.cap_poly[i] * f, p.cap_poly[i] * f);
+            k2[i] = pack2(cap_poly(i) * f, cap_poly(i) * f);
             f *= aa;
           }
         }
@@ -746,16 +745,22 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             });
           }
         } else {
+          // some score of the warp's rows is near the cap
+          auto each = [&](auto&& score) {
+            probabilities([&](uint64_t s2) {
+              float sa, sd;
+              unpack2(s2, sa, sd);
+              float xa = score(sa), xd = score(sd);
+              if (sa == -CUDART_INF_F) xa = -CUDART_INF_F;
+              if (sd == -CUDART_INF_F) xd = -CUDART_INF_F;
+              return pack2(xa, xd);
+            });
+          };
           const float off = p.score.cap_out + neg_m;
-          probabilities([&](uint64_t s2) {
-            float sa, sd;
-            unpack2(s2, sa, sd);
-            float xa = fmaf(-2.0f * p.score.cap_out, paged_rcp(1.0f + ex2_approx(sa * cap_arg)), off);
-            float xd = fmaf(-2.0f * p.score.cap_out, paged_rcp(1.0f + ex2_approx(sd * cap_arg)), off);
-            if (sa == -CUDART_INF_F) xa = -CUDART_INF_F;
-            if (sd == -CUDART_INF_F) xd = -CUDART_INF_F;
-            return pack2(xa, xd);
-          });
+          if (p.score.cap_out <= CAP_SMALL_OUT)
+            each([&](float x) { return fmaf(-2.0f * p.score.cap_out, paged_rcp(1.0f + ex2_approx(x * cap_arg)), off); });
+          else
+            each([&](float x) { return score_any_cap(scale, cap_arg, p.score.cap_out, x) + neg_m; });
         }
         float ls[4];
         {
@@ -979,7 +984,7 @@ int launch_tile(const PagedAttnArgs& a, const PagedTilePlan& plan) {
   const b200tile_paged_cache& c = *a.cache;
   TileParams p = {};
   p.batch = a.batch;
-  p.score = a.score;
+  p.score = paged_score_params(a, FP4 ? c.k_global : 1.0f);
   p.kv_heads = c.kv_heads;
   p.group = a.q_heads / c.kv_heads;
   p.tpt = FA_BM / p.group;
@@ -992,7 +997,6 @@ int launch_tile(const PagedAttnArgs& a, const PagedTilePlan& plan) {
   p.o_hs = a.o_hs;
   p.wide_out = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && a.o_ts % 16 == 0 && a.o_hs % 16 == 0;
   p.out_scale = 1.0f;
-  for (int i = 0; i < CAP_POLY_N; ++i) p.cap_poly[i] = CAP_POLY[i] * a.score.cap_out;
   p.part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + a.tile_off);
   p.desc = reinterpret_cast<int4*>(static_cast<char*>(a.workspace) + a.tile_off + plan.desc_off);
   const CUtensorMapDataType dt = F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -1004,8 +1008,6 @@ int launch_tile(const PagedAttnArgs& a, const PagedTilePlan& plan) {
                                      CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   if constexpr (FP4) {
-    p.score.scale_log2 *= c.k_global;
-    p.score.cap_arg *= c.k_global;
     p.out_scale = c.v_global;
     p.k = static_cast<const uint8_t*>(c.k);
     p.v = static_cast<const uint8_t*>(c.v);

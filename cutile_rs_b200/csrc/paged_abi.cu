@@ -242,11 +242,9 @@ int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cach
   a.q_hs = q_strides[1];
   a.o_ts = out_strides[0];
   a.o_hs = out_strides[1];
-  const float log2e = 1.4426950408889634f;
-  a.score.scale_log2 = qk_scale * log2e;
+  a.qk_scale = qk_scale;
+  a.softcap = softcap;
   a.capped = softcap > 0.0f;
-  a.score.cap_arg = a.capped ? 2.0f * log2e * qk_scale / softcap : 0.0f;
-  a.score.cap_out = softcap * log2e;
   a.causal = causal != 0;
   a.window = window;
   a.workspace = workspace;
