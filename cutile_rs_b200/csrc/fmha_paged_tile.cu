@@ -655,6 +655,9 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           const float big = fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3]));
           poly = __all_sync(0xffffffffu, blind || big <= poly_max);
         }
+        // What a masked column holds: -inf, or with a cap, which makes -c of a score of -inf, a NaN of its own that no product
+        // gives and the maximum passes over.
+        constexpr uint32_t MASKED = CAP ? 0xffc0ffeeu : 0xff800000u;
         if (masked_tile) {
 #pragma unroll
           for (int c = 0; c < FA_BN / 32; ++c) {
@@ -664,7 +667,7 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             bits &= l <= 0 ? ~0u : l > 31 ? 0u : ~0u << l;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (!((bits >> i) & 1u)) v[c * 32 + i] = 0xff800000u;  // -inf
+              if (!((bits >> i) & 1u)) v[c * 32 + i] = MASKED;
           }
         }
         float mx[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
@@ -675,8 +678,9 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             mx[u] = max3(mx[u], __uint_as_float(v[i + 2 * u]), __uint_as_float(v[i + 2 * u + 1]));
         }
         const float rmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        // the score grows with s: the largest s has the largest score (the cap maps -inf to -cap: kept apart)
-        const float m_tile = blind || rmax == -CUDART_INF_F ? -CUDART_INF_F
+        // the score grows with s: the largest s has the largest score (under a cap a row of -inf has -c)
+        const bool none = CAP ? max(c_lo, 0) > min(c_hi, FA_BN - 1) : rmax == -CUDART_INF_F;
+        const float m_tile = blind || none ? -CUDART_INF_F
                              : CAP             ? paged_score<true>(ScoreParams{scale, cap_arg, p.score.cap_out}, rmax)
                                                : rmax * scale;
         const float m_new = fmaxf(m_run, m_tile);
@@ -739,8 +743,8 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
               float sa, sd, xa, xd;
               unpack2(s2, sa, sd);
               unpack2(capped(s2), xa, xd);
-              if (sa == -CUDART_INF_F) xa = -CUDART_INF_F;             // masked: stays out, cap or not
-              if (sd == -CUDART_INF_F) xd = -CUDART_INF_F;
+              if (__float_as_uint(sa) == MASKED) xa = -CUDART_INF_F;
+              if (__float_as_uint(sd) == MASKED) xd = -CUDART_INF_F;
               return pack2(xa, xd);
             });
           }
@@ -751,8 +755,8 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
               float sa, sd;
               unpack2(s2, sa, sd);
               float xa = score(sa), xd = score(sd);
-              if (sa == -CUDART_INF_F) xa = -CUDART_INF_F;
-              if (sd == -CUDART_INF_F) xd = -CUDART_INF_F;
+              if (__float_as_uint(sa) == MASKED) xa = -CUDART_INF_F;
+              if (__float_as_uint(sd) == MASKED) xd = -CUDART_INF_F;
               return pack2(xa, xd);
             });
           };

@@ -76,3 +76,50 @@ def test_caps_far_below_the_scores(b200, fmt, keys):
         want, tol = ref.attention(p, 0.125, softcap=cap)
         # the scores are off by no more than 2 c: nothing; the bound without a cap holds them
         assert ((got.double() - want).abs() <= tol).all(), cap
+
+
+@pytest.mark.parametrize("keys", [0, ref.MANY_KEYS])
+@pytest.mark.parametrize("window", [0, 60])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_infinite_scores_under_a_cap(b200, dtype, window, keys):
+    """c tanh(-inf) = -c and c tanh(inf) = c: a key with an infinite score takes part, whichever kernel looks at it."""
+    cap = 4.0
+    p = ref.Problem([70, 3, 40], [300, 40, 40], 4, 2, 64, 16, dtype, seed=63, table_keys=keys)
+    p.q[..., 0] = 0.5
+    for b, key in ((0, 250), (0, 100), (1, 5), (2, 0), (2, 17)):
+        page, slot = int(p.table[b, key // 16]), key % 16
+        p.pools[0][page, 0, slot, 0] = float("-inf")
+        p.pools[0][page, 1, slot, 0] = float("inf")
+    got = _attend(p, 0.125, softcap=cap, window=window)
+    # the definition with stand-ins for the infinite values that are far beyond the cap, too
+    q = ref.Problem([70, 3, 40], [300, 40, 40], 4, 2, 64, 16, dtype, seed=63, table_keys=keys)
+    q.q[..., 0] = 0.5
+    for b, key in ((0, 250), (0, 100), (1, 5), (2, 0), (2, 17)):
+        page, slot = int(q.table[b, key // 16]), key % 16
+        q.pools[0][page, 0, slot, 0] = -30000.0
+        q.pools[0][page, 1, slot, 0] = 30000.0
+    want, _ = ref.attention(q, 0.125, softcap=cap, window=window)
+    # as ref.attention's bound, for the scores that are not at the cap (which are exact), against the largest |v|
+    q.pools[0][q.pools[0].abs() == 30000.0] = 0.0
+    eps, room = torch.finfo(dtype).eps, 0.0
+    for b, kv in enumerate(p.kv_lens):
+        k, v = q.rows(b, kv)
+        qk = float(torch.einsum("qhd,khd->hqk", q.q[q.cu[b]:q.cu[b + 1]].double().abs(),
+                                k.abs().repeat_interleave(2, 1)).max()) * 0.125
+        terms = 3 * ((64 + 8) * 2.0 ** -24 * qk + cap * 2.0 ** -19) + eps / 2 + (kv + 16) * 2.0 ** -24 + 2.0 ** -20
+        room = max(room, float(v.abs().max()) * (terms + 2.0 ** -25 * kv))
+    assert not torch.isnan(got).any()
+    assert ((got.double() - want).abs() <= eps / 2 * want.abs() + room).all()
+
+
+@pytest.mark.parametrize("keys", [0, ref.MANY_KEYS])
+@pytest.mark.parametrize("softcap", [0.0, 4.0, 1e4])
+def test_nan_scores_stay_nan(b200, softcap, keys):
+    """The rows that see a NaN key are NaN, for the heads that it belongs to; the others are numbers."""
+    for dtype in (BF16, F16):
+        p = ref.Problem([70, 3], [300, 40], 4, 2, 64, 16, dtype, seed=68, table_keys=keys)
+        p.pools[0][int(p.table[0, 260 // 16]), 1, 260 % 16, 5] = float("nan")
+        got = _attend(p, 0.125, softcap=softcap)
+        want = torch.zeros_like(got, dtype=torch.bool)
+        want[260 - 230:70, 2:] = True                      # positions 230 .. 299
+        assert torch.equal(torch.isnan(got), want)
