@@ -178,7 +178,7 @@ __device__ __forceinline__ RowMask<NT> row_mask(const SplitParams& p, const SeqV
 // The online softmax of one step: s[nt] holds S^T (keys g and g + 8, rows 2t and 2t + 1 of block nt) and becomes the
 // B operand of O^T += V^T P^T.  Statistics in 32 bits.  The reference m that is subtracted from the exponents is the
 // same for all lanes of a row and moves only when some score exceeds it by more than 2^8: one vote per step instead of
-// a maximum over eight lanes.  P <= 256 then, and l >= 1 for any row that saw a key.  P is handed over as a 16-bit value
+// a maximum over eight lanes.  P <= 2^(8 + p_shift) then, and l >= 1 for any row that saw a key.  P is handed over as a 16-bit value
 // plus the 16-bit rest of it (HILO): the rounding of P alone would put an error as large as the output's own rounding
 // beside it, and the second product costs nothing next to the loads.
 template <bool F16, int KS, int NT, int DT, bool CAP, bool HILO>
@@ -240,7 +240,7 @@ __device__ __forceinline__ void softmax_step(const ScoreParams (&sp)[NT][2], con
   for (int nt = 0; nt < NT; ++nt) {
     float m_use[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) m_use[j] = m_run[nt][j] == -CUDART_INF_F ? 0.0f : m_run[nt][j];   // nothing seen yet
+    for (int j = 0; j < 2; ++j) m_use[j] = m_run[nt][j] == -CUDART_INF_F ? 0.0f : m_run[nt][j] - p_shift<F16>();   // nothing seen yet
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll

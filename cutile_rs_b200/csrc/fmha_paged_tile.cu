@@ -706,7 +706,7 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
             tmem_st_32x32b_x32(tO + c * 32, o);
           }
         }
-        const float neg_m = m_run == -CUDART_INF_F ? 0.0f : -m_run;
+        const float neg_m = m_run == -CUDART_INF_F ? 0.0f : p_shift<MF16>() - m_run;
         uint64_t ls2[4] = {0ull, 0ull, 0ull, 0ull};
         // P = exp2(score - m) of 32 columns at a time, to 16 bits, over S's columns
         auto probabilities = [&](auto&& score_minus_m) {

@@ -109,6 +109,13 @@ __device__ __forceinline__ float paged_score(const ScoreParams& sp, float s) {
   return cap_is_far(s * sp.cap_arg) ? a : b;
 }
 
+// Probabilities are handed to the second product as 16-bit values.  f16 has nothing between 0 and 2^-24: behind a key that
+// holds most of a row's weight with little of its value, 2^18 keys of 2^-19.6 each came out 2 % too small.  So they are
+// exp2(x - m + 7), with the running reference m at most 8 below the maximum: up to 2^15, and down to 2^-31 of the largest,
+// which is below what sums in 32 bits hold.  bf16 has f32's range.
+template <bool F16>
+__device__ constexpr float p_shift() { return F16 ? 7.0f : 0.0f; }
+
 template <bool F16>
 __device__ __forceinline__ uint32_t paged_pack16(float lo, float hi) {
   return F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);

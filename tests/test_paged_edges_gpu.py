@@ -1,9 +1,11 @@
 """Paged key/value cache at the ends of what its calls accept, against 64-bit plain forms."""
+import math
+
 import pytest
 import torch
 
 import paged_reference as ref
-from cutile_rs_b200 import api, launch
+from cutile_rs_b200 import api, launch, paged
 
 pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
@@ -123,3 +125,45 @@ def test_nan_scores_stay_nan(b200, softcap, keys):
         want = torch.zeros_like(got, dtype=torch.bool)
         want[260 - 230:70, 2:] = True                      # positions 230 .. 299
         assert torch.equal(torch.isnan(got), want)
+
+
+@pytest.mark.parametrize("fmt,d,dtype", [("16bit", 128, F16), ("16bit", 64, F16), ("nvfp4", 128, BF16), ("nvfp4", 64, F16),
+                                         ("nvfp4", 128, F16)])
+@pytest.mark.parametrize("q_len,batch", [(1, 150), (40, 20)])
+def test_a_long_tail_of_small_probabilities(b200, fmt, d, dtype, q_len, batch):
+    """One key that holds most of the weight, with a value of zero, and 2^18 that share the rest: their probabilities,
+    2^-19.6 of the first's, are far below the normal range of 16-bit floats (20.45 of f16's smallest steps), their sum is
+    not.  The tail's keys are all alike, so that the result is known.  So many sequences, over the same pages, that most
+    items are not cut and a worker meets the first key and its tail."""
+    kv, kvh = (1 << 18) + 1, 8
+    x = 24 - math.log2(20.45)                              # log2 of the first key's weight over one of the tail
+    p = ref.Problem([q_len], [kv], kvh, kvh, d, 256, dtype, fmt, seed=64)
+    for pool, scales in zip(p.pools, p.scales):
+        pool.zero_()
+        if scales is not None:
+            scales.fill_(0x38)                             # 1.0
+    first = int(p.table[0, 0])
+    if fmt == "16bit":
+        p.pools[0][first, :, 0, 0] = 1.0
+        p.pools[1].fill_(0.5)
+        p.pools[1][first, :, 0] = 0.0
+    else:
+        p.pools[0][first, :, 0, 0] = 0x2                   # code of 1
+        p.pools[1].fill_(0x11)                             # codes of 0.5
+        p.pools[1][first, :, 0] = 0
+    q = torch.zeros(batch * q_len, kvh, d, dtype=dtype, device="cuda")
+    q[..., 0] = 1.0
+    cu = torch.arange(batch + 1, dtype=torch.int32, device="cuda") * q_len
+    batch_of = paged.PagedBatch(p.table.repeat(batch, 1), cu, p.kv.repeat(batch), q_len)
+    out = torch.empty_like(q)
+    launch.paged_attention(api.from_torch(out), api.from_torch(q), p.cache, batch_of, x * math.log(2.0))
+    n = torch.arange(kv - q_len, kv, device="cuda", dtype=torch.float64).repeat(batch)     # keys of the tail a token sees
+    tail = n * 2.0 ** -x
+    want = 0.5 * tail / (1 + tail)
+    # half a step of the type; weights handed over in one f16 piece, 2^-11, and their exponents, x 2^-22, above and below
+    # the line; the sum of the weights: up to 2^18 / 8 terms a lane, each rounded by 2^-24 of a partial sum of 1 + tail at
+    # most, that of the products: 2^18 / 16 steps, two products each, that drop up to 2^-23 of the sum
+    eps = torch.finfo(dtype).eps
+    room = (eps / 2 + 2.0 ** -11 + 2 * x * 2.0 ** -22 + 2.0 ** -9 + 2.0 ** -8) * want
+    off = (out.double() - want[:, None, None]).abs()
+    assert (off <= room[:, None, None]).all(), float((off / room[:, None, None]).max())
