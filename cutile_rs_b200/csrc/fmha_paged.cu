@@ -579,8 +579,8 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float f = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * j);
-          sp[nt][j].scale_log2 *= f;
-          sp[nt][j].cap_arg = cap_arg_in_range(sp[nt][j].cap_arg * f);
+          sp[nt][j].scale_log2 = factor_in_range(sp[nt][j].scale_log2 * f);
+          sp[nt][j].cap_arg = factor_in_range(sp[nt][j].cap_arg * f);
         }
       }
     }

@@ -616,8 +616,8 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_q_ready + t * 8);
-        scale *= unit;
-        cap_arg = cap_arg_in_range(cap_arg * unit);
+        scale = factor_in_range(scale * unit);
+        cap_arg = factor_in_range(cap_arg * unit);
       }
       for (int j = 0; j < n_mine; ++j, ++steps) {
         if (!wait_all(bar_s_full + t * 8, steps & 1, 30)) { ok = false; break; }

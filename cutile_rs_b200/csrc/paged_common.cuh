@@ -78,8 +78,8 @@ __host__ __device__ constexpr float cap_poly(int i) {
 }
 constexpr float CAP_SMALL_OUT = 64.0f * 1.4426950408889634f;    // cap_out up to which one form serves
 constexpr float CAP_HALF_ARG = 0.5f / 1.4426950408889634f;     // t = z * this
-// A factor of 0 or infinity would make NaN of scores that are infinite or 0.
-__host__ __device__ __forceinline__ float cap_arg_in_range(float x) { return fminf(fmaxf(x, 0x1p-126f), 0x1p126f); }
+// A factor that underflows to 0 or overflows would make NaN of scores that are infinite, masked ones too, or 0.
+__host__ __device__ __forceinline__ float factor_in_range(float x) { return fminf(fmaxf(x, 0x1p-126f), 0x1p126f); }
 __device__ __forceinline__ float paged_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -154,8 +154,8 @@ struct PagedAttnArgs {
 inline b200::ScoreParams paged_score_params(const PagedAttnArgs& a, float factor) {
   const double log2e = 1.4426950408889634, scale = a.qk_scale * factor;
   b200::ScoreParams p;
-  p.scale_log2 = (float)(scale * log2e);
-  p.cap_arg = a.capped ? b200::cap_arg_in_range((float)(2.0 * log2e * scale / a.softcap)) : 0.0f;
+  p.scale_log2 = b200::factor_in_range((float)(scale * log2e));
+  p.cap_arg = a.capped ? b200::factor_in_range((float)(2.0 * log2e * scale / a.softcap)) : 0.0f;
   p.cap_out = (float)std::min(a.softcap * log2e, 1e38);      // twice it is still a number
   return p;
 }

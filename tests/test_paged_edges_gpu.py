@@ -167,3 +167,17 @@ def test_a_long_tail_of_small_probabilities(b200, fmt, d, dtype, q_len, batch):
     room = (eps / 2 + 2.0 ** -11 + 2 * x * 2.0 ** -22 + 2.0 ** -9 + 2.0 ** -8) * want
     off = (out.double() - want[:, None, None]).abs()
     assert (off <= room[:, None, None]).all(), float((off / room[:, None, None]).max())
+
+
+def test_factors_that_underflow_together(b200):
+    """A scale times a factor of the pool below the smallest 32-bit number: every score is 0, masked keys stay out."""
+    for keys in (0, ref.MANY_KEYS):
+        for softcap in (0.0, 20.0):
+            p = ref.Problem([70, 2], [90, 200], 4, 2, 64, 16, BF16, "nvfp4", seed=65, table_keys=keys)
+            p.poison()
+            p.kg = 1e-30
+            p.cache = paged.PagedKvCache(*p.pools, *p.scales, 1e-30, 1.0)
+            got = _attend(p, 1e-20, softcap=softcap)
+            want, tol = ref.attention(p, 1e-20, softcap=softcap)
+            assert not torch.isnan(got).any()
+            assert ((got.double() - want).abs() <= tol).all()
