@@ -113,11 +113,18 @@ __device__ __forceinline__ uint64_t quotient2(uint64_t a, uint64_t neg_b, uint64
   const uint64_t q = mul2(a, inv);
   return fma2(fma2(q, neg_b, a), inv, q);
 }
+// The largest magnitude, NaN if one is NaN: the block's scale then is NaN too, and all of it reads back as NaN.  A maximum
+// that passes over NaN would store it as the block's largest code, which is 0 among zeros.
+__device__ __forceinline__ float absmax_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // A block's scale e4m3(amax / (6 g)) and 8 of its values -> codes of 4 bits, first value lowest.
 struct BlockScale {
   uint32_t byte;
   float s;
-  bool plain;              // the quotients need the general division: s far out of range, or an infinity in the block
+  bool plain;              // the quotients need the general division: s far out of range, an infinity or a NaN in the block
 };
 __device__ __forceinline__ BlockScale block_scale(float amax, float glob, float six_g, float inv_six_g, bool tame_g) {
   BlockScale x;
@@ -280,19 +287,19 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
         for (int e = 0; e < 4; ++e) {
           float x, y;
           unpack2(a[e], x, y);
-          ma = fmaxf(ma, fmaxf(fabsf(x), fabsf(y)));
+          ma = absmax_nan(ma, x, y);
           unpack2(c[e], x, y);
-          mc = fmaxf(mc, fmaxf(fabsf(x), fabsf(y)));
+          mc = absmax_nan(mc, x, y);
         }
         const float na = __shfl_xor_sync(0xffffffffu, ma, 1), nc = __shfl_xor_sync(0xffffffffu, mc, 1);
         if (!is_q && i < total && at.page >= 0) {
           const bool halves = is_v || rotates;
-          const float both = fmaxf(ma, mc);
+          const float both = absmax_nan(ma, mc, mc);
           const float gl = is_v ? p.c.v_global : p.c.k_global, six = is_v ? p.v_six : p.k_six,
                       inv = is_v ? p.v_inv_six : p.k_inv_six;
           const bool tame = is_v ? p.v_tame : p.k_tame;
-          const BlockScale sa = block_scale(halves ? fmaxf(ma, na) : both, gl, six, inv, tame);
-          const BlockScale sc = block_scale(halves ? fmaxf(mc, nc) : both, gl, six, inv, tame);
+          const BlockScale sa = block_scale(halves ? absmax_nan(ma, na, na) : both, gl, six, inv, tame);
+          const BlockScale sc = block_scale(halves ? absmax_nan(mc, nc, nc) : both, gl, six, inv, tame);
           uint32_t wa = e2m1_codes(a, sa.s), wc = e2m1_codes(c, sc.s);
           if (sa.plain || sc.plain) {
             wa = e2m1_codes_plain(a[0], a[1], a[2], a[3], sa.s);

@@ -401,7 +401,8 @@ typedef struct b200tile_paged_batch {
  * Dimensions from rotary_dim on are copied.  theta is taken in 64 bits: far positions keep their angle, where
  * a 32-bit product is off by 2^-24 of it.  Format 1 writes, per 16 values, the scale e4m3(amax / (6 * global))
  * and the codes e2m1(y / (scale * global)), ties to even, saturating; y is not rounded to 16 bits before.  A block
- * cannot hold infinities or NaN: they become its largest code.
+ * cannot hold an infinity, which becomes its largest code (2688 * global).  A NaN makes its block's scale NaN (0x7f):
+ * the whole block reads as NaN.
  * Every new position needs a slot of its own; pages that sequences share are read only.
  *   q [tokens, q_heads, D] or NULL (then q_out is NULL too), k / v [tokens, kv_heads, D]; strides {token, head} in
  *   elements, multiples of 8; all tensors 16-byte aligned.  `q_out` may be `q`.

@@ -181,3 +181,40 @@ def test_factors_that_underflow_together(b200):
             want, tol = ref.attention(p, 1e-20, softcap=softcap)
             assert not torch.isnan(got).any()
             assert ((got.double() - want).abs() <= tol).all()
+
+
+def test_nan_on_the_way_into_nvfp4_stays_visible(b200):
+    """A block that holds a NaN, among finite values, among zeros, among infinities or alone, reads back as NaN; the other
+    blocks of its row keep their values; attention over it is NaN for the heads that see it."""
+    for d, rot in ((64, 0), (128, 32), (128, 128)):
+        p = ref.Problem([6], [6], 2, 1, d, 16, BF16, "nvfp4", seed=66)
+        clean = [x.clone() for x in (p.k, p.v)]
+        nan, inf = float("nan"), float("inf")
+        p.v[0, 0, 3] = nan
+        p.v[1, 0, :16] = 0.0
+        p.v[1, 0, 7] = nan
+        p.v[2, 0, 16:32] = nan
+        p.v[3, 0, 16], p.v[3, 0, 17] = inf, nan
+        p.v[4, 0, 31] = -nan
+        p.k[5, 0, d - 1] = nan
+        f = None
+        if rot:
+            i = torch.arange(0, rot, 2, dtype=torch.float64, device="cuda")
+            f = api.from_torch((10000.0 ** (-i / rot)).float())
+        launch.paged_kv_append(p.cache, p.batch, api.from_torch(p.k), api.from_torch(p.v), inv_freq=f)
+        out = [torch.empty(6, 1, d, dtype=BF16, device="cuda") for _ in range(2)]
+        launch.paged_kv_gather(api.from_torch(out[0]), api.from_torch(out[1]), p.cache, p.batch)
+        k, v = out
+        for t, block in ((0, 0), (1, 0), (2, 1), (3, 1), (4, 1)):
+            want = torch.zeros(d // 16, dtype=torch.bool, device="cuda")
+            want[block] = True
+            assert torch.equal(torch.isnan(v[t, 0]).reshape(-1, 16).all(-1), want)
+            assert torch.equal(torch.isnan(v[t, 0]).reshape(-1, 16).any(-1), want)
+        lost = torch.isnan(k[5, 0]).reshape(-1, 16)
+        turned = {d // 16 - 1} | ({d // 32 - 1} if rot == d else set())      # its partner in the rotation, too
+        assert {i for i in range(d // 16) if lost[i].any()} == turned and all(lost[i].all() for i in turned)
+        assert not torch.isnan(k[:5]).any() and not torch.isnan(v[5]).any()
+        good = ~torch.isnan(v)
+        q = ref.Problem([6], [6], 2, 1, d, 16, BF16, "nvfp4", seed=66)
+        launch.paged_kv_append(q.cache, q.batch, api.from_torch(clean[0]), api.from_torch(clean[1]))
+        assert torch.equal(p.rows(0, 6)[1][good], q.rows(0, 6)[1][good])
