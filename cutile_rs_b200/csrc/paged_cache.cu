@@ -193,8 +193,8 @@ __global__ void __launch_bounds__(128) paged_append_kernel(const __grid_constant
       a = v_lo;
       c = v_hi;
     }
-    lo = __ldg(reinterpret_cast<const uint4*>(x + a));
-    hi = __ldg(reinterpret_cast<const uint4*>(x + c));
+    lo = *reinterpret_cast<const uint4*>(x + a);             // not as read-only data: q may be q_out
+    hi = *reinterpret_cast<const uint4*>(x + c);
   };
   constexpr int U = 3;                        // rounds in flight: 3 x 32 bytes a lane
   uint4 lo[U], hi[U];

@@ -218,3 +218,25 @@ def test_nan_on_the_way_into_nvfp4_stays_visible(b200):
         q = ref.Problem([6], [6], 2, 1, d, 16, BF16, "nvfp4", seed=66)
         launch.paged_kv_append(q.cache, q.batch, api.from_torch(clean[0]), api.from_torch(clean[1]))
         assert torch.equal(p.rows(0, 6)[1][good], q.rows(0, 6)[1][good])
+
+
+@pytest.mark.parametrize("fmt", ["16bit", "nvfp4"])
+@pytest.mark.parametrize("heads,kvh,n", [(5, 1, 3), (32, 8, 1), (32, 8, 2000), (128, 2, 40)])
+def test_append_rotates_queries_in_place(b200, fmt, heads, kvh, n):
+    """q_out may be q, also inside a fused projection's rows, with one or many warps to a token: the bits of a call with an
+    output of its own."""
+    p = ref.Problem([n, 1], [n + 100, 7], heads, kvh, 128, 16, BF16, fmt, seed=69)
+    i = torch.arange(0, 128, 2, dtype=torch.float64, device="cuda")
+    f = api.from_torch((10000.0 ** (-i / 128)).float())
+    k, v = api.from_torch(p.k), api.from_torch(p.v)
+    want = torch.empty_like(p.q)
+    launch.paged_kv_append(p.cache, p.batch, k, v, q=api.from_torch(p.q), q_out=api.from_torch(want), inv_freq=f)
+    pools = [x.clone() for x in p.pools]
+    for _ in range(3):
+        rows = torch.full((p.tokens, heads + 2 * kvh, 128), 5.0, dtype=BF16, device="cuda")
+        q = rows[:, :heads]
+        q.copy_(p.q)
+        t = api.from_torch(q)
+        launch.paged_kv_append(p.cache, p.batch, k, v, q=t, q_out=t, inv_freq=f)
+        assert torch.equal(q, want) and (rows[:, heads:] == 5.0).all()
+        assert all(torch.equal(a, b) for a, b in zip(pools, p.pools))
