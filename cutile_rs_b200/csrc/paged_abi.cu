@@ -254,13 +254,20 @@ int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cach
                      !(a.q_hs % 8) && !(a.o_ts % 8) && !(a.o_hs % 8) && a.q_ts > 0 && a.q_hs > 0;
   a.tile_off = tiles ? split_bytes(cache, batch, tile_rows(cache)) : 0;
   // Prompts alone take one launch of the tile kernel; decode steps with prompts among them take both kernels, each its
-  // own sequences.  The second kernel costs 5 to 20 us (launches, merge, its CTAs in front of the tiles'); a decode step in
-  // the tile kernel costs a whole tile per 128 keys.  Beside a prompt of 512 tokens, one kernel against two: 31 steps of 256
-  // keys 39 / 44 us, 255 of them 159 / 101, over NVFP4 56 / 62 and 219 / 110; 100 steps of 4096 keys over NVFP4 491 / 217.  How
-  // many decode steps there may be follows from the sizes: as many sequences as are left when the others have max_q_len
-  // tokens each.
+  // own sequences.  The second kernel costs 2 to 20 us (launches, merge, its CTAs in front of the tiles'); a decode step in
+  // the tile kernel costs a whole tile per 128 keys and about two more to begin and end, and its probabilities get one
+  // 16-bit piece instead of two.  How many decode steps there may be follows from the sizes: as many sequences as are
+  // left when the others have max_q_len tokens each; how many keys they may have, from the table's width.
+  // Measured (us, one kernel against two, 8 K/V heads of 128, beside a prompt of 512 tokens; in brackets heads * (keys / 128 + 2)):
+  //   NVFP4   16 steps of 1024 keys (1280) 44 / 49, 31 of 1024 (2480) 62 / 55, 16 of 4096 (4352) 96 / 67, 1 of 65536 (4112)
+  //           96 / 66, 255 of 256 (8160) 197 / 90, 8 of 131072 (65664) 1115 / 407
+  //   16-bit  16 steps of 4096 keys (4352) 72 / 96, 16 of 16384 (16640) 210 / 223, 31 of 16384 (32240) 384 / 365, 8 of
+  //           131072 (65664) 766 / 726; by their number: 31 of 256 37 / 40, 64 of 256 53 / 52, 127 of 256 87 / 72
+  //   prompts alone, their lengths so uneven that some could be steps: 35 / 37 to 182 / 187, NVFP4 40 / 41 to 135 / 142
   const long long full = (tokens + (long long)batch->max_q_len - 1) / batch->max_q_len;
-  const bool only_tiles = tiles && (batch->batch - full) * cache->kv_heads <= (cache->format ? 64 : 256);
+  const long long steps = (batch->batch - full) * cache->kv_heads;
+  const long long each = (long long)batch->max_pages * cache->page_size / 128 + 2;
+  const bool only_tiles = tiles && (cache->format ? steps * each <= 1536 : steps <= 256 && steps * each <= 20480);
   a.row_limit = only_tiles ? 0 : tiles ? tile_rows(cache) : 0x7fffffff;
   if (!only_tiles)
     if (int rc = b200_paged_split_dispatch(a)) return rc;

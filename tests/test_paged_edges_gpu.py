@@ -220,6 +220,30 @@ def test_nan_on_the_way_into_nvfp4_stays_visible(b200):
         assert torch.equal(p.rows(0, 6)[1][good], q.rows(0, 6)[1][good])
 
 
+def test_decode_steps_keep_their_kernel_beside_anything(b200):
+    """Single tokens over long tables go to the kernel of few rows, which hands probabilities over in two pieces, beside a
+    prompt or under a max_q_len that allows far more tokens than there are.  Keys of two scores, whose values cancel: the
+    output is small beside the sums, so that the rounding of one piece, up to 2^-9 of them, would show."""
+    d, kv, page = 64, 4096, 64
+    for prompts, max_q in (([], 4096), ([200], None), ([200, 300], None)):
+        q_lens = [1] * 12 + prompts
+        p = ref.Problem(q_lens, [kv] * len(q_lens), 16, 8, d, page, BF16, seed=67, table_keys=ref.MANY_KEYS, max_q=max_q)
+        p.q.zero_()
+        p.q[..., 0] = 1.0
+        for pool in p.pools:
+            pool.zero_()
+        p.pools[0][:, :, ::2, 0] = 0.25                    # half of the keys score 0.25, the others 0
+        p.pools[1][:, :, ::2] = 1.0
+        p.pools[1][:, :, 1::2] = -1.28125
+        want, _ = ref.attention(p, 1.0)
+        got = _attend(p, 1.0)[:12].double()
+        want = want[:12]
+        weight = 1.15                                      # sum p |v| / sum p
+        assert want.abs().max() < 0.01
+        assert ((got - want).abs() <= 2.0 ** -9 * want.abs() + (2.0 ** -15 + 80 * 2.0 ** -24 + 4096 * 2.0 ** -24) * weight).all(), \
+            float((got - want).abs().max())
+
+
 @pytest.mark.parametrize("fmt", ["16bit", "nvfp4"])
 @pytest.mark.parametrize("heads,kvh,n", [(5, 1, 3), (32, 8, 1), (32, 8, 2000), (128, 2, 40)])
 def test_append_rotates_queries_in_place(b200, fmt, heads, kvh, n):
