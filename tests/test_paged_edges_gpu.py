@@ -264,3 +264,40 @@ def test_append_rotates_queries_in_place(b200, fmt, heads, kvh, n):
         launch.paged_kv_append(p.cache, p.batch, k, v, q=t, q_out=t, inv_freq=f)
         assert torch.equal(q, want) and (rows[:, heads:] == 5.0).all()
         assert all(torch.equal(a, b) for a, b in zip(pools, p.pools))
+
+
+def test_wide_scales_in_f16(b200):
+    """Scales over the whole of e4m3, 2^-9 to 448, with a factor that keeps the output inside f16."""
+    for keys in (0, ref.MANY_KEYS):
+        p = ref.Problem([1, 30], [70, 41], 4, 2, 64, 16, F16, "nvfp4", seed=71, table_keys=keys, v_global=2.0 ** -4)
+        for x in p.scales[1:]:
+            x.copy_(torch.randint(1, 0x7f, x.shape, device="cuda").to(torch.uint8))
+        got = _attend(p, 0.125)
+        want, tol = ref.attention(p, 0.125)
+        assert not torch.isnan(got).any() and ((got.double() - want).abs() <= tol).all()
+
+
+def _piece_bound(p, scale, rows):
+    """ref.attention's bound for tokens that the kernel of few rows takes, whatever else is in the call: probabilities in
+    two pieces, 2^-15 (one f16 piece, 2^-11, for bf16 over NVFP4)."""
+    keep = p.batch
+    p.batch = paged.PagedBatch(p.table, p.cu_q, p.kv, 1)    # the bound of a call of single tokens
+    want, tol = ref.attention(p, scale)
+    p.batch = keep
+    return want[rows], tol[rows]
+
+
+@pytest.mark.parametrize("fmt,d,dtype", FORMS + [("nvfp4", 128, F16)])
+def test_steps_beside_prompts_are_held_to_their_own_bound(b200, fmt, d, dtype):
+    """150 decode steps beside two prompts, where each kernel takes its own sequences, and short prompts behind a short
+    table, which the kernel of few rows takes alone: two pieces in both."""
+    q_lens = [1] * 150 + [130, 40]
+    kv_lens = [1 + (53 * i) % 400 for i in range(150)] + [300, 500]
+    p = ref.Problem(q_lens, kv_lens, 8, 2, d, 16, dtype, fmt, seed=72, table_keys=ref.MANY_KEYS)
+    got = _attend(p, d ** -0.5)
+    want, tol = _piece_bound(p, d ** -0.5, slice(0, 150))
+    assert ((got[:150].double() - want).abs() <= tol).all()
+    p = ref.Problem([40, 17, 1], [60, 40, 90], 8, 2, d, 16, dtype, fmt, seed=73)
+    got = _attend(p, d ** -0.5)
+    want, tol = _piece_bound(p, d ** -0.5, slice(None))
+    assert ((got.double() - want).abs() <= tol).all()
