@@ -54,13 +54,6 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* desc, uint32_t bar, int x, int y, int z, int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(dst), "l"(desc), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
@@ -69,24 +62,6 @@ __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bo
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(ok ? BYTES : 0)
                : "memory");
 }
-__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
-  uint32_t r;
-  asm("{.reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t;}" : "=r"(r) : "r"(two_bytes));
-  return r;
-}
-// The four bytes of w, two e2m1 codes each, as f16 pairs (low nibble in the low half).  One conversion instruction per
-// pair runs at 50 pairs per clock and SM against 22 for shifting the bits into place.
-__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&r)[4]) {
-  asm("{.reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4;"
-      " cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b; cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d;}"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(w));
-}
-
 constexpr int STEP = 16;             // keys per step
 // Warps per CTA, one CTA per SM.  16-bit, D = 128: 8 rings of 3 x 8 KB fill the shared memory; D = 64 halves the step and
 // takes half again as many warps.  NVFP4: what the registers allow (16 rows of 128: 8 warps 97, 12 that spill 108 us for 32 x
@@ -226,7 +201,7 @@ __device__ __forceinline__ void softmax_step(const ScoreParams (&sp)[NT][2], con
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         const float m_new = fmaxf(m_run[nt][j], mx);
-        const float alpha = m_new == m_run[nt][j] ? 1.0f : paged_ex2(m_run[nt][j] - m_new);
+        const float alpha = m_new == m_run[nt][j] ? 1.0f : ex2_approx(m_run[nt][j] - m_new);
         m_run[nt][j] = m_new;
         l_run[nt][j] *= alpha;
 #pragma unroll
@@ -245,8 +220,8 @@ __device__ __forceinline__ void softmax_step(const ScoreParams (&sp)[NT][2], con
     for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        s[ks][nt][j] = paged_ex2(s[ks][nt][j] - m_use[j]);
-        s[ks][nt][2 + j] = paged_ex2(s[ks][nt][2 + j] - m_use[j]);
+        s[ks][nt][j] = ex2_approx(s[ks][nt][j] - m_use[j]);
+        s[ks][nt][2 + j] = ex2_approx(s[ks][nt][2 + j] - m_use[j]);
         l_run[nt][j] += s[ks][nt][j] + s[ks][nt][2 + j];
       }
 #pragma unroll
@@ -814,7 +789,7 @@ fmha_paged_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_co
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float mn = fmaxf(m[j], a[j]), mu = mn == -CUDART_INF_F ? 0.0f : mn;
-          const float wa = paged_ex2(m[j] - mu), wb = paged_ex2(a[j] - mu);
+          const float wa = ex2_approx(m[j] - mu), wb = ex2_approx(a[j] - mu);
           m[j] = mn;
           l[j] = l[j] * wa + q[j] * wb;
           x[j] = x[j] * wa + vv[j] * wb;
@@ -957,7 +932,7 @@ __global__ void __launch_bounds__(256, NT == 1 ? 4 : 2) fmha_paged_merge_kernel(
     for (int j = 0; j < 2; ++j) {
       const float mn = fmaxf(m[nt][j], pm[j]);
       const float mu = mn == -CUDART_INF_F ? 0.0f : mn;
-      const float wa = paged_ex2(m[nt][j] - mu), wb = paged_ex2(pm[j] - mu);
+      const float wa = ex2_approx(m[nt][j] - mu), wb = ex2_approx(pm[j] - mu);
       m[nt][j] = mn;
       l[nt][j] = l[nt][j] * wa + plx[j] * wb;
       o[nt][j] = o[nt][j] * wa + vv[j] * wb;

@@ -26,7 +26,6 @@
 
 #include <algorithm>
 
-#include "fmha_common.cuh"
 #include "paged_common.cuh"
 
 namespace b200 {
@@ -75,13 +74,6 @@ struct TileSmem {
   static constexpr int THREADS = FP4 ? 512 : 384;
 };
 
-__device__ __forceinline__ void tma_load_4d_tile(uint32_t dst, const void* desc, uint32_t bar, int x, int y, int z, int w) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(dst), "l"(desc), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
-      : "memory");
-}
 __device__ __forceinline__ float absmax3(float a, float b, float c) {
   float d;
   asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -284,15 +276,6 @@ __device__ __forceinline__ Part make_part(const TileParams& p, const Walk& w, lo
   return x;
 }
 
-// The four bytes of w, two e2m1 codes each, as f16 pairs times a pair of equal scales: exact (two bits times four).
-__device__ __forceinline__ void expand8(uint32_t w, uint32_t scale, uint32_t (&o)[4]) {
-  asm("{.reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4;"
-      " cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b; cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d;}"
-      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]) : "r"(w));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(o[i]) : "r"(o[i]), "r"(scale));
-}
-
 template <int D, bool F16, bool CAP, bool FP4>
 __global__ void __launch_bounds__(FP4 ? 512 : 384, 1)
 fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -439,12 +422,12 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         if (!wait_all(bar_k_empty + stage * 8, phase ^ 1, 10)) { ok = false; break; }
         if (lane == 0) mbar_expect_tx(bar_k_full + stage * 8, TILE);
         __syncwarp();
-        if (half < HALVES) tma_load_4d_tile(sK + off, &tmK, bar_k_full + stage * 8, half * 64, slot, head, pg);
+        if (half < HALVES) tma_load_4d(sK + off, &tmK, bar_k_full + stage * 8, half * 64, slot, head, pg);
         ++armed_k;
         if (!wait_all(bar_v_empty + stage * 8, phase ^ 1, 11)) { ok = false; break; }
         if (lane == 0) mbar_expect_tx(bar_v_full + stage * 8, TILE);
         __syncwarp();
-        if (half < HALVES) tma_load_4d_tile(sV + off, &tmV, bar_v_full + stage * 8, half * 64, slot, head, pg);
+        if (half < HALVES) tma_load_4d(sV + off, &tmV, bar_v_full + stage * 8, half * 64, slot, head, pg);
         ++armed_v;
         pages = next;
       }
@@ -875,12 +858,14 @@ fmha_paged_tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     auto expand = [&](uint32_t dst, const uint32_t (&x)[WORDS], const uint32_t (&s)[D / 64]) {
 #pragma unroll
       for (int i = 0; i < WORDS; i += 4) {           // two scales
-        uint32_t two;
-        asm("{.reg .b16 h; cvt.u16.u32 h, %1; cvt.rn.f16x2.e4m3x2 %0, h;}" : "=r"(two) : "r"((s[i / 8] >> (4 * (i & 4))) & 0xffffu));
+        const uint32_t two = e4m3x2_to_f16x2((s[i / 8] >> (4 * (i & 4))) & 0xffffu);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
+          const uint32_t scale = __byte_perm(two, two, k < 2 ? 0x1010 : 0x3232);
           uint32_t o[4];
-          expand8(x[i + k], __byte_perm(two, two, k < 2 ? 0x1010 : 0x3232), o);
+          e2m1x8_to_f16(x[i + k], o);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = hmul2(o[e], scale);       // exact: two bits times four
           const int c = i + k;
           st_shared_v4(dst + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4), o[0], o[1], o[2], o[3]);
         }

@@ -7,6 +7,7 @@
 #include <algorithm>
 
 #include "../../include/b200tile.h"
+#include "fmha_common.cuh"
 #include "host_common.h"
 #include "sm100_ptx.cuh"
 
@@ -80,11 +81,6 @@ constexpr float CAP_SMALL_OUT = 64.0f * 1.4426950408889634f;    // cap_out up to
 constexpr float CAP_HALF_ARG = 0.5f / 1.4426950408889634f;     // t = z * this
 // A factor that underflows to 0 or overflows would make NaN of scores that are infinite, masked ones too, or 0.
 __host__ __device__ __forceinline__ float factor_in_range(float x) { return fminf(fmaxf(x, 0x1p-126f), 0x1p126f); }
-__device__ __forceinline__ float paged_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float paged_rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -100,7 +96,7 @@ __device__ __forceinline__ float paged_score_far(const ScoreParams& sp, float s)
   return s * sp.scale_log2 * fmaf(h, u, cap_poly(0));
 }
 __device__ __forceinline__ float paged_score_near(const ScoreParams& sp, float s) {
-  return fmaf(-2.0f * sp.cap_out, paged_rcp(1.0f + paged_ex2(s * sp.cap_arg)), sp.cap_out);
+  return fmaf(-2.0f * sp.cap_out, paged_rcp(1.0f + ex2_approx(s * sp.cap_arg)), sp.cap_out);
 }
 template <bool CAP>
 __device__ __forceinline__ float paged_score(const ScoreParams& sp, float s) {
@@ -115,6 +111,32 @@ __device__ __forceinline__ float paged_score(const ScoreParams& sp, float s) {
 // which is below what sums in 32 bits hold.  bf16 has f32's range.
 template <bool F16>
 __device__ constexpr float p_shift() { return F16 ? 7.0f : 0.0f; }
+
+// The four bytes of w, two e2m1 codes each, as f16 pairs (low nibble in the low half).  One conversion instruction per
+// pair runs at 50 pairs per clock and SM against 22 for shifting the bits into place.
+__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t (&r)[4]) {
+  asm("{.reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4;"
+      " cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b; cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d;}"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(w));
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes) {
+  uint32_t r;
+  asm("{.reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t;}" : "=r"(r) : "r"(two_bytes));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// A box of a page pool: {dimension, slot, head, page}.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* desc, uint32_t bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(desc), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
 
 template <bool F16>
 __device__ __forceinline__ uint32_t paged_pack16(float lo, float hi) {
