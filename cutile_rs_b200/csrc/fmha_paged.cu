@@ -5,17 +5,19 @@
 //
 // Query rows are packed per K/V head (row = token * group + head of the group) in blocks of 8 or 16, so that a K/V row
 // is read once for all heads that share it.  What bounds it is HBM: each cached byte is used for `group` rows only.
-// 8 x 65536 keys of 8 x 128: 330 us, 6.5 TB/s; 64 sequences to 8192 keys 157 us, 6.0 TB/s; launch, first copies and merge take
-// about 9 us of any call.  NVFP4 is bound by instructions, 325 a step of 16 keys, 128 of them conversions and scale
-// products: 32 sequences to 16384 keys 69 us, 3.9 TB/s.
+// 8 x 65536 keys of 8 x 128: 333 us, 6.4 TB/s; 64 sequences to 8192 keys 157 us, 6.0 TB/s; launch, first copies and merge take
+// about 9 us of any call.  NVFP4, 32 sequences to 16384 keys: 69 us, 3.9 TB/s, of 41 at the copy rate.  57 of them remain
+// without the arithmetic: 9 to start and merge, and copies of 16 bytes a lane that reach 5.6 TB/s; the arithmetic adds 12.
+// 327 instructions a step of 16 keys, 128 of them conversions and scale products, fill 59 % of the issue slots; three warps
+// a scheduler, what the registers allow, wait for one another's fixed latencies in the rest.
 //
 // Work split.  One worker is ONE WARP.  Sequence b has steps(b) steps of 16 keys, an item is (sequence, row block, K/V
 // head), and the steps of all items form one line that is cut into equal runs, one per worker.  Lengths may be as
 // uneven as they like: every warp of the machine reads the same number of bytes, whatever the batch looks like, and
 // nothing about the lengths has to be known on the host (a captured graph may be replayed with other lengths).  A run
 // that holds whole items writes their output; a run that holds part of an item writes (m, l, O) in 32 bits, at most
-// two such parts per worker, and the merge kernel adds the parts of an item in the order of the workers.  No atomics
-// and no state between launches: the same call gives the same bits.  (A run is taken by a few workers, one per head of
+// two such parts per worker, and the merge kernel adds the parts of an item in the order of the workers.  No result
+// depends on an atomic (only the status record of a bad page does) or on an earlier launch: the same call gives the same bits.  (A run is taken by a few workers, one per head of
 // `heads_abreast`: the line counts groups of heads.)
 //
 // Inside a worker the products are transposed, S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16): the 16 rows of the

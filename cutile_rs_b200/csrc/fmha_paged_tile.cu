@@ -19,9 +19,15 @@
 //     products are then f16 x f16, which holds every code * scale exactly; bf16 queries are brought to a power of two near
 //     1 row by row and converted in shared memory by the softmax threads before their first scores.
 //
-// What bounds it: as fmha_fwd.cu, the softmax threads and the tensor pipe together, 2.1 us a step of 256 x 128 (2.45 with the
-// cap, 2.6 over NVFP4), and 4 to 5 us to begin and end an item.  A prompt of 4096 tokens, 32 / 8 heads of 128: 144 us, 950
-// TFLOP/s; four chunks to 256 tokens over 5000 NVFP4 keys 51 us.
+// What bounds it: as fmha_fwd.cu, the softmax threads and the tensor pipe in turn, 2.1 us a step of 256 x 128 (2.45 with the
+// cap, 2.6 over NVFP4) where the tensor pipe alone needs 1.5, and 4 to 5 us to begin and end an item.  A prompt of 4096
+// tokens, 32 / 8 heads of 128: 144 us, 950 TFLOP/s, the tensor pipe 51 % active (163 us with all data from HBM); four chunks
+// to 256 tokens over 5000 NVFP4 keys 51 us, 29 % active.
+//
+// P is handed to the second product as ONE 16-bit value (bf16 2^-9, f16 2^-12 of each weight, at random), as in fmha_fwd.cu;
+// the row-block kernel's two pieces would double the second product, 0.75 us of tensor time a step.  Against 64 bits the
+// output's error grows from 1.6e-3 to 2.0e-3 of its norm in bf16 and from 2.1e-4 to 2.9e-4 in f16, about as much as the output's own
+// rounding.  The sums of the weights take the values before that rounding, in 32 bits.
 #include <math_constants.h>
 
 #include <algorithm>

@@ -5,11 +5,13 @@
 // for every head of Q (to q_out) and K (to its slot); V and the dimensions from r on are copied.  An NVFP4 cache takes
 // blocks of 16: scale = e4m3(max |y| / (6 g)), code = e2m1(y / (scale g)) with g the pool's factor.
 //
-// HBM-bound in 16 bits (8192 tokens, 32 + 8 heads of 128: 45 us, 5.6 TB/s), by instructions with FP4 blocks (6700 tokens: 34
-// us against 22 us of traffic; two values at a time where the machine can).
+// HBM-bound in 16 bits (8192 tokens, 32 + 8 heads of 128: 46 us, 5.5 TB/s).  With FP4 blocks 6691 tokens take 34 us against
+// 22 of traffic, 31 with angles, maxima and quotients left out: 16 warps an SM (126 registers) issue in 59 % of the cycles
+// and wait for fixed latencies and loads in the rest, DRAM 38 % busy; codes and scales leave in pieces of 4 and 1 bytes.
+// Reading 6691 tokens back takes 10 to 11 us against 5.4 of traffic: 55 % of the issue slots, the conversion pipe at 40 %.
 // Each value is read once and written once.  A warp takes a token (or a share of its heads): lane l always
-// holds the same D/16-th of a head, so its 8 cosines and sines stay in registers for all heads, and nothing but loads,
-// eight FMAs per vector and stores is left in the loop.  Angles: p * f_i reaches 1e5 and more, where a product rounded
+// holds the same D/16-th of a head, so its 8 cosines and sines stay in registers for all heads, and nothing but loads, 32
+// products and 16 sums (each rounded by itself, see the rotation) and stores is left in the loop.  Angles: p * f_i reaches 1e5 and more, where a product rounded
 // to 32 bits is off by 1e-2 radians; angle, sine and cosine are taken in 64 bits and rounded to 32 once (64 of them per
 // token against 10^4 values moved), so that the rotated value, and with it every rounding to 4 bits, does not depend
 // on how far the position is.
@@ -96,8 +98,8 @@ __device__ __noinline__ void angle_64(int pos, float inv_freq, double* s, double
   sincos((double)pos * (double)inv_freq, s, c);
 }
 
-// Quotients a / b from inv close to 1 / b: q = a inv, then one correction by its exact remainder, which leaves half a step
-// and a few millionths of one.  16-bit values meet the rounding borders of e2m1 and e4m3 exactly, where a plain product
+// Quotients a / b from inv close to 1 / b by Markstein's correction: q = a inv, then q + (a - q b) inv with the exact
+// remainder, which leaves half a step and a few millionths of one.  16-bit values meet the rounding borders of e2m1 and e4m3 exactly, where a plain product
 // with the reciprocal would miss the tie; the correction hits a quotient that 32 bits hold.  For b and a / b well inside
 // the range of f32.
 __device__ __forceinline__ float quotient(float a, float b, float inv) {

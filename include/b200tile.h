@@ -437,9 +437,15 @@ B200TILE_API int b200tile_paged_kv_gather(const char* dtype, const b200tile_page
  *   workspace  DEVICE scratch of b200tile_paged_attention_workspace_bytes(...) bytes for the same cache and batch
  *              (sizes only, not contents), 16-byte aligned; nothing in it outlives the call.  Calls that may overlap
  *              on the device must not share one, nor graphs that may be replayed at the same time
+ * Probabilities enter the second product in 16-bit pieces, their sums in 32 bits: two pieces (2^-15 of a weight or less) for
+ * sequences of few rows (tokens * q_heads / kv_heads per K/V head), one of the call's type (bf16 2^-9, f16 2^-12) for
+ * prompts and chunks, and one of f16 for bf16 rows over format 1.  Which sequences count as few goes by the sizes of the
+ * call, so the same sequence may come out with other last bits in another batch; the same call gives the same bits.
  * `out` may be `q` (the same rows); it must not overlap anything else that the call reads.  Cached rows at or behind
- * kv_lens[b] are never looked at: they may hold anything, NaN included.  A NaN or infinity in V at a key that some token of the sequence sees may also reach other tokens of the
- * same sequence in the call (it is multiplied by a probability of 0). */
+ * kv_lens[b] are never looked at: they may hold anything, NaN included.  A NaN or infinity in V at a key that some token of
+ * the sequence sees may also reach other tokens of the same sequence in the call (it is multiplied by a probability of 0),
+ * and an infinite V may come out as NaN.  A row whose scores are all -inf counts as one that sees no key; with a softcap
+ * infinite scores are +-c. */
 B200TILE_API uint64_t b200tile_paged_attention_workspace_bytes(const b200tile_paged_cache* cache,
                                                                const b200tile_paged_batch* batch, int q_heads);
 B200TILE_API int b200tile_paged_attention(const char* dtype, const b200tile_paged_cache* cache,
