@@ -930,7 +930,7 @@ def paged_kv_gather(k_out: Tensor, v_out: Tensor, cache: PagedKvCache, batch: Pa
 
 def paged_attention_workspace(cache: PagedKvCache, batch: PagedBatch, q_heads: int) -> torch.Tensor:
     """Scratch for :func:`paged_attention` on a batch of these sizes (whatever its lengths are).  Calls that may run at
-    the same time, and graphs that may be replayed at the same time, need one each."""
+    the same time, and graphs that may be replayed at the same time, need one each; a graph needs it as long as it lives."""
     need = int(_lib.load().b200tile_paged_attention_workspace_bytes(cache.c, batch.c, int(q_heads)))
     return torch.empty(max(need, 16), dtype=torch.uint8, device=cache.device)
 

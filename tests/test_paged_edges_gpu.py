@@ -301,3 +301,48 @@ def test_steps_beside_prompts_are_held_to_their_own_bound(b200, fmt, d, dtype):
     got = _attend(p, d ** -0.5)
     want, tol = _piece_bound(p, d ** -0.5, slice(None))
     assert ((got.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("fmt", ["16bit", "nvfp4"])
+@pytest.mark.parametrize("steps,prompts,kv", [(150, [130, 40], 400), (3, [200, 90], 300), (40, [], 3000)])
+def test_captured_calls_of_every_kernel_at_once(b200, fmt, steps, prompts, kv):
+    """Decode steps beside prompts, prompts alone and steps alone, several calls to a graph, two graphs replayed on two
+    streams at once with a workspace each and lengths that change between replays: the bits of eager calls."""
+    q_lens = [1] * steps + prompts
+    ps = []
+    for seed in (80, 81):
+        kv_lens = [kv - (53 * i) % (kv - 20) for i in range(steps)] + [n + 70 for n in prompts]
+        ps.append(ref.Problem(q_lens, kv_lens, 8, 2, 64, 16, BF16, fmt, seed=seed, table_keys=ref.MANY_KEYS))
+    first = [p.kv.clone() for p in ps]
+    # everything a graph points to lives as long as the graph does: beginning a capture gives cached memory back
+    spaces = [launch.paged_attention_workspace(p.cache, p.batch, 8) for p in ps]
+    outs = [[torch.zeros_like(p.q) for _ in range(3)] for p in ps]
+    streams = [torch.cuda.Stream() for _ in ps]
+    torch.cuda.synchronize()
+
+    def calls(p, ws, out, s):
+        for o, cap in zip(out, (0.0, 20.0, 1e4)):
+            launch.paged_attention(api.from_torch(o), api.from_torch(p.q), p.cache, p.batch, 0.125, softcap=cap,
+                                   workspace=ws, stream=s)
+
+    graphs = []
+    for p, ws, out, s in zip(ps, spaces, outs, streams):
+        calls(p, ws, out, s)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            calls(p, ws, out, s)
+        graphs.append(g)
+    for shorter in (0, 7, 19):
+        want = []
+        for p, lens in zip(ps, first):
+            p.kv.copy_((lens - shorter).clamp(min=1))
+            want.append([_attend(p, 0.125, softcap=cap) for cap in (0.0, 20.0, 1e4)])
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, outs):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
