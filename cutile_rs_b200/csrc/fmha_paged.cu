@@ -17,8 +17,8 @@
 // nothing about the lengths has to be known on the host (a captured graph may be replayed with other lengths).  A run
 // that holds whole items writes their output; a run that holds part of an item writes (m, l, O) in 32 bits, at most
 // two such parts per worker, and the merge kernel adds the parts of an item in the order of the workers.  No result
-// depends on an atomic (only the status record of a bad page does) or on an earlier launch: the same call gives the same bits.  (A run is taken by a few workers, one per head of
-// `heads_abreast`: the line counts groups of heads.)
+// depends on an atomic (only the status record of a bad page does) or on an earlier launch: the same call gives the same
+// bits.  (A run is taken by a few workers, one per head of `heads_abreast`: the line counts groups of heads.)
 //
 // Inside a worker the products are transposed, S^T = K Q^T and O^T = V^T P^T (mma.sync m16n8k16): the 16 rows of the
 // instruction are keys (or head dimensions) and its 8 columns the query rows, so 8 rows fill it; the usual orientation
@@ -155,9 +155,9 @@ __device__ __forceinline__ RowMask<NT> row_mask(const SplitParams& p, const SeqV
 // The online softmax of one step: s[nt] holds S^T (keys g and g + 8, rows 2t and 2t + 1 of block nt) and becomes the
 // B operand of O^T += V^T P^T.  Statistics in 32 bits.  The reference m that is subtracted from the exponents is the
 // same for all lanes of a row and moves only when some score exceeds it by more than 2^8: one vote per step instead of
-// a maximum over eight lanes.  P <= 2^(8 + p_shift) then, and l >= 1 for any row that saw a key.  P is handed over as a 16-bit value
-// plus the 16-bit rest of it (HILO): the rounding of P alone would put an error as large as the output's own rounding
-// beside it, and the second product costs nothing next to the loads.
+// a maximum over eight lanes.  P <= 2^(8 + p_shift) then, and l >= 1 for any row that saw a key.  P is handed over as a
+// 16-bit value plus the 16-bit rest of it (HILO): the rounding of P alone would put an error as large as the output's own
+// rounding beside it, and the second product costs nothing next to the loads.
 template <bool F16, int KS, int NT, int DT, bool CAP, bool HILO>
 __device__ __forceinline__ void softmax_step(const ScoreParams (&sp)[NT][2], const RowMask<NT>& rm, int key0, int lane,
                                              bool ragged, float (&s)[KS][NT][4], float (&m_run)[NT][2],
@@ -217,7 +217,8 @@ __device__ __forceinline__ void softmax_step(const ScoreParams (&sp)[NT][2], con
   for (int nt = 0; nt < NT; ++nt) {
     float m_use[2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) m_use[j] = m_run[nt][j] == -CUDART_INF_F ? 0.0f : m_run[nt][j] - p_shift<F16>();   // nothing seen yet
+    for (int j = 0; j < 2; ++j)                        // -inf: nothing seen yet
+      m_use[j] = m_run[nt][j] == -CUDART_INF_F ? 0.0f : m_run[nt][j] - p_shift<F16>();
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll

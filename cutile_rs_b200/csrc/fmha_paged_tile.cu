@@ -26,8 +26,8 @@
 //
 // P is handed to the second product as ONE 16-bit value (bf16 2^-9, f16 2^-12 of each weight, at random), as in fmha_fwd.cu;
 // the row-block kernel's two pieces would double the second product, 0.75 us of tensor time a step.  Against 64 bits the
-// output's error grows from 1.6e-3 to 2.0e-3 of its norm in bf16 and from 2.1e-4 to 2.9e-4 in f16, about as much as the output's own
-// rounding.  The sums of the weights take the values before that rounding, in 32 bits.
+// output's error grows from 1.6e-3 to 2.0e-3 of its norm in bf16 and from 2.1e-4 to 2.9e-4 in f16, by about as much as the
+// output's own rounding.  The sums of the weights take the values before that rounding, in 32 bits.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -98,8 +98,8 @@ __device__ __forceinline__ void ld_shared_v4(uint32_t src, uint32_t (&w)[4]) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(src) : "memory");
 }
 
-// Out of line: with a cap beyond CAP_SMALL_OUT and scores near it, which hardly ever meet, and the registers of both forms
-// stay out of the softmax loop (inlined, prompt chunks with a cap of 30 took 126 us instead of 122).
+// Out of line, for caps beyond CAP_SMALL_OUT with scores near them, which is rare: the registers of both forms stay out of
+// the softmax loop (inlined, prompt chunks with a cap of 30 took 126 us instead of 122).
 __device__ __noinline__ float score_any_cap(float scale, float cap_arg, float cap_out, float s) {
   return paged_score<true>(ScoreParams{scale, cap_arg, cap_out}, s);
 }

@@ -9,12 +9,12 @@
 // 22 of traffic, 31 with angles, maxima and quotients left out: 16 warps an SM (126 registers) issue in 59 % of the cycles
 // and wait for fixed latencies and loads in the rest, DRAM 38 % busy; codes and scales leave in pieces of 4 and 1 bytes.
 // Reading 6691 tokens back takes 10 to 11 us against 5.4 of traffic: 55 % of the issue slots, the conversion pipe at 40 %.
-// Each value is read once and written once.  A warp takes a token (or a share of its heads): lane l always
-// holds the same D/16-th of a head, so its 8 cosines and sines stay in registers for all heads, and nothing but loads, 32
-// products and 16 sums (each rounded by itself, see the rotation) and stores is left in the loop.  Angles: p * f_i reaches 1e5 and more, where a product rounded
-// to 32 bits is off by 1e-2 radians; angle, sine and cosine are taken in 64 bits and rounded to 32 once (64 of them per
-// token against 10^4 values moved), so that the rotated value, and with it every rounding to 4 bits, does not depend
-// on how far the position is.
+// Each value is read once and written once.  A warp takes a token (or a share of its heads): lane l always holds the same
+// D/16-th of a head, so its 8 cosines and sines stay in registers for all heads, and nothing but loads, 32 products and 16
+// sums (each rounded by itself, see the rotation) and stores is left in the loop.  Angles: p * f_i reaches 1e5 and more,
+// where a product rounded to 32 bits is off by 1e-2 radians; angle, sine and cosine are taken in 64 bits and rounded to 32
+// once (64 of them per token against 10^4 values moved), so that the rotated value, and with it every rounding to 4 bits,
+// does not depend on how far the position is.
 #include <cuda_fp4.h>
 #include <cuda_fp8.h>
 

@@ -65,7 +65,8 @@ class PagedBatch:
     """The sequences of a call, int32 on the device: ``cu_q`` [batch + 1] (token rows of sequence b:
     [cu_q[b], cu_q[b + 1])), ``kv_lens`` [batch] (cached length, the new tokens included), ``block_table``
     [batch, max_pages].  ``max_q_len`` bounds the tokens of one sequence.  The contents are read when a kernel runs: they
-    may be rewritten between calls and between replays of a captured graph."""
+    may be rewritten between calls and between replays of a captured graph.  Kernels are chosen by ``max_q_len`` and the
+    table's width: bounds that fit the step (1 for decode steps, ``table[:, :pages_in_use]``) are faster than capacities."""
 
     def __init__(self, block_table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor, max_q_len: int):
         batch = kv_lens.shape[0] if kv_lens.dim() == 1 else -1

@@ -384,8 +384,8 @@ typedef struct b200tile_paged_cache {
  *   max_q_len    upper bound of cu_q[b+1] - cu_q[b]: attention computes no more rows of a sequence
  * Which kernels run, and how the work is split, goes by sizes that the host knows: max_pages, max_q_len, batch, tokens.
  * Bounds far above what the arrays hold are right but slower: a decode step whose max_q_len allows prompts takes 1.1 to
- * 1.5 times as long, one sequence of a few hundred keys behind a table of 100000 positions 1.3 times.  Pass max_q_len = 1 (or
- * what the step has) and only as many columns of the table (max_pages, with the whole table's pitch) as can be in use.
+ * 1.5 times as long, sequences of a few hundred keys behind a table of 100000 positions 1.3 to 2 times.  Pass max_q_len = 1
+ * (or what the step has) and only as many columns of the table (max_pages, with the whole table's pitch) as can be in use.
  * Contents cannot be checked by the call; the kernels keep to the tensors whatever they find: token rows
  * outside every sequence are left as they are, positions outside [0, max_pages * page_size) are not written,
  * and a page number outside the pool is recorded as status code 4 (site = sequence, aux = page), reads as zeros and
